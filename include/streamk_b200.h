@@ -178,7 +178,7 @@ int sk_debug_set_trace(void* buf);
 /* kernel_kind: 0 = fp32 SIMT tiles (64x64x16), 1 = what sk_gemm_f16 runs for the problem
  * (single-CTA UMMA tiles, or the CTA-pair kernel over num_sms / 2 pairs: the info then
  * describes 256-row tiles), 2 = W4A16 UMMA tiles (tile_m x tile_n x 64), 3 = the CTA-pair
- * kernel with num_sms pairs.  Mirrors streamk_fp16.py:83-113 for SK_SCHED_HYBRID. */
+ * kernel with num_sms pairs, 4 = what sk_gemm_i8 runs.  Mirrors streamk_fp16.py:83-113 for SK_SCHED_HYBRID. */
 int sk_schedule(const sk_problem* p, int kernel_kind, int num_sms, sk_schedule_info* out);
 /* The same question for sk_gemm_f16_gather with n_peers peers (a link-bound gather makes the
  * library drop the 256 x 512 units and, if the schedule was left to it, run data-parallel). */
@@ -235,6 +235,28 @@ int sk_gemm_f32_noalloc(const sk_problem* p, const float* A, const float* B, flo
  * aligned, lda/ldb multiples of 8.  C need not be zeroed.                    */
 int sk_gemm_f16(const sk_problem* p, const void* A, const void* B, void* C,
                 void* ws, size_t ws_bytes, void* stream);
+
+/* C[m,n] = scale_a[m] * scale_b[n] * sum_k A[m,k] B[n,k]: 8-bit integer operands (A [M,K] and
+ * B [N,K], row-major int8, two's complement) with one fp32 scale for each row of A (token) and
+ * each row of B (output channel), 32-bit integer accumulation, fp16 result (bf16 with
+ * SK_FLAG_BF16).  The sums are exact whatever the schedule, so every schedule gives the same
+ * bits; C = ((float)sum * scale_a[m]) * scale_b[n], rounded once more to 16 bits.  Same
+ * schedules, tiles and workspace as sk_gemm_f16.  layout NT; fixup SK_FIXUP_BLOCK_REDUCE (there
+ * is no fp32 partial to add atomically: SK_ERR_ARG); lda, ldb multiples of 16, A and B 16-byte
+ * aligned; K at most SK_I8_MAX_K (the largest whose sum cannot leave 32 bits; SK_ERR_LIMIT);
+ * CTA pairs (tile_m = 256): tile_n a multiple of 32.  No counterpart in the reference.       */
+enum { SK_I8_MAX_K = 131071 };
+int sk_gemm_i8(const sk_problem* p, const void* A, const void* B, const float* scale_a, const float* scale_b,
+               void* C, void* ws, size_t ws_bytes, void* stream);
+/* Rows of fp16 (bf16 with SK_FLAG_BF16 in flags) to 8-bit integers, one scale per row: with
+ * a = max_k |X[m,k]|, scale[m] = a / 127 (fp32, one rounding) and Q[m,k] = 127 X[m,k] / a rounded
+ * to the nearest integer, halves to even (of the exact quotient, not of X / scale[m]).  A row of
+ * zeros: scale 0, Q = 0.  A row that holds a NaN or an infinity: scale NaN, Q = 0, so that a
+ * product with it is NaN.  Activations of sk_gemm_i8 (one scale per token), or its weights (one
+ * per channel).  Any pitch ldx >= K (elements) and ldq >= K (bytes); X 2-byte aligned.
+ * Elements K .. ldq of a row of Q are not written.                                            */
+int sk_quantize_i8(const void* X, int M, int K, int ldx, int flags, void* Q, int ldq, float* scale,
+                   void* stream);
 
 /* sk_gemm_f16 fused with the all-gather of an N-sharded product (the reference is a
  * single-GPU study; this is the column-sharded configuration's collective).  Every GPU of

@@ -88,6 +88,8 @@ SIGNATURES = {
     "sk_q4_bytes_ex": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "sk_prepack_q4_ex": (C.c_int, [_P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P, C.c_size_t, _P]),
     "sk_dequant_q4_ex": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, _P, C.c_int, _P]),
+    "sk_gemm_i8": (C.c_int, [C.POINTER(SkProblem), _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
+    "sk_quantize_i8": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int, _P, C.c_int, _P, _P]),
     "sk_gemm_w4a16": (C.c_int, [C.POINTER(SkProblem), _P, _P, _P, _P, C.c_size_t, _P]),
 }
 

@@ -99,6 +99,8 @@ struct SkParams {
   int fixup;               // SK_FIXUP_*
   int c_vec_ok;            // C rows can take 16-byte stores
   int out_bf16;            // 1: operands and result are bfloat16 (SK_FLAG_BF16), else fp16
+  const float* row_scale;  // 8-bit integer product: scales along kernel-space rows / cols
+  const float* col_scale;
   int drop_flag_cta;       // test hook (sk_problem.test_drop_flag_cta - 1): this CTA never publishes
                            //    its block-reduce flag; negative = off
   unsigned long long timeout_ns;
@@ -279,6 +281,19 @@ int sk_resolve_grid(const sk_problem* p, int* num_sms_out, int* device_sms_out);
 int sk_make_sched(const sk_problem* p, int kernel_kind, int num_sms, sk_schedule_info* info,
                   SkSched* s, SkPlan* plan);
 unsigned long long* sk_trace_buffer();
+
+// 8-bit integer products (sk_gemm_i8) are planned as 16-bit ones of half the K: a K step, a
+// stage and a tile then hold the same bytes, which is what the scheduler's rules go by.
+// SK_FLAG_INTERNAL_I8 marks such a problem (the table of tuned 16-bit shapes is not for it).
+constexpr int SK_FLAG_INTERNAL_I8 = 1 << 30;
+inline sk_problem sk_i8_problem(const sk_problem* p) {
+  sk_problem q = *p;
+  q.K = p->K / 2 + (p->K & 1);
+  q.lda = p->lda / 2;
+  q.ldb = p->ldb / 2;
+  q.flags |= SK_FLAG_INTERNAL_I8 | SK_FLAG_NO_TABLE;
+  return q;
+}
 void sk_resolve_auto(sk_problem* q, int kernel_kind, int num_sms);
 // What the fp16 entry point runs for a problem: SK_SCHED_AUTO resolved, the fused gather's
 // link-bound rule applied (n_peers > 0), and the kernel chosen: *kernel_kind = 1 (single-CTA

@@ -60,10 +60,34 @@ __device__ __forceinline__ __half sk_cvt1(float a, int bf16) {
   return __ushort_as_half(static_cast<unsigned short>(r & 0xFFFFu));
 }
 
+// I8: the accumulators are 32-bit integers (8-bit integer operands).  They travel through the
+// same float registers, shared memory and workspace slots as bit patterns, partial sums are
+// added as integers (exact, so every schedule gives the same bits), and the scales are applied
+// where a value is turned into its 16-bit result: (sum * scale_a) * scale_b, the sum rounded
+// once to fp32 (it has up to 31 bits) and each product once, whichever operand feeds the rows.
+template <bool I8>
+__device__ __forceinline__ float sk_acc_add(float a, float b) {
+  if constexpr (I8) return __int_as_float(__float_as_int(a) + __float_as_int(b));
+  else return a + b;
+}
+__device__ __forceinline__ float sk_scaled(const SkParams& p, float raw, float row_scale, float col_scale) {
+  const float x = __int2float_rn(__float_as_int(raw));
+  return p.transposed ? (x * col_scale) * row_scale : (x * row_scale) * col_scale;
+}
+
 // nv (<= NC) fp32 values of tile row `grow`, columns gcol0.. -> 16-bit C  (NC = 16 or 32)
-template <int NC>
+template <int NC, bool I8 = false>
 __device__ __forceinline__ void sk_store_cols(__half* __restrict__ C, const SkParams& p, int grow,
-                                              int gcol0, int nv, const float (&v)[NC]) {
+                                              int gcol0, int nv, const float (&in)[NC]) {
+  float v[NC];
+  if constexpr (I8) {
+    const float rs = __ldg(p.row_scale + grow);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) v[j] = j < nv ? sk_scaled(p, in[j], rs, __ldg(p.col_scale + gcol0 + j)) : 0.f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) v[j] = in[j];
+  }
   if (p.transposed) {
     __half* dst = C + static_cast<size_t>(gcol0) * p.ldc + grow;
 #pragma unroll
@@ -88,15 +112,23 @@ __device__ __forceinline__ void sk_store_cols(__half* __restrict__ C, const SkPa
       if (j < nv) dst[j] = sk_cvt1(v[j], p.out_bf16);
   }
 }
+template <bool I8 = false>
 __device__ __forceinline__ void sk_store_chunk1(__half* __restrict__ C, const SkParams& p, int grow,
                                                 int gcol0, int nv, const float (&v)[32]) {
-  sk_store_cols<32>(C, p, grow, gcol0, nv, v);
+  sk_store_cols<32, I8>(C, p, grow, gcol0, nv, v);
 }
 
 // Four columns (gcol..gcol+3) of tile row `grow` -> 16-bit C
+template <bool I8 = false>
 __device__ __forceinline__ void sk_store4(__half* __restrict__ C, const SkParams& p, int grow, int gcol,
                                           const float4& x) {
-  const float v[4] = {x.x, x.y, x.z, x.w};
+  float v[4] = {x.x, x.y, x.z, x.w};
+  if constexpr (I8) {
+    const float rs = __ldg(p.row_scale + grow);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v[e] = gcol + e < p.cols ? sk_scaled(p, v[e], rs, __ldg(p.col_scale + gcol + e)) : 0.f;
+  }
   if (p.transposed) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -118,10 +150,11 @@ __device__ __forceinline__ void sk_store4(__half* __restrict__ C, const SkParams
 
 // ... and, in the fused all-gather, to the same place of every peer GPU's matrix.  `peers` is a
 // compile-time null in every kernel but the gathering one, where the loop disappears.
+template <bool I8 = false>
 __device__ __forceinline__ void sk_store_chunk(__half* __restrict__ C, const SkParams& p, int grow,
                                                int gcol0, int nv, const float (&v)[32],
                                                const SkPeers* peers = nullptr) {
-  sk_store_chunk1(C, p, grow, gcol0, nv, v);
+  sk_store_chunk1<I8>(C, p, grow, gcol0, nv, v);
   if (peers != nullptr)
     for (int i = 0; i < peers->n; ++i) sk_store_chunk1(static_cast<__half*>(peers->c[i]), p, grow, gcol0, nv, v);
 }
@@ -172,7 +205,7 @@ struct SkPending {
 // are fetched at once: QC * V loads in flight per thread; the loop is bound by L2 latency, not
 // by arithmetic.  The code is kept small on purpose: it runs once per launch, from cold
 // instruction caches.
-template <int QC, int V>
+template <int QC, int V, bool I8>
 __device__ __forceinline__ void sk_reduce_items_qv(const SkParams& p, __half* __restrict__ C,
                                                    int first, int last, int rank, int r0, int c0,
                                                    int rows_valid, int valid_cols, int begin, int end,
@@ -205,19 +238,21 @@ __device__ __forceinline__ void sk_reduce_items_qv(const SkParams& p, __half* __
         if (cta + v <= last) {
 #pragma unroll
           for (int q = 0; q < QC; ++q) {
-            acc[4 * q + 0] += x[v][q].x; acc[4 * q + 1] += x[v][q].y;
-            acc[4 * q + 2] += x[v][q].z; acc[4 * q + 3] += x[v][q].w;
+            acc[4 * q + 0] = sk_acc_add<I8>(acc[4 * q + 0], x[v][q].x);
+            acc[4 * q + 1] = sk_acc_add<I8>(acc[4 * q + 1], x[v][q].y);
+            acc[4 * q + 2] = sk_acc_add<I8>(acc[4 * q + 2], x[v][q].z);
+            acc[4 * q + 3] = sk_acc_add<I8>(acc[4 * q + 3], x[v][q].w);
           }
         }
       }
     }
-    sk_store_cols<QC * 4>(C, p, r0 + row, c0 + chunk * (QC * 4), nv, acc);
+    sk_store_cols<QC * 4, I8>(C, p, r0 + row, c0 + chunk * (QC * 4), nv, acc);
   }
 }
 
 // LIGHT: 16-column items (8 loads in flight instead of 16), for kernels with many threads and
 // few registers each (the W4A16 kernel: 736 threads, 80 registers).
-template <bool LIGHT = false>
+template <bool LIGHT = false, bool I8 = false>
 __device__ __forceinline__ void sk_reduce_items(const SkParams& p, __half* __restrict__ C,
                                                 const SkPending& pd, int pid, int rank, int tid,
                                                 int nthreads, const SkPeers* peers) {
@@ -237,7 +272,7 @@ __device__ __forceinline__ void sk_reduce_items(const SkParams& p, __half* __res
   const int begin = j * L / n;
   const int end = (j + 1) * L / n;
   // The summation order (0 + p_first + p_first+1 + ...) is the same whatever the grouping.
-  sk_reduce_items_qv<QC, 2>(p, C, first, last, rank, r0, c0, rows_valid, valid_cols, begin, end, tid, nthreads);
+  sk_reduce_items_qv<QC, 2, I8>(p, C, first, last, rank, r0, c0, rows_valid, valid_cols, begin, end, tid, nthreads);
   if (peers != nullptr) {   // (called by every thread of the CTA, see sk_reduce_pending)
     __syncthreads();
     sk_copy_items_to_peers(C, p, peers, r0, c0, rows_valid, (valid_cols + 3) >> 2, QC, begin, end, tid >> 5,
@@ -248,7 +283,7 @@ __device__ __forceinline__ void sk_reduce_items(const SkParams& p, __half* __res
 // Deferred block-reduce of the (at most two) split tiles this CTA took part in (see the
 // header comment).  Called by EVERY thread of the CTA after all roles have finished;
 // pend[0] is the tile the CTA started, pend[1] the tile it continued; ok[] is scratch.
-template <bool LIGHT = false>
+template <bool LIGHT = false, bool I8 = false>
 __device__ __forceinline__ void sk_reduce_pending(const SkParams& p, __half* __restrict__ C, int pid,
                                                   int rank, const SkPending* pend,
                                                   volatile uint32_t* ok, const SkPeers* peers = nullptr) {
@@ -282,12 +317,12 @@ __device__ __forceinline__ void sk_reduce_pending(const SkParams& p, __half* __r
     const int half = (nthreads >> 6) << 5;        // whole warps
     const int t = tid < half ? 0 : 1;
     if (ok[t] != 0u)
-      sk_reduce_items<LIGHT>(p, C, pend[t], pid, rank, t ? tid - half : tid, t ? nthreads - half : half, peers);
+      sk_reduce_items<LIGHT, I8>(p, C, pend[t], pid, rank, t ? tid - half : tid, t ? nthreads - half : half, peers);
     if (tid == 0) { sk_trace(p, 9); sk_trace(p, 10); }
   } else {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      if (pend[t].tile >= 0 && ok[t] != 0u) sk_reduce_items<LIGHT>(p, C, pend[t], pid, rank, tid, nthreads, peers);
+      if (pend[t].tile >= 0 && ok[t] != 0u) sk_reduce_items<LIGHT, I8>(p, C, pend[t], pid, rank, tid, nthreads, peers);
       if (tid == 0) sk_trace(p, 9 + t);
     }
   }
@@ -321,6 +356,7 @@ __device__ __forceinline__ bool sk_second_acc_used(const SkParams& p, int k0, in
 
 // 32 accumulator columns of this thread's row; with b_off != 0 the sum of the two accumulators
 // that two MMA-issuing threads filled (sk_gemm_f16.cu).
+template <bool I8 = false>
 __device__ __forceinline__ void sk_load_acc(uint32_t taddr, uint32_t b_off, float (&v)[32]) {
   using namespace skptx;
   uint32_t r[32];
@@ -332,7 +368,7 @@ __device__ __forceinline__ void sk_load_acc(uint32_t taddr, uint32_t b_off, floa
     tmem_ld_32x32(taddr + b_off, r);
     tmem_ld_wait();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
+    for (int j = 0; j < 32; ++j) v[j] = sk_acc_add<I8>(v[j], __uint_as_float(r[j]));
   }
 }
 
@@ -354,7 +390,7 @@ constexpr int SK_CSTAGE_BYTES = 4 * 2 * 4096;
 // groups g_first, g_first + g_step, ... (the warps that share a TMEM lane quadrant split the
 // columns).  NBUF: staging buffers per warp.  Returns the number of columns the warps handle
 // together (a multiple of 64; the rest of the tile goes through sk_store_chunk).
-template <int NBUF = 2>
+template <int NBUF = 2, bool I8 = false>
 __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtensorMap* tmC, uint32_t cstage,
                                                  int warp_slot, int lane, uint32_t t_addr, uint32_t b_off,
                                                  int grow0, int gcol0, int valid_cols, uint32_t& groups,
@@ -362,6 +398,8 @@ __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtens
                                                  int g_step = 1) {
   using namespace skptx;
   const int full = valid_cols >> 6;
+  float rs = 0.f;
+  if constexpr (I8) rs = grow0 + lane < p.rows ? __ldg(p.row_scale + grow0 + lane) : 0.f;   // (rows past the end are clipped)
   for (int g = g_first; g < full; g += g_step, ++groups) {
     const uint32_t buf = cstage + static_cast<uint32_t>(warp_slot * NBUF + (NBUF == 2 ? (groups & 1u) : 0u)) * 4096u;
     // the store issued from this buffer NBUF groups ago must have read it
@@ -382,7 +420,11 @@ __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtens
         tmem_ld_32x32(t_addr + b_off + g * 64 + h * 32, r2);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r2[j]);
+        for (int j = 0; j < 32; ++j) v[j] = sk_acc_add<I8>(v[j], __uint_as_float(r2[j]));
+      }
+      if constexpr (I8) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = sk_scaled(p, v[j], rs, __ldg(p.col_scale + gcol0 + g * 64 + h * 32 + j));
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -446,7 +488,7 @@ __device__ __forceinline__ void sk_store_tile_tma_f32(const CUtensorMap* tm, uin
 
 // FOLD: items the atomic fixup's last arriver fetches per thread and pass (2 = 16 loads in
 // flight; 1 for kernels whose threads have few registers).
-template <int MODE = SK_EPI_ANY, int EPI_WARPS = 4, int FOLD = (EPI_WARPS == 4 ? 2 : 1)>
+template <int MODE = SK_EPI_ANY, int EPI_WARPS = 4, int FOLD = (EPI_WARPS == 4 ? 2 : 1), bool I8 = false>
 __device__ __forceinline__ void sk_epilogue_loop(const SkParams& p, __half* __restrict__ C, int pid,
                                                  int rank, int warp, int lane, uint32_t tmem_base,
                                                  uint32_t tmem_full_bar, uint32_t tmem_empty_bar,
@@ -512,18 +554,18 @@ __device__ __forceinline__ void sk_epilogue_loop(const SkParams& p, __half* __re
     const bool two = sk_second_acc_used(p, seg.k0, seg.k1);
     int c_first = 0;   // first 32-column chunk that still has to go through the register path
     if (whole && p.c_tma && cstage != 0 && warp_ok && !dead)
-      c_first = sk_store_tile_tma<NBUF>(p, tmC, cstage, warp - 2, lane, t_addr, two ? p.acc_b_off : 0,
+      c_first = sk_store_tile_tma<NBUF, I8>(p, tmC, cstage, warp - 2, lane, t_addr, two ? p.acc_b_off : 0,
                                         r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB) >> 5;
     if (warp_ok && !dead) {
       for (int c = c_first + sub; c < nchunks; c += NSUB) {
         float v[32];
-        sk_load_acc(t_addr + c * 32, two ? p.acc_b_off : 0, v);
+        sk_load_acc<I8>(t_addr + c * 32, two ? p.acc_b_off : 0, v);
         if (!row_ok) continue;
         int nv = valid_cols - c * 32;
         if (nv > 32) nv = 32;
         if (whole) {
-          sk_store_chunk(C, p, grow, c0 + c * 32, nv, v, peers);
-        } else if (atomic) {
+          sk_store_chunk<I8>(C, p, grow, c0 + c * 32, nv, v, peers);
+        } else if (atomic) {   // (fp32 sums only: integer partials take the block reduction)
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             if (4 * j < nv)
@@ -661,6 +703,7 @@ __host__ __device__ __forceinline__ int sk_cluster_recv_bytes(int bn, int split)
 // iterations (an empty one contributes zeros).  recv_bar: this CTA's mbarrier, initialised with
 // five arrivals (one per epilogue warp here, one with the expected byte count).
 // Chunks are sent as soon as they are staged, so one travels while the next is being staged.
+template <bool I8 = false>
 __device__ __forceinline__ void sk_cluster_send(const SkParams& p, int rank, int warp, int lane,
                                                 uint32_t tmem_base, uint32_t tmem_full_bar,
                                                 uint32_t stage_base, uint32_t recv_base,
@@ -703,7 +746,7 @@ __device__ __forceinline__ void sk_cluster_send(const SkParams& p, int rank, int
       for (int qq = q0; qq < q1; qq += 8) {
         float v[32];
         if (live) {
-          sk_load_acc(t_addr + 4 * qq, b_off, v);
+          sk_load_acc<I8>(t_addr + 4 * qq, b_off, v);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = 0.f;
@@ -738,7 +781,7 @@ __device__ __forceinline__ void sk_cluster_send(const SkParams& p, int rank, int
   for (int c = 0; c < p.bn; c += 32) {
     float v[32];
     if (live) {
-      sk_load_acc(t_addr + c, b_off, v);
+      sk_load_acc<I8>(t_addr + c, b_off, v);
     } else {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = 0.f;
@@ -776,7 +819,7 @@ __device__ __forceinline__ void sk_cluster_send(const SkParams& p, int rank, int
 }
 
 // Step 3; runs on every thread of the CTA once its receive mbarrier has completed.
-template <int S>
+template <int S, bool I8>
 __device__ __forceinline__ void sk_cluster_reduce_s(const SkParams& p, __half* __restrict__ C, int tile,
                                                     int rank, uint32_t recv_base) {
   using namespace skptx;
@@ -809,16 +852,20 @@ __device__ __forceinline__ void sk_cluster_reduce_s(const SkParams& p, __half* _
     for (int snd = 0; snd < S; ++snd) x[snd] = ld_shared_v4(a + snd * chunk_bytes);
     float4 acc = x[0];
 #pragma unroll
-    for (int snd = 1; snd < S; ++snd) { acc.x += x[snd].x; acc.y += x[snd].y; acc.z += x[snd].z; acc.w += x[snd].w; }
-    sk_store4(C, p, r0 + row, gcol0 + lq * 4, acc);
+    for (int snd = 1; snd < S; ++snd) {
+      acc.x = sk_acc_add<I8>(acc.x, x[snd].x); acc.y = sk_acc_add<I8>(acc.y, x[snd].y);
+      acc.z = sk_acc_add<I8>(acc.z, x[snd].z); acc.w = sk_acc_add<I8>(acc.w, x[snd].w);
+    }
+    sk_store4<I8>(C, p, r0 + row, gcol0 + lq * 4, acc);
   }
 }
 
+template <bool I8 = false>
 __device__ __forceinline__ void sk_cluster_reduce(const SkParams& p, __half* __restrict__ C, int tile,
                                                   int rank, uint32_t recv_base) {
   switch (p.sched.split) {
-    case 2: sk_cluster_reduce_s<2>(p, C, tile, rank, recv_base); break;
-    case 4: sk_cluster_reduce_s<4>(p, C, tile, rank, recv_base); break;
-    default: sk_cluster_reduce_s<8>(p, C, tile, rank, recv_base); break;
+    case 2: sk_cluster_reduce_s<2, I8>(p, C, tile, rank, recv_base); break;
+    case 4: sk_cluster_reduce_s<4, I8>(p, C, tile, rank, recv_base); break;
+    default: sk_cluster_reduce_s<8, I8>(p, C, tile, rank, recv_base); break;
   }
 }

@@ -52,6 +52,7 @@ static_assert(sizeof(Ctrl) <= CTRL_BYTES, "Ctrl must fit its reserved space");
 __device__ __forceinline__ void load_operand(int loader, uint32_t dst, const CUtensorMap* tm,
                                              const void* img, uint32_t bar, int first_row, int k,
                                              int tile_rows, int kblocks) {
+  // (16-bit operands only: 8-bit integers are always K-major)
   if (loader == SK_LOAD_TMA_K) {
     tma_load_2d(dst, tm, bar, k * BK, first_row);
   } else if (loader == SK_LOAD_TMA_MN) {
@@ -74,7 +75,11 @@ __device__ __forceinline__ void load_operand(int loader, uint32_t dst, const CUt
 // is a miss.
 constexpr int SK_MODE_CLUSTER = 3;   // besides SK_EPI_ATOMIC, SK_EPI_BLOCK_REDUCE, SK_EPI_WHOLE
 
-template <int MODE>
+// I8: the operands are 8-bit integers (sk_gemm_i8).  A K step is the same 128 bytes of a row, i.e.
+// 128 of K instead of 64, in four UMMAs of 32; descriptors, stages and barriers do not change,
+// and the tensor cores take the four instructions in the same time, so the bytes an SM can load
+// bound it at the same tile shapes.  The accumulators are 32-bit integers (sk_epilogue.cuh).
+template <int MODE, bool I8>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_constant__ CUtensorMap tmCol,
                    const __grid_constant__ CUtensorMap tmC, __half* __restrict__ C, const SkParams p) {
@@ -98,6 +103,7 @@ sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_const
   // instantiation keeps the plain form and single-lane loops: with the uniform form the W4A16
   // kernel's cluster start-up barrier never completed (cause not found by reading).
   constexpr bool clustered = MODE == SK_MODE_CLUSTER;
+  constexpr int XK = I8 ? 2 * BK : BK;   // elements of K per step (the tensor maps count elements)
   const int warp = clustered ? static_cast<int>(threadIdx.x >> 5) : uniform_warp_idx();
   const int lane = threadIdx.x & 31;
   const int pid = blockIdx.x;
@@ -164,7 +170,7 @@ sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_const
       int n = seg.k1 - seg.k0;
       if (n > STAGES * G) n = STAGES * G;
       if (n > p.prefetch_steps) n = p.prefetch_steps;
-      for (int j = 0; j < n; ++j) tma_prefetch_2d(tm, (seg.k0 + j) * BK, first_row);
+      for (int j = 0; j < n; ++j) tma_prefetch_2d(tm, (seg.k0 + j) * XK, first_row);
     }
   }
   uint32_t tmem_base = 0;
@@ -224,7 +230,7 @@ sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_const
             if (is_row) mbar_arrive_expect_tx(full, n * tx);
             for (int j = 0; j < n; ++j) {
               const uint32_t dst = dst0 + (stage * G + j) * stage_bytes;
-              if (loader == SK_LOAD_TMA_K) tma_load_2d(dst, tm, full, (k + j) * BK, first_row);
+              if (I8 || loader == SK_LOAD_TMA_K) tma_load_2d(dst, tm, full, (k + j) * XK, first_row);
               else load_operand(loader, dst, tm, img, full, first_row, k + j, tile_rows, s.iters_per_tile);
             }
           }
@@ -311,9 +317,11 @@ sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_const
             const uint32_t b_lo = col_lo0 + (stage * G + j) * col_stage16;
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
-              if (leader)
-                umma_f16_ss(d_tmem, row_hi | (a_lo + kk * row_kstep16), col_hi | (b_lo + kk * col_kstep16),
-                            idesc, accumulate);
+              if (leader) {
+                const uint64_t da = row_hi | (a_lo + kk * row_kstep16), db = col_hi | (b_lo + kk * col_kstep16);
+                if constexpr (I8) umma_i8_ss(d_tmem, da, db, idesc, accumulate);
+                else umma_f16_ss(d_tmem, da, db, idesc, accumulate);
+              }
               accumulate = 1u;
             }
           }
@@ -339,12 +347,12 @@ sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_const
   } else if (warp >= 2 && warp < 6) {
     // ------------------------------------------------------------- epilogue
     if constexpr (clustered)   // (takes part in the cluster's start-up barrier on its own)
-      sk_cluster_send(p, static_cast<int>(cluster_ctarank()), warp, lane, tmem_base,
+      sk_cluster_send<I8>(p, static_cast<int>(cluster_ctarank()), warp, lane, tmem_base,
                       smem_u32(&ctrl->tmem_full[0]), sRow, recv_base, smem_u32(&ctrl->recv_full),
                       abort_flag, sk_cta_begin(s, pid) % s.iters_per_tile,
                       sk_cta_begin(s, pid + 1) - sk_cta_begin(s, pid));
     else
-      sk_epilogue_loop<MODE>(p, C, pid, 0, warp, lane, tmem_base, smem_u32(&ctrl->tmem_full[0]),
+      sk_epilogue_loop<MODE, 4, 2, I8>(p, C, pid, 0, warp, lane, tmem_base, smem_u32(&ctrl->tmem_full[0]),
                              smem_u32(&ctrl->tmem_empty[0]), &ctrl->bcast, abort_flag, ctrl->pend, &tmC,
                              p.c_tma ? smem_u32(ctrl) + 1024u : 0u);   // staging behind the control block
   }
@@ -379,13 +387,13 @@ sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_const
   }
   if constexpr (clustered) {
     if (reduce_ok)
-      sk_cluster_reduce(p, C, pid >> s.split_log2, static_cast<int>(cluster_ctarank()), recv_base);
+      sk_cluster_reduce<I8>(p, C, pid >> s.split_log2, static_cast<int>(cluster_ctarank()), recv_base);
     if (threadIdx.x == 0) sk_trace(p, 12);
     cluster_wait();
   } else {
     // Block-reduce fixup: every thread of the CTA now helps to reduce this CTA's slices of
     // the split tiles it took part in.
-    if constexpr (MODE == SK_EPI_BLOCK_REDUCE) sk_reduce_pending(p, C, pid, 0, ctrl->pend, ctrl->ok);
+    if constexpr (MODE == SK_EPI_BLOCK_REDUCE) sk_reduce_pending<false, I8>(p, C, pid, 0, ctrl->pend, ctrl->ok);
   }
   if (threadIdx.x == 32) sk_trace(p, 7);
 }
@@ -428,6 +436,22 @@ int sk_make_tmap_f16(CUtensorMap* out, const void* base, uint64_t rows, uint64_t
   return SK_OK;
 }
 
+// The same over 8-bit integers: boxes of 128 of K (128 bytes) by box_rows rows.
+int sk_make_tmap_i8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
+                    uint32_t box_rows) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) return SK_ERR_LAUNCH;
+  cuuint64_t gdim[2] = {cols, rows};
+  cuuint64_t gstride[1] = {ld_bytes};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), gdim, gstride, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return sk_set_driver_error(static_cast<int>(r));
+  return SK_OK;
+}
+
 // Fields of SkParams that depend only on the tile width: TMEM layout and pipeline depth.
 void sk_fill_tile_params(SkParams* p, int bn, int stage_fixed_bytes, int max_stages,
                          int reserved_bytes, bool two_issuers) {
@@ -447,11 +471,16 @@ void sk_fill_tile_params(SkParams* p, int bn, int stage_fixed_bytes, int max_sta
 }
 
 int sk_launch_f16_2cta(const sk_problem* prob, const void* A, const void* B, void* C, SkParams* p,
-                       void* const* peer_c, int n_peers, void* stream);
+                       void* const* peer_c, int n_peers, int k_i8, void* stream);
 
+// scale_a != NULL: the 8-bit integer product; prob then counts A and B in pairs of elements (K, lda
+// and ldb halved: 16-bit units, so that every size-in-bytes rule below and in the scheduler holds
+// as it stands), and k_elems is the true K.
 static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* C, void* const* peer_c,
-                    int n_peers, void* ws, size_t ws_bytes, void* stream) {
+                    int n_peers, void* ws, size_t ws_bytes, void* stream, const float* scale_a = nullptr,
+                    const float* scale_b = nullptr, int k_elems = 0) {
   if (!prob || !A || !B || !C) return SK_ERR_ARG;
+  const bool i8 = scale_a != nullptr;
   if (prob->layout < SK_LAYOUT_NN || prob->layout > SK_LAYOUT_LADDER) return SK_ERR_ARG;
   if (prob->fixup != SK_FIXUP_ATOMIC && prob->fixup != SK_FIXUP_BLOCK_REDUCE) return SK_ERR_ARG;
   int num_sms = 0, dev_sms = 0;
@@ -492,7 +521,7 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
   if (!ws || ws_bytes < sk_ws_total_bytes(dev_sms)) return SK_ERR_WORKSPACE;
   if ((reinterpret_cast<uintptr_t>(ws) & 255u) != 0) return SK_ERR_ALIGN;
   if (prob->schedule == SK_SCHED_GEMV) {   // small M: the CUDA-core path (sk_gemv.cu)
-    if (n_peers != 0) return SK_ERR_SHAPE;
+    if (n_peers != 0 || i8) return SK_ERR_SHAPE;
     return sk_launch_gemv_f16(prob, A, B, C, sk_ws_carve(ws, dev_sms), num_sms, dev_sms, stream);
   }
 
@@ -510,9 +539,15 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
                                              : 2000000ULL) * 1000ULL;
   p.ws = sk_ws_carve(ws, dev_sms);  // layout fixed per device, whatever the grid
   p.trace = sk_trace_buffer();
+  if (i8) {
+    p.row_scale = plan.swap ? scale_b : scale_a;
+    p.col_scale = plan.swap ? scale_a : scale_b;
+  }
   if (pairs) {
     p.bn = plan.bn;
-    return sk_launch_f16_2cta(prob, A, B, C, &p, peer_c, n_peers, stream);
+    // (kind::i8 over a CTA pair: the UMMA N dimension comes in steps of 32)
+    if (i8 && (plan.bn & 31) != 0) return SK_ERR_ARG;
+    return sk_launch_f16_2cta(prob, A, B, C, &p, peer_c, n_peers, k_elems, stream);
   }
   if (n_peers > 0) return SK_ERR_SHAPE;   // the fused all-gather lives in the CTA-pair kernel
   const int split = p.sched.split;   // SK_SCHED_CLUSTER: CTAs per tile
@@ -543,14 +578,19 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
   memset(&tmRow, 0, sizeof(tmRow));
   memset(&tmCol, 0, sizeof(tmCol));
   auto weight_map = [&](CUtensorMap* tm, int tile_rows) -> int {
+    if (i8) return sk_make_tmap_i8(tm, B, N, k_elems, 2 * static_cast<uint64_t>(prob->ldb), tile_rows);
     if (layout == SK_LAYOUT_NT) return sk_make_tmap_f16(tm, B, N, K, prob->ldb, BK, tile_rows);
     if (layout == SK_LAYOUT_NN) return sk_make_tmap_f16(tm, B, K, N, prob->ldb, 64, BK);
     return SK_OK;
   };
+  auto token_map = [&](CUtensorMap* tm, int tile_rows) -> int {
+    if (i8) return sk_make_tmap_i8(tm, A, M, k_elems, 2 * static_cast<uint64_t>(prob->lda), tile_rows);
+    return sk_make_tmap_f16(tm, A, M, K, prob->lda, BK, tile_rows);
+  };
   if (!plan.swap) {
     p.row_loader = SK_LOAD_TMA_K;
     p.col_loader = w_loader;
-    st = sk_make_tmap_f16(&tmRow, A, M, K, prob->lda, BK, plan.bm);
+    st = token_map(&tmRow, plan.bm);
     if (st == SK_OK) st = weight_map(&tmCol, plan.bn);
     p.col_img = B;
     if (w_loader != SK_LOAD_TMA_K && (plan.bn % 128) != 0) return SK_ERR_ARG;
@@ -558,7 +598,7 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
     p.row_loader = w_loader;
     p.col_loader = SK_LOAD_TMA_K;
     st = weight_map(&tmRow, plan.bm);
-    if (st == SK_OK) st = sk_make_tmap_f16(&tmCol, A, M, K, prob->lda, BK, plan.bn);
+    if (st == SK_OK) st = token_map(&tmCol, plan.bn);
     p.row_img = B;
   }
   if (st != SK_OK) return st;
@@ -570,7 +610,8 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
   }
   p.row_tx_bytes = plan.bm * BK * 2;   // the TMA box of the M-side operand has plan.bm rows
   p.col_tx_bytes = p.col_stage_bytes;
-  p.idesc = umma_idesc_f16(BM, plan.bn, 0, p.out_bf16) |
+  p.idesc = i8 ? umma_idesc_i8(BM, plan.bn) :
+            umma_idesc_f16(BM, plan.bn, 0, p.out_bf16) |
             (p.row_loader == SK_LOAD_TMA_MN ? (1u << 15) : 0u) |
             (p.col_loader == SK_LOAD_TMA_MN ? (1u << 16) : 0u);
 
@@ -586,12 +627,15 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
   static SkPerDeviceOnce attrs;
   cudaError_t e = attrs.run([]() {
     cudaError_t r = cudaSuccess;
-    const void* kernels[4] = {
-        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_EPI_ATOMIC>),
-        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_EPI_BLOCK_REDUCE>),
-        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_EPI_WHOLE>),
-        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_MODE_CLUSTER>)};
-    for (int i = 0; i < 4 && r == cudaSuccess; ++i)
+    const void* kernels[7] = {
+        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_EPI_ATOMIC, false>),
+        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_EPI_BLOCK_REDUCE, false>),
+        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_EPI_WHOLE, false>),
+        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_MODE_CLUSTER, false>),
+        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_EPI_BLOCK_REDUCE, true>),
+        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_EPI_WHOLE, true>),
+        reinterpret_cast<const void*>(sk_gemm_f16_kernel<SK_MODE_CLUSTER, true>)};
+    for (int i = 0; i < 7 && r == cudaSuccess; ++i)
       r = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
     return r;
   });
@@ -599,17 +643,26 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   __half* Ch = static_cast<__half*>(C);
   const bool pdl = (prob->flags & SK_FLAG_PDL) != 0;
-  if (split)
-    e = sk_launch(sk_gemm_f16_kernel<SK_MODE_CLUSTER>, p.sched.grid, NUM_THREADS, smem_bytes, cs, split, pdl,
+  if (i8 && split)
+    e = sk_launch(sk_gemm_f16_kernel<SK_MODE_CLUSTER, true>, p.sched.grid, NUM_THREADS, smem_bytes, cs, split, pdl,
+                  tmRow, tmCol, tmC, Ch, p);
+  else if (i8 && prob->schedule == SK_SCHED_DP)
+    e = sk_launch(sk_gemm_f16_kernel<SK_EPI_WHOLE, true>, p.sched.grid, NUM_THREADS, smem_bytes, cs, 1, pdl,
+                  tmRow, tmCol, tmC, Ch, p);
+  else if (i8)
+    e = sk_launch(sk_gemm_f16_kernel<SK_EPI_BLOCK_REDUCE, true>, p.sched.grid, NUM_THREADS, smem_bytes, cs, 1, pdl,
+                  tmRow, tmCol, tmC, Ch, p);
+  else if (split)
+    e = sk_launch(sk_gemm_f16_kernel<SK_MODE_CLUSTER, false>, p.sched.grid, NUM_THREADS, smem_bytes, cs, split, pdl,
                   tmRow, tmCol, tmC, Ch, p);
   else if (prob->schedule == SK_SCHED_DP)   // whole tiles only: no fixup code
-    e = sk_launch(sk_gemm_f16_kernel<SK_EPI_WHOLE>, p.sched.grid, NUM_THREADS, smem_bytes, cs, 1, pdl,
+    e = sk_launch(sk_gemm_f16_kernel<SK_EPI_WHOLE, false>, p.sched.grid, NUM_THREADS, smem_bytes, cs, 1, pdl,
                   tmRow, tmCol, tmC, Ch, p);
   else if (prob->fixup == SK_FIXUP_ATOMIC)
-    e = sk_launch(sk_gemm_f16_kernel<SK_EPI_ATOMIC>, p.sched.grid, NUM_THREADS, smem_bytes, cs, 1, pdl,
+    e = sk_launch(sk_gemm_f16_kernel<SK_EPI_ATOMIC, false>, p.sched.grid, NUM_THREADS, smem_bytes, cs, 1, pdl,
                   tmRow, tmCol, tmC, Ch, p);
   else
-    e = sk_launch(sk_gemm_f16_kernel<SK_EPI_BLOCK_REDUCE>, p.sched.grid, NUM_THREADS, smem_bytes, cs, 1, pdl,
+    e = sk_launch(sk_gemm_f16_kernel<SK_EPI_BLOCK_REDUCE, false>, p.sched.grid, NUM_THREADS, smem_bytes, cs, 1, pdl,
                   tmRow, tmCol, tmC, Ch, p);
   if (e != cudaSuccess) return sk_set_cuda_error(e);
   return SK_OK;
@@ -618,6 +671,18 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
 extern "C" int sk_gemm_f16(const sk_problem* prob, const void* A, const void* B, void* C, void* ws,
                            size_t ws_bytes, void* stream) {
   return gemm_f16(prob, A, B, C, nullptr, 0, ws, ws_bytes, stream);
+}
+
+extern "C" int sk_gemm_i8(const sk_problem* prob, const void* A, const void* B, const float* scale_a,
+                          const float* scale_b, void* C, void* ws, size_t ws_bytes, void* stream) {
+  if (!prob || !scale_a || !scale_b) return SK_ERR_ARG;
+  if (prob->layout != SK_LAYOUT_NT || prob->fixup != SK_FIXUP_BLOCK_REDUCE) return SK_ERR_ARG;
+  if (prob->M <= 0 || prob->N <= 0 || prob->K <= 0 || prob->lda < prob->K || prob->ldb < prob->K) return SK_ERR_SHAPE;
+  if (prob->K > SK_I8_MAX_K) return SK_ERR_LIMIT;
+  if ((prob->lda & 15) != 0 || (prob->ldb & 15) != 0) return SK_ERR_ALIGN;
+  if (((reinterpret_cast<uintptr_t>(scale_a) | reinterpret_cast<uintptr_t>(scale_b)) & 3u) != 0) return SK_ERR_ALIGN;
+  const sk_problem half = sk_i8_problem(prob);
+  return gemm_f16(&half, A, B, C, nullptr, 0, ws, ws_bytes, stream, scale_a, scale_b, prob->K);
 }
 
 extern "C" int sk_gemm_f16_scatter(const sk_problem* prob, const void* A, const void* B, void* const* dst,

@@ -64,12 +64,18 @@ static_assert(sizeof(Ctrl) <= CTRL_BYTES, "Ctrl must fit its reserved space");
 // GPU that owns its column block, and nothing is written to C.
 constexpr int OUT_PLAIN = 0, OUT_GATHER = 1, OUT_SCATTER = 2;
 
-template <int OUT>
+// I8: 8-bit integer operands, 32-bit integer accumulators (see sk_gemm_f16.cu); OUT_PLAIN only.
+template <int OUT, bool I8 = false>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmC, __half* __restrict__ C, const SkParams p,
                         const __grid_constant__ SkPeers peer_set) {
   constexpr bool PEERS = OUT == OUT_GATHER;
+  constexpr int XK = I8 ? 2 * BK : BK;   // elements of K per step
+  auto umma = [](uint32_t d, uint64_t da, uint64_t db, uint32_t id, uint32_t acc) {
+    if constexpr (I8) umma_i8_ss_pair(d, da, db, id, acc);
+    else umma_f16_ss_pair(d, da, db, id, acc);
+  };
   const SkPeers* peers = PEERS ? &peer_set : nullptr;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -154,8 +160,8 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           const uint32_t full_leader = full0_leader + 8u * stage;
           if (rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, n * 2 * (A_STAGE_BYTES + p.col_tx_bytes));
           for (int j = 0; j < n; ++j) {
-            tma_load_2d_pair(sA + (stage * KG + j) * A_STAGE_BYTES, &tmA, full_leader, (k + j) * BK, a_row0);
-            tma_load_2d_pair(sB + (stage * KG + j) * B_STAGE_BYTES, &tmB, full_leader, (k + j) * BK, b_row0);
+            tma_load_2d_pair(sA + (stage * KG + j) * A_STAGE_BYTES, &tmA, full_leader, (k + j) * XK, a_row0);
+            tma_load_2d_pair(sB + (stage * KG + j) * B_STAGE_BYTES, &tmB, full_leader, (k + j) * XK, b_row0);
           }
           k += n;
           if (++stage == STAGES) { stage = 0; ph ^= 1u; }
@@ -185,9 +191,9 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             const uint32_t dst = base + ws * W_STAGE_BYTES;
             const uint32_t full_leader = fullw0_leader + 8u * ws;
             if (rank == 0) mbar_arrive_expect_tx(fullw0 + 8u * ws, 2 * W_STAGE_BYTES);
-            tma_load_2d_pair(dst, &tmA, full_leader, k * BK, a_row0);
-            tma_load_2d_pair(dst + A_STAGE_BYTES, &tmB, full_leader, k * BK, b_row0);
-            tma_load_2d_pair(dst + A_STAGE_BYTES + B_STAGE_BYTES, &tmB, full_leader, k * BK, b_row0 + BN);
+            tma_load_2d_pair(dst, &tmA, full_leader, k * XK, a_row0);
+            tma_load_2d_pair(dst + A_STAGE_BYTES, &tmB, full_leader, k * XK, b_row0);
+            tma_load_2d_pair(dst + A_STAGE_BYTES + B_STAGE_BYTES, &tmB, full_leader, k * XK, b_row0 + BN);
             if (++ws == WSTAGES) { ws = 0; wph ^= 1u; }
           }
         }
@@ -228,7 +234,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             const uint32_t b_lo = b_lo0 + (stage * KG + j) * (B_STAGE_BYTES >> 4);
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
-              umma_f16_ss_pair(d_tmem, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc, accumulate);
+              umma(d_tmem, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc, accumulate);
               accumulate = 1u;
             }
           }
@@ -281,7 +287,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
               const uint32_t b_lo = a_lo + (A_STAGE_BYTES >> 4);
 #pragma unroll
               for (int kk = 0; kk < BK / 16; ++kk)
-                umma_f16_ss_pair(d0, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc,
+                umma(d0, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc,
                                  (k0 | kk) ? 1u : 0u);
               ++k0;
               if (++ws == WSTAGES) { ws = 0; wph ^= 1u; }
@@ -304,7 +310,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
               const uint32_t b_lo = a_lo + ((A_STAGE_BYTES + B_STAGE_BYTES) >> 4);
 #pragma unroll
               for (int kk = 0; kk < BK / 16; ++kk)
-                umma_f16_ss_pair(d1, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc,
+                umma(d1, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc,
                                  (k1 | kk) ? 1u : 0u);
               umma_commit_pair(emptyw0 + 8u * ws1);   // both halves have read the stage
               ++k1;
@@ -356,7 +362,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
       }
       if (lane == 0) tma_store_wait_read<0>();
     } else {
-    sk_epilogue_loop<SK_EPI_ANY, EPI_WARPS>(p, C, unit, rank, warp, lane, tmem_base, tmem_full0, tmem_empty0,
+    sk_epilogue_loop<I8 ? SK_EPI_BLOCK_REDUCE : SK_EPI_ANY, EPI_WARPS, 1, I8>(p, C, unit, rank, warp, lane, tmem_base, tmem_full0, tmem_empty0,
                                             &ctrl->bcast, abort_flag, ctrl->pend, &tmC, cstage, &nseg, peers);
     }
     if (OUT != OUT_SCATTER && p.wide_units > 0) {
@@ -386,14 +392,14 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           if (warp_ok && !dead && valid_cols > 0) {
             int c_first = 0;
             if (cstage != 0)
-              c_first = sk_store_tile_tma<1>(p, &tmC, cstage, warp - 2, lane, t_addr, 0, r0 + q * 32, c0,
+              c_first = sk_store_tile_tma<1, I8>(p, &tmC, cstage, warp - 2, lane, t_addr, 0, r0 + q * 32, c0,
                                              valid_cols, groups, peers, sub, EPI_WARPS / 4) >> 5;
             for (int c = c_first + sub; c < ((valid_cols + 31) >> 5); c += EPI_WARPS / 4) {
               float v[32];
               sk_load_acc(t_addr + c * 32, 0, v);
               int nv = valid_cols - c * 32;
               if (nv > 32) nv = 32;
-              if (row_ok) sk_store_chunk(C, p, r0 + row, c0 + c * 32, nv, v, peers);
+              if (row_ok) sk_store_chunk<I8>(C, p, r0 + row, c0 + c * 32, nv, v, peers);
             }
           }
           tc_fence_before();
@@ -408,7 +414,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   // ------------------------------------------------------------- teardown
   tc_fence_before();
   __syncthreads();
-  if constexpr (OUT != OUT_SCATTER) sk_reduce_pending(p, C, unit, rank, ctrl->pend, ctrl->ok, peers);
+  if constexpr (OUT != OUT_SCATTER) sk_reduce_pending<false, I8>(p, C, unit, rank, ctrl->pend, ctrl->ok, peers);
   // Neither CTA may leave while its partner can still signal its barriers or read its
   // shared memory.
   __syncthreads();
@@ -429,6 +435,8 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 
 int sk_make_tmap_f16(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols,
                      uint64_t ld_elems, uint32_t box_cols, uint32_t box_rows);
+int sk_make_tmap_i8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
+                    uint32_t box_rows);
 
 // fp32 row-major [rows, cols] tensor map with a 32 x 32 box (128-byte rows), 128-byte swizzle.
 static int make_tmap_f32_store(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld) {
@@ -455,15 +463,18 @@ static int make_tmap_f32_store(CUtensorMap* out, const void* base, uint64_t rows
 // Launch with CTA pairs.  `units` persistent pairs; p->sched must have been built for
 // 256-row tiles and `units` schedulable units.  n_peers > 0: the fused all-gather; n_peers < 0:
 // the fused reduce-scatter with -n_peers column blocks, peer_c[j] the fp32 receive slot of block j.
+// k_i8 > 0: 8-bit integer operands with that many elements of K; prob counts them in pairs.
 int sk_launch_f16_2cta(const sk_problem* prob, const void* A, const void* B, void* C, SkParams* p,
-                       void* const* peer_c, int n_peers, void* stream) {
+                       void* const* peer_c, int n_peers, int k_i8, void* stream) {
   const int n_blocks = n_peers < 0 ? -n_peers : 0;
   if (n_blocks) n_peers = 0;
   CUtensorMap tmA, tmB;
-  int st = sk_make_tmap_f16(&tmA, A, prob->M, prob->K, prob->lda, BK, BM);
+  int st = k_i8 ? sk_make_tmap_i8(&tmA, A, prob->M, k_i8, 2 * static_cast<uint64_t>(prob->lda), BM)
+                : sk_make_tmap_f16(&tmA, A, prob->M, prob->K, prob->lda, BK, BM);
   if (st != SK_OK) return st;
   const int bn = p->bn;   // tile columns (sk_make_sched): 256, or narrower when asked for (multiple of 16)
-  st = sk_make_tmap_f16(&tmB, B, prob->N, prob->K, prob->ldb, BK, bn / 2);
+  st = k_i8 ? sk_make_tmap_i8(&tmB, B, prob->N, k_i8, 2 * static_cast<uint64_t>(prob->ldb), bn / 2)
+            : sk_make_tmap_f16(&tmB, B, prob->N, prob->K, prob->ldb, BK, bn / 2);
   CUtensorMap tmC;
   memset(&tmC, 0, sizeof(tmC));
   p->c_tma = p->c_vec_ok;   // whole tiles leave through shared memory and TMA stores
@@ -508,7 +519,7 @@ int sk_launch_f16_2cta(const sk_problem* prob, const void* A, const void* B, voi
   p->col_tx_bytes = (bn / 2) * BK * 2;   // bytes of this CTA's half of a B stage
   p->tmem_cols = TMEM_COLS;
   p->stages = STAGES;
-  p->idesc = umma_idesc_f16(2 * BM, bn, 0, p->out_bf16);
+  p->idesc = k_i8 ? umma_idesc_i8(2 * BM, bn) : umma_idesc_f16(2 * BM, bn, 0, p->out_bf16);
   // K steps the second half of a 256 x 512 unit stays behind the first (see the MMA issuer).
   // Measured on configuration 5, sustained loop: 1278 TFLOP/s with 0, 1291 with 1, 1137 with 2
   // (two held stages leave the producer too little room).
@@ -518,6 +529,9 @@ int sk_launch_f16_2cta(const sk_problem* prob, const void* A, const void* B, voi
   cudaError_t e = attrs.run([]() {
     cudaError_t r = cudaFuncSetAttribute(sk_gemm_f16_2cta_kernel<OUT_PLAIN>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    if (r == cudaSuccess)
+      r = cudaFuncSetAttribute(sk_gemm_f16_2cta_kernel<OUT_PLAIN, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               SMEM_BYTES);
     if (r == cudaSuccess)
       r = cudaFuncSetAttribute(sk_gemm_f16_2cta_kernel<OUT_GATHER>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                SMEM_BYTES);
@@ -530,7 +544,10 @@ int sk_launch_f16_2cta(const sk_problem* prob, const void* A, const void* B, voi
   const bool pdl = (prob->flags & SK_FLAG_PDL) != 0;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   __half* Ch = static_cast<__half*>(C);
-  if (n_blocks)
+  if (k_i8)
+    e = sk_launch(sk_gemm_f16_2cta_kernel<OUT_PLAIN, true>, p->sched.grid * 2, NUM_THREADS, SMEM_BYTES, cs, 2, pdl,
+                  tmA, tmB, tmC, Ch, *p, peer_set);
+  else if (n_blocks)
     e = sk_launch(sk_gemm_f16_2cta_kernel<OUT_SCATTER>, p->sched.grid * 2, NUM_THREADS, SMEM_BYTES, cs, 2, pdl,
                   tmA, tmB, tmC, Ch, *p, peer_set);
   else if (n_peers > 0)

@@ -215,6 +215,18 @@ __device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t desc_a, ui
       ::"r"(d_tmem), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// 8-bit integer operands, 32-bit integer accumulators: 32 of K (the same 32 bytes) per instruction.
+__device__ __forceinline__ void umma_i8_ss(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      ::"r"(d_tmem), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // D[tmem] (+)= A[tmem] * B[smem desc]: the A operand (M = 128 rows in the 128 lanes, 16 halves
 // of K packed two per 32-bit column, even k in the low half: 8 columns per instruction) comes
 // from tensor memory, where tcgen05.st put it.
@@ -305,6 +317,13 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, int b_mn_maj
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// Instruction descriptor for kind::i8, signed A/B, 32-bit integer D, no saturation.
+//   [3] saturate   [4,6) D format 2=s32   [7,10) / [10,13) A / B format 0=u8, 1=s8
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+
 // ---- CTA-pair (cta_group::2) forms: one thread of the leader CTA issues the MMA for both
 // CTAs; each CTA loads its own half of the operands and signals the leader's barrier.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, uint32_t leader_bar,
@@ -334,6 +353,17 @@ __device__ __forceinline__ void umma_f16_ss_pair(uint32_t d_tmem, uint64_t desc_
       ".reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      ::"r"(d_tmem), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_ss_pair(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b,
+                                                uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
       "}\n"
       ::"r"(d_tmem), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");

@@ -22,7 +22,7 @@ __all__ = [
     "streamk_fp32", "streamk_fp16_nn", "streamk_fp16_nt", "streamk_fp16_nt_host", "streamk_fp16_atomic",
     "streamk_fp16_block_reduce", "ladder_prepack", "streamk_fp16_ladder",
     "streamk_fp16_ladder_block_reduce", "q4_prepack", "dequant_w4",
-    "streamk_fp16_ladder_block_reduce_q4", "schedule_info", "check_status",
+    "streamk_fp16_ladder_block_reduce_q4", "int8_quantize", "streamk_int8_nt", "schedule_info", "check_status",
     "SCHEDULE_NAMES", "reset_workspace", "release_cached_memory", "cached_memory_bytes", "device_info", "LadderWeight", "PackedQ4", "StreamKError", "SCHEDULES", "FIXUPS",
 ]
 
@@ -161,12 +161,13 @@ def schedule_info(M: int, N: int, K: int, *, kind: str = "f16", schedule: str = 
     """Host scheduler integers (streamk_fp16.py:83-113) and the tile plan for a problem;
     needs no GPU.  kind: "f32", "f16" (what the fp16 NT entry point runs: single-CTA tiles, or
     for large problems the CTA-pair kernel, described over num_sms / 2 pairs), "w4a16", or
-    "f16_pairs" (the CTA-pair kernel with num_sms pairs).  gather_peers > 0: the plan of the
+    "f16_pairs" (the CTA-pair kernel with num_sms pairs), or "int8" (what the 8-bit integer
+    entry point runs).  gather_peers > 0: the plan of the
     fused all-gather call with that many peers."""
     o = _options(kw)
     prob = _problem(M, N, K, K, K, N, "nt", schedule, "atomic", o)
     info = L.SkScheduleInfo()
-    kinds = {"f32": 0, "f16": 1, "w4a16": 2, "f16_pairs": 3}
+    kinds = {"f32": 0, "f16": 1, "w4a16": 2, "f16_pairs": 3, "int8": 4}
     if gather_peers:
         L.check(L.load().sk_schedule_gather(C.byref(prob), gather_peers, num_sms, C.byref(info)),
                 "sk_schedule_gather")
@@ -577,4 +578,89 @@ def streamk_fp16_ladder_block_reduce_q4(A, QLB: PackedQ4, *, fixup="block_reduce
         L.check(L.load().sk_gemm_w4a16(C.byref(prob), A.data_ptr(), QLB.data.data_ptr(),
                                        Cout.data_ptr(), ws.buf.data_ptr(), ws.nbytes,
                                        _stream_ptr(A.device)), "sk_gemm_w4a16")
+    return Cout
+
+
+# --------------------------------------------------------------------------- 8-bit integers
+def int8_quantize(X: torch.Tensor, *, pdl: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of X [M,K] (fp16 or bf16) as 8-bit integers: (Q int8 [M,K], scale fp32 [M]).
+
+    With a = max_k |X[m,k]|: scale[m] = a / 127 and Q[m,k] = 127 X[m,k] / a rounded to the
+    nearest integer (halves to even, of the exact quotient), so X is about Q * scale[:, None].
+    One scale per row: tokens when X holds activations, output channels when it holds a weight
+    [N,K].  A row of zeros has scale 0; a row that holds a NaN or an infinity has scale NaN and
+    Q = 0, so that products with it are NaN.  Q's row pitch is K rounded up to 16 bytes (what
+    streamk_int8_nt reads without a copy).  Rows of X may be strided.  No counterpart in the
+    reference."""
+    _check_matrix("X", X, HALF_TYPES)
+    M, K = X.shape
+    _check_extents(M=M, K=K)
+    X = _rowmajor(X)
+    pitch = -(-K // 16) * 16
+    Q = torch.empty((M, pitch), dtype=torch.int8, device=X.device)
+    scale = torch.empty(M, dtype=torch.float32, device=X.device)
+    flags = (L.SK_FLAG_BF16 if X.dtype == torch.bfloat16 else 0) | (L.SK_FLAG_PDL if pdl else 0)
+    with torch.cuda.device(X.device):
+        L.check(L.load().sk_quantize_i8(X.data_ptr(), M, K, X.stride(0) if M > 1 else K, flags, Q.data_ptr(), pitch,
+                                        scale.data_ptr(), _stream_ptr(X.device)), "sk_quantize_i8")
+    return Q[:, :K], scale
+
+
+def _check_extents(**extents) -> None:
+    for name, v in extents.items():
+        if v < 1:
+            raise ValueError(f"{name} must be at least 1, got {v}")
+
+
+def _check_scale(name: str, s: torch.Tensor, n: int, device) -> torch.Tensor:
+    if not isinstance(s, torch.Tensor) or s.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on the operands' device")
+    if s.dtype != torch.float32:
+        raise TypeError(f"{name} must be torch.float32, got {s.dtype}")
+    if s.shape not in ((n,), (n, 1), (1, n)):
+        raise ValueError(f"{name} must have {n} elements, got shape {tuple(s.shape)}")
+    return s.reshape(n).contiguous()
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """An int8 matrix with 16-byte aligned rows (TMA), copied only if it has none."""
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    n = torch.empty((t.shape[0], -(-t.shape[1] // 16) * 16), dtype=t.dtype, device=t.device)
+    n[:, : t.shape[1]].copy_(t)
+    return n[:, : t.shape[1]]
+
+
+def streamk_int8_nt(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor, *,
+                    out_dtype: torch.dtype = torch.float16, schedule: str = "auto", **kw) -> torch.Tensor:
+    """C = (A @ B.T) * scale_a[:, None] * scale_b[None, :] with 8-bit integer operands: A [M,K] and
+    B [N,K] int8, scales fp32 [M] (tokens) and [N] (output channels), C fp16 or bf16.
+
+    32-bit integer sums, exact whatever the schedule: every schedule returns the same bits.
+    C = (float(sum) * scale_a) * scale_b, then one rounding to out_dtype.  K at most 131071.
+    Operands whose rows are not 16-byte aligned are copied first.  Same schedules and keyword
+    options as streamk_fp16_nt (see _options()).  No counterpart in the reference."""
+    o = _options(kw)
+    if out_dtype not in HALF_TYPES:
+        raise TypeError(f"out_dtype must be one of {HALF_TYPES}, got {out_dtype}")
+    o["_bf16"] = out_dtype == torch.bfloat16
+    _check_matrix("A", A, torch.int8)
+    _check_matrix("B", B, torch.int8)
+    if A.device != B.device:
+        raise ValueError("A and B must be on the same device")
+    M, K = A.shape
+    N, Kb = B.shape
+    if K != Kb:
+        raise ValueError(f"Incompatible dimensions: A {tuple(A.shape)} B {tuple(B.shape)}")
+    _check_extents(M=M, N=N, K=K)
+    with torch.cuda.device(A.device):
+        scale_a = _check_scale("scale_a", scale_a, M, A.device)
+        scale_b = _check_scale("scale_b", scale_b, N, A.device)
+        A, B = _rows16(A), _rows16(B)
+        Cout = _out(o["out"], M, N, out_dtype, A.device)
+        prob = _problem(M, N, K, A.stride(0), B.stride(0), Cout.stride(0), "nt", schedule, "block_reduce", o)
+        ws = _workspace(A.device)
+        L.check(L.load().sk_gemm_i8(C.byref(prob), A.data_ptr(), B.data_ptr(), scale_a.data_ptr(), scale_b.data_ptr(),
+                                    Cout.data_ptr(), ws.buf.data_ptr(), ws.nbytes, _stream_ptr(A.device)),
+                "sk_gemm_i8")
     return Cout
