@@ -116,6 +116,9 @@ enum { SK_FLAG_PDL = 1, /* fp16 / W4A16 entry points: launch with programmatic s
           field; the default, 0, is 128).  Must match what sk_prepack_q4_ex was given.         */
        SK_FLAG_Q4_GROUP_32 = 0x100, SK_FLAG_Q4_GROUP_64 = 0x200, SK_FLAG_Q4_PER_CHANNEL = 0x300,
        SK_FLAG_Q4_GROUP_MASK = 0x300,
+       /* sk_gemm_grouped: offsets are int64 (int32 without); TN: C is fp32; NT / NN: rows of C that
+          belong to no group are set to zero (left as they are without).                         */
+       SK_FLAG_OFFSETS_64 = 0x1000, SK_FLAG_OUT_F32 = 0x2000, SK_FLAG_ZERO_REST = 0x4000,
        SK_FLAG_NO_TABLE = 2 /* SK_SCHED_AUTO: resolve by the built-in rules only, without
                           consulting the table of tuned shapes (what the offline tuner itself
                           uses to time the rules' choice).                                 */ };
@@ -150,7 +153,8 @@ typedef struct sk_device_info {
 } sk_device_info;
 
 typedef struct sk_status {
-  uint32_t code;     /* SK_OK, SK_ERR_FIXUP_TIMEOUT or SK_ERR_PIPE_TIMEOUT     */
+  uint32_t code;     /* SK_OK, SK_ERR_FIXUP_TIMEOUT, SK_ERR_PIPE_TIMEOUT or, from
+                        sk_gemm_grouped, SK_ERR_ARG (offsets out of order)     */
   uint32_t cta;      /* CTA that reported                                      */
   uint32_t detail0;  /* fixup: tile id      pipe: barrier id                   */
   uint32_t detail1;  /* fixup: awaited CTA  pipe: role                         */
@@ -257,6 +261,35 @@ int sk_gemm_i8(const sk_problem* p, const void* A, const void* B, const float* s
  * Elements K .. ldq of a row of Q are not written.                                            */
 int sk_quantize_i8(const void* X, int M, int K, int ldx, int flags, void* Q, int ldq, float* scale,
                    void* stream);
+
+/* Products grouped by expert with ragged sizes, fp16 operands (bf16 with SK_FLAG_BF16), fp32
+ * accumulation.  The rows of A are sorted by group: group e holds rows offsets[e] ..
+ * offsets[e+1) (device memory, E + 1 ascending numbers in [0, T]; a group may be empty, rows
+ * before offsets[0] and from offsets[E] on belong to no group).
+ *   SK_GROUPED_NT  A [T,K], B [E,N,K]: C[t,:] = B[e] A[t,:]          C [T,N]
+ *   SK_GROUPED_NN  A [T,K], B [E,K,N]: C[t,:] = A[t,:] B[e]          C [T,N]
+ *   SK_GROUPED_TN  A [T,K], B [T,N]:   C[e] = sum A[t,:]^T B[t,:]    C [E,K,N], zero for an empty group
+ * With Y = NT(X, W): the gradient of X is NN(dY, W), that of W is TN(dY, X).  lda, ldb, stride_b
+ * (between the groups' matrices) multiples of 8 elements, A and B 16-byte aligned; any C aligned
+ * to its type, any ldc >= N and stride_c >= K ldc (16-byte rows are the fast ones).  Every value
+ * is one sum in a fixed order: bitwise reproducible.  What other rows hold (infinities, NaN) does
+ * not reach a group's results.  Offsets that descend or leave [0, T] are clamped on the device,
+ * nothing is read or written out of range, and the status word reports SK_ERR_ARG (detail0: the
+ * first index found).  E at most SK_GROUPED_MAX_GROUPS, T at most SK_GROUPED_MAX_ROWS; the
+ * workspace is that of the other products.  No counterpart in the reference.               */
+enum { SK_GROUPED_NT = 0, SK_GROUPED_NN = 1, SK_GROUPED_TN = 2 };
+enum { SK_GROUPED_MAX_GROUPS = 1024, SK_GROUPED_MAX_ROWS = 0x7fff0000 };
+typedef struct sk_grouped_problem {
+  int32_t kind;               /* SK_GROUPED_*                                                  */
+  int32_t T, E, N, K;
+  int32_t num_sms;            /* 0 = all SMs of the device                                     */
+  int32_t timeout_us;         /* 0 = default (2 s); bound of every device wait                 */
+  int32_t flags;              /* SK_FLAG_*                                                     */
+  int64_t lda, ldb, ldc;      /* elements                                                      */
+  int64_t stride_b, stride_c; /* elements between the matrices of two groups: B of NT / NN, C of TN */
+} sk_grouped_problem;
+int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const void* B, const void* offsets, void* C,
+                    void* ws, size_t ws_bytes, void* stream);
 
 /* sk_gemm_f16 fused with the all-gather of an N-sharded product (the reference is a
  * single-GPU study; this is the column-sharded configuration's collective).  Every GPU of

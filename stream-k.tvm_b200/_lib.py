@@ -21,6 +21,8 @@ FIXUPS = {"atomic": 0, "block_reduce": 1}
 SK_FLAG_PDL = 1
 SK_FLAG_NO_TABLE = 2
 SK_FLAG_BF16 = 4
+SK_FLAG_OFFSETS_64, SK_FLAG_OUT_F32, SK_FLAG_ZERO_REST = 0x1000, 0x2000, 0x4000
+GROUPED_KINDS = {"nt": 0, "nn": 1, "tn": 2}
 SK_FLAG_Q4_GROUP = {128: 0, 32: 0x100, 64: 0x200, 0: 0x300}   # group size -> sk_problem.flags bits (0 = per-channel)
 
 
@@ -28,6 +30,11 @@ class SkProblem(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "M", "N", "K", "lda", "ldb", "ldc", "layout", "schedule", "fixup", "tile_m", "tile_n", "num_sms",
         "group_m", "fixup_timeout_us", "test_drop_flag_cta", "flags")]
+
+
+class SkGroupedProblem(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("kind", "T", "E", "N", "K", "num_sms", "timeout_us", "flags")]
+                + [(n, C.c_int64) for n in ("lda", "ldb", "ldc", "stride_b", "stride_c")])
 
 
 class SkScheduleInfo(C.Structure):
@@ -90,6 +97,7 @@ SIGNATURES = {
     "sk_dequant_q4_ex": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, _P, C.c_int, _P]),
     "sk_gemm_i8": (C.c_int, [C.POINTER(SkProblem), _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "sk_quantize_i8": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int, _P, C.c_int, _P, _P]),
+    "sk_gemm_grouped": (C.c_int, [C.POINTER(SkGroupedProblem), _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "sk_gemm_w4a16": (C.c_int, [C.POINTER(SkProblem), _P, _P, _P, _P, C.c_size_t, _P]),
 }
 

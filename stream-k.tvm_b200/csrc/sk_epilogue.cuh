@@ -29,13 +29,19 @@ constexpr int SK_EPI_BAR_ID = 1;
 
 // Bounded mbarrier wait.  On time-out the waiter raises the CTA-wide abort flag
 // and records the barrier; every other wait in the CTA then returns false too.
+// CLUSTER: the arrivals come from other CTAs of the cluster, whose writes must be visible.
+template <bool CLUSTER = false, typename Params>
 __device__ __forceinline__ bool sk_wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
-                                            const SkParams& p, uint32_t bar_id, uint32_t role) {
-  if (skptx::mbar_try_wait(bar, parity)) return true;
+                                            const Params& p, uint32_t bar_id, uint32_t role) {
+  auto tried = [&]() {
+    if constexpr (CLUSTER) return skptx::mbar_try_wait_cluster(bar, parity);
+    else return skptx::mbar_try_wait(bar, parity);
+  };
+  if (tried()) return true;
   const unsigned long long t0 = skptx::globaltimer_ns();
   unsigned spins = 0;
   for (;;) {
-    if (skptx::mbar_try_wait(bar, parity)) return true;
+    if (tried()) return true;
     if (*abort_flag) return false;
     if ((++spins & 7u) == 0u) {
       if (skptx::globaltimer_ns() - t0 > p.timeout_ns) {

@@ -1,0 +1,810 @@
+// Products grouped by expert with ragged sizes (sk_gemm_grouped): the rows of A are sorted by
+// group, group e holding rows offsets[e] .. offsets[e+1), and every group has a matrix of its own.
+//
+//   NT   C[t,:] = B[e] A[t,:]            B [E,N,K]   (a linear layer of every expert)
+//   NN   C[t,:] = A[t,:] B[e]            B [E,K,N]   (its input gradient)
+//   TN   C[e]   = sum_t A[t,:]^T B[t,:]  C [E,K,N]   (its weight gradient)
+//
+// The sizes live on the device: every CTA reads the offsets, makes their prefix sums of tiles in
+// shared memory, and walks its share of the tile list (a persistent launch, no host round trip).
+// Offsets are clamped into [0, T] and made ascending before use, so no table of offsets makes a
+// kernel read or write out of range; a table that needed it is reported through the status word.
+//
+// NT and NN: CTA pairs (cta_group::2).  The weights feed the UMMA M dimension (256 of the N output
+// features per pair, 128 per CTA) and the rows of a group the UMMA N dimension, whose extent the
+// instruction descriptor sets tile by tile in steps of 32: a group of 5 rows costs the tensor
+// cores 32 columns and a group of 300 two tiles of 160, where rows on the M side would cost whole
+// multiples of 128 or 256.  Groups of a few rows are then what they should be, a stream of the
+// weights.  A pair's accumulator is transposed (lane = feature, column = row of A): 32 lanes
+// store 64 contiguous bytes of a row of C.
+//
+// TN: the sum runs over a group's rows, so both operands are MN-major (TMA boxes of 64 columns x
+// 64 rows) and a group's last step holds rows of the next group.  Those must not count, whatever
+// they hold: UMMAs past the group's end are not issued (16 rows each), and the rows of the last
+// one that lie past it are zeroed in shared memory, in both operands (0 x NaN is NaN).
+#include "sk_common.cuh"
+#include "sk_epilogue.cuh"
+
+namespace {
+
+using namespace skptx;
+
+constexpr int BK = 64;                  // K per step: 128 bytes of a row
+constexpr int HALF_M = 128;             // UMMA M rows per CTA of a pair
+constexpr int A_STEP_BYTES = HALF_M * BK * 2;   // 16 KB
+constexpr int MAX_BN = 256;
+constexpr int KG = 2;                   // steps that share a stage
+constexpr int MAX_STAGES = 6;
+constexpr int EPI_WARPS = 8;
+constexpr int TMEM_COLS = 512;
+constexpr int SMEM_LIMIT = 232448;
+constexpr int CTRL_BYTES = 512;
+
+struct GroupedParams {
+  int T, E, N, K;
+  long long ldc, stride_c;   // elements
+  const void* offsets;
+  int off64;
+  int bn_max;                // most rows of a group per tile (NT / NN): a multiple of 32
+  int tiles_f;               // tiles along the UMMA M side (NT / NN: of N; TN: of K)
+  int tiles_n;               // TN: tiles of N
+  int stages;
+  int b_step_bytes;          // shared memory per step of this CTA's half of the UMMA N operand
+  int zero_rest;             // NT / NN: rows of C that belong to no group are set to zero
+  int out_bf16;
+  int c_vec_ok;              // rows of C can take 16-byte stores
+  int c_tma;                 // TN: C leaves through TMA stores
+  uint32_t idesc;            // with N = 0
+  unsigned long long timeout_ns;
+  SkWorkspace ws;
+};
+
+struct Ctrl {
+  uint64_t full[MAX_STAGES];        // leader: both CTAs' loads
+  uint64_t empty[MAX_STAGES];       // each CTA
+  uint64_t tail_full[MAX_STAGES];   // TN, each CTA: this CTA's loads of a stage that needs zeroing
+  uint64_t tail_ready[MAX_STAGES];  // TN, leader: both CTAs' halves are zeroed
+  uint64_t tmem_full[2], tmem_empty[2];
+  uint32_t tmem_base;
+  uint32_t abort;
+};
+static_assert(sizeof(Ctrl) <= CTRL_BYTES, "Ctrl must fit its reserved space");
+
+__host__ __device__ constexpr int align_up(int v, int a) { return (v + a - 1) / a * a; }
+// Group table in shared memory: start[E + 1], then (NT / NN) first[E + 1], the first row tile.
+__host__ __device__ constexpr int table_bytes(int E) { return align_up(2 * (E + 1) * 4, 16); }
+
+// Fills the table.  Called by every thread; ends with the table visible to all.
+__device__ __forceinline__ void make_table(const GroupedParams& p, int* start, int* first) {
+  for (int i = threadIdx.x; i <= p.E; i += blockDim.x) {
+    long long o = p.off64 ? __ldg(static_cast<const long long*>(p.offsets) + i)
+                          : static_cast<long long>(__ldg(static_cast<const int*>(p.offsets) + i));
+    bool bad = o < 0 || o > p.T;
+    o = o < 0 ? 0 : o > p.T ? p.T : o;
+    if (i > 0) {
+      const long long before = p.off64 ? __ldg(static_cast<const long long*>(p.offsets) + i - 1)
+                                       : static_cast<long long>(__ldg(static_cast<const int*>(p.offsets) + i - 1));
+      bad = bad || before > o;
+    }
+    start[i] = static_cast<int>(o);
+    if (bad && blockIdx.x == 0) sk_report(p.ws.status, SK_ERR_ARG, static_cast<uint32_t>(i), 0u);
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    // running maximum of the starts, running sum of the tiles
+    const int lane = threadIdx.x;
+    int top = 0, sum = 0, prev_start = 0;
+    for (int base = 0; base <= p.E; base += 32) {
+      const int i = base + lane;
+      int s = i <= p.E ? start[i] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, s, d);
+        if (lane >= d && o > s) s = o;
+      }
+      if (s < top) s = top;
+      int before = __shfl_up_sync(0xffffffffu, s, 1);
+      if (lane == 0) before = prev_start;
+      // tiles of group i - 1 (rows before .. s): first[i] = tiles of groups 0 .. i - 1
+      int t = i > 0 && i <= p.E ? (s - before + p.bn_max - 1) / p.bn_max : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, t, d);
+        if (lane >= d) t += o;
+      }
+      t += sum;
+      if (i <= p.E) {
+        start[i] = s;
+        first[i] = t;
+      }
+      top = prev_start = __shfl_sync(0xffffffffu, s, 31);
+      sum = __shfl_sync(0xffffffffu, t, 31);
+    }
+  }
+  __syncthreads();
+}
+
+// ------------------------------------------------------------------------------- NT and NN
+struct RowTile {
+  int e;          // group
+  int f0;         // first output feature of the pair's 256
+  int r0, rows;   // rows of A
+  int bn;         // UMMA N: rows rounded up to 32
+};
+
+// Walks the tiles unit, unit + grid, ...: group by group, inside a group bands of up to eight row
+// tiles, the feature tiles of a band one after the other (the pairs that run at a time then share
+// few weight panels and few row panels).
+struct RowWalk {
+  int t, e;
+  __device__ __forceinline__ bool next(const GroupedParams& p, const int* start, const int* first, int units,
+                                       RowTile& o) {
+    const int total = first[p.E] * p.tiles_f;     // (at most T / 1 * N / 256: checked by the launcher)
+    if (t >= total) return false;
+    while (first[e + 1] * p.tiles_f <= t) ++e;
+    const int mt = first[e + 1] - first[e];
+    int local = t - first[e] * p.tiles_f;
+    const int band = local / (8 * p.tiles_f);
+    local -= band * 8 * p.tiles_f;
+    const int in_band = mt - band * 8 < 8 ? mt - band * 8 : 8;
+    const int f = local / in_band;
+    const int m = band * 8 + (local - f * in_band);
+    const int rows = start[e + 1] - start[e];
+    const int per = (rows + mt - 1) / mt;         // the group's rows in equal tiles
+    o.e = e;
+    o.f0 = f * (2 * HALF_M);
+    o.r0 = start[e] + m * per;
+    o.rows = rows - m * per < per ? rows - m * per : per;
+    o.bn = o.rows > 0 ? (o.rows + 31) & ~31 : 32;
+    t += units;
+    return true;
+  }
+};
+
+constexpr int NT_THREADS = 64 + 32 * EPI_WARPS;   // warp 0 producer, 1 MMA issuer, 2..9 epilogue
+
+// W_MN: the weights are MN-major (NN): two boxes of 64 features x 64 of K per step.
+template <bool W_MN>
+__global__ void __launch_bounds__(NT_THREADS, 1)
+sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX16,
+                       const __grid_constant__ CUtensorMap tmX64, const __grid_constant__ CUtensorMap tmX128,
+                       uint16_t* __restrict__ C, const GroupedParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw_addr);
+  const int STAGES = p.stages;
+  const uint32_t sW = base, sX = base + STAGES * KG * A_STEP_BYTES;
+  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + STAGES * KG * (A_STEP_BYTES + p.b_step_bytes));
+  int* start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ctrl) + CTRL_BYTES);
+  int* first = start + p.E + 1;
+  volatile uint32_t* abort_flag = &ctrl->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    griddep_launch_dependents();
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(smem_u32(&ctrl->full[i]), 1);
+      mbar_init(smem_u32(&ctrl->empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctrl->tmem_full[i]), 1);
+      mbar_init(smem_u32(&ctrl->tmem_empty[i]), 2 * EPI_WARPS);
+    }
+    ctrl->abort = 0u;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    prefetch_tensormap(&tmW);
+    prefetch_tensormap(&tmX16);
+    prefetch_tensormap(&tmX64);
+    prefetch_tensormap(&tmX128);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&ctrl->tmem_base), TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  griddep_wait();
+  make_table(p, start, first);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&ctrl->tmem_base);
+  const int I = (p.K + BK - 1) / BK;
+  RowWalk walk{unit, 0};
+  RowTile tile;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------- producer (both CTAs)
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      const uint32_t full0 = smem_u32(&ctrl->full[0]), empty0 = smem_u32(&ctrl->empty[0]);
+      const uint32_t full0_leader = mapa_shared(full0, 0);
+      while (ok && walk.next(p, start, first, units, tile)) {
+        const int half = tile.bn / 2;             // rows of A that this CTA supplies
+        const CUtensorMap* tmX = half <= 16 ? &tmX16 : half <= 64 ? &tmX64 : &tmX128;
+        const int box = half <= 16 ? 16 : half <= 64 ? 64 : 128;
+        const uint32_t tx = 2u * (A_STEP_BYTES + static_cast<uint32_t>(box) * 128u);   // of both CTAs
+        const int f_row = tile.f0 + rank * HALF_M, x_row = tile.r0 + rank * half;
+        for (int k = 0; k < I;) {
+          const int n = I - k < KG ? I - k : KG;
+          if (!sk_wait_bar(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = full0_leader + 8u * stage;
+          if (rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, n * tx);
+          for (int j = 0; j < n; ++j) {
+            const uint32_t dW = sW + (stage * KG + j) * A_STEP_BYTES;
+            if constexpr (W_MN) {
+              tma_load_3d_pair(dW, &tmW, bar, f_row, (k + j) * BK, tile.e);
+              tma_load_3d_pair(dW + 8192, &tmW, bar, f_row + 64, (k + j) * BK, tile.e);
+            } else {
+              tma_load_3d_pair(dW, &tmW, bar, (k + j) * BK, f_row, tile.e);
+            }
+            tma_load_2d_pair(sX + (stage * KG + j) * p.b_step_bytes, tmX, bar, (k + j) * BK, x_row);
+          }
+          k += n;
+          if (++stage == STAGES) { stage = 0; ph ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------- MMA issuer (leader)
+    if (lane == 0 && rank == 0) {
+      int stage = 0;
+      uint32_t ph = 0, nseg = 0;
+      bool ok = true;
+      constexpr uint32_t w_kstep16 = (W_MN ? 2048u : 32u) >> 4;
+      const uint64_t w_hi = umma_desc_sw128_hi(W_MN ? 8192u : 16u, 1024), x_hi = umma_desc_sw128_hi(16u, 1024);
+      const uint32_t w_lo0 = umma_desc_lo(sW), x_lo0 = umma_desc_lo(sX);
+      const uint32_t full0 = smem_u32(&ctrl->full[0]), empty0 = smem_u32(&ctrl->empty[0]);
+      while (ok && walk.next(p, start, first, units, tile)) {
+        const uint32_t buf = nseg & 1u;
+        if (!sk_wait_bar(smem_u32(&ctrl->tmem_empty[buf]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf, 1)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * MAX_BN;
+        const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tile.bn >> 3) << 17);
+        uint32_t accumulate = 0u;
+        for (int k = 0; k < I;) {
+          const int n = I - k < KG ? I - k : KG;
+          if (!sk_wait_bar(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          for (int j = 0; j < n; ++j) {
+            const uint32_t w_lo = w_lo0 + (stage * KG + j) * (A_STEP_BYTES >> 4);
+            const uint32_t x_lo = x_lo0 + (stage * KG + j) * (static_cast<uint32_t>(p.b_step_bytes) >> 4);
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk) {
+              umma_f16_ss_pair(d_tmem, w_hi | (w_lo + kk * w_kstep16), x_hi | (x_lo + kk * 2), idesc, accumulate);
+              accumulate = 1u;
+            }
+          }
+          umma_commit_pair(empty0 + 8u * stage);
+          k += n;
+          if (++stage == STAGES) { stage = 0; ph ^= 1u; }
+        }
+        if (!ok) break;
+        umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));
+        ++nseg;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------- epilogue (both CTAs)
+    const int q = warp & 3, sub = (warp - 2) >> 2;   // TMEM lane quadrant; which of its two warps
+    if (p.zero_rest) {
+      // rows before the first group and after the last, while the first tile is on its way
+      const int lo = start[0], hi = start[p.E], rest = lo + (p.T - hi);
+      const int nw = gridDim.x * EPI_WARPS;
+      for (int i = blockIdx.x * EPI_WARPS + (warp - 2); i < rest; i += nw) {
+        uint16_t* row = C + static_cast<long long>(i < lo ? i : hi + (i - lo)) * p.ldc;
+        if (p.c_vec_ok) {
+          for (int c = lane * 8; c + 8 <= p.N; c += 256) *reinterpret_cast<uint4*>(row + c) = make_uint4(0u, 0u, 0u, 0u);
+          for (int c = (p.N & ~7) + lane; c < p.N; c += 32) row[c] = 0;
+        } else {
+          for (int c = lane; c < p.N; c += 32) row[c] = 0;
+        }
+      }
+    }
+    const uint32_t tmem_full0 = smem_u32(&ctrl->tmem_full[0]);
+    const uint32_t tmem_empty0 = mapa_shared(smem_u32(&ctrl->tmem_empty[0]), 0);
+    uint32_t nseg = 0;
+    bool dead = false;
+    while (walk.next(p, start, first, units, tile)) {
+      const uint32_t buf = nseg & 1u;
+      if (!dead) {
+        const bool got = sk_wait_bar(tmem_full0 + 8u * buf, (nseg >> 1) & 1u, abort_flag, p, 24 + buf, 2);
+        if (!__all_sync(0xffffffffu, got)) dead = true;
+      }
+      ++nseg;
+      tc_fence_after();
+      const uint32_t t_addr = tmem_base + buf * MAX_BN + (static_cast<uint32_t>(q * 32) << 16);
+      const int f = tile.f0 + rank * HALF_M + q * 32 + lane;
+      const bool f_ok = f < p.N;
+      if (!dead && tile.f0 + rank * HALF_M + q * 32 < p.N) {
+        for (int c = sub * 32; c < tile.rows; c += 64) {
+          float v[32];
+          sk_load_acc(t_addr + c, 0, v);
+          uint16_t* dst = C + static_cast<long long>(tile.r0 + c) * p.ldc + f;
+          const int nv = tile.rows - c;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (f_ok && j < nv) dst[j * p.ldc] = static_cast<uint16_t>(sk_pack2(v[j], 0.f, p.out_bf16));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tmem_empty0 + 8u * buf);
+    }
+  }
+
+  // ------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    if (*abort_flag) {
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 200000ULL) __nanosleep(1000);
+    }
+    tc_fence_after();
+    __syncwarp();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------- TN
+struct SumTile {
+  int e, f0, c0;    // group, first row (of K) and column (of N) of the pair's 256 x 256 tile of C[e]
+  int r0, rows;     // the group's rows of A and B
+};
+
+struct SumWalk {
+  int t;
+  __device__ __forceinline__ bool next(const GroupedParams& p, const int* start, int units, SumTile& o) {
+    const int per_e = p.tiles_f * p.tiles_n;
+    if (t >= p.E * per_e) return false;
+    const int e = t / per_e;
+    int local = t - e * per_e;
+    const int band = local / (8 * p.tiles_n);
+    local -= band * 8 * p.tiles_n;
+    const int in_band = p.tiles_f - band * 8 < 8 ? p.tiles_f - band * 8 : 8;
+    const int n = local / in_band;
+    o.e = e;
+    o.f0 = (band * 8 + (local - n * in_band)) * (2 * HALF_M);
+    o.c0 = n * MAX_BN;
+    o.r0 = start[e];
+    o.rows = start[e + 1] - start[e];
+    t += units;
+    return true;
+  }
+};
+
+constexpr int TN_THREADS = NT_THREADS + 32;   // one warp more: it zeroes what lies past a group's end
+constexpr int TN_STAGES = 5;                  // one step each
+constexpr int TN_B_STEP = 128 * BK * 2;
+constexpr int TN_PIPE = TN_STAGES * (A_STEP_BYTES + TN_B_STEP);
+
+// Does step k of a group of `rows` rows hold a UMMA that reaches past the group's end?
+__device__ __forceinline__ bool step_needs_zeros(int k, int rows) {
+  return (k + 1) * BK > rows && (rows & 15) != 0;
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(TN_THREADS, 1)
+sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                      const __grid_constant__ CUtensorMap tmC, void* __restrict__ Cv, const GroupedParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw_addr);
+  constexpr int STAGES = TN_STAGES;
+  const uint32_t sA = base, sB = base + STAGES * A_STEP_BYTES;
+  const uint32_t cstage = base + TN_PIPE;                    // 8 x 4 KB staging of the TMA stores
+  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + TN_PIPE + EPI_WARPS * 4096);
+  int* start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ctrl) + CTRL_BYTES);
+  int* first = start + p.E + 1;
+  volatile uint32_t* abort_flag = &ctrl->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    griddep_launch_dependents();
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(smem_u32(&ctrl->full[i]), 1);
+      mbar_init(smem_u32(&ctrl->empty[i]), 1);
+      mbar_init(smem_u32(&ctrl->tail_full[i]), 1);
+      mbar_init(smem_u32(&ctrl->tail_ready[i]), 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctrl->tmem_full[i]), 1);
+      mbar_init(smem_u32(&ctrl->tmem_empty[i]), 2 * EPI_WARPS);
+    }
+    ctrl->abort = 0u;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    prefetch_tensormap(&tmA);
+    prefetch_tensormap(&tmB);
+    if (p.c_tma) prefetch_tensormap(&tmC);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&ctrl->tmem_base), TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  griddep_wait();
+  make_table(p, start, first);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&ctrl->tmem_base);
+  SumWalk walk{unit};
+  SumTile tile;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------- producer (both CTAs)
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      const uint32_t full0 = smem_u32(&ctrl->full[0]), empty0 = smem_u32(&ctrl->empty[0]);
+      const uint32_t tail0 = smem_u32(&ctrl->tail_full[0]);
+      const uint32_t full0_leader = mapa_shared(full0, 0);
+      while (ok && walk.next(p, start, units, tile)) {
+        const int I = (tile.rows + BK - 1) / BK;
+        const int a_col = tile.f0 + rank * HALF_M, b_col = tile.c0 + rank * (MAX_BN / 2);
+        for (int k = 0; k < I; ++k) {
+          if (!sk_wait_bar(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0)) {
+            ok = false;
+            break;
+          }
+          // A stage that needs zeroing is announced in each CTA by itself: the zeroing warp has
+          // to see its own CTA's bytes land.  (The leader's barrier completes a phase all the
+          // same, so that the parities of the ring stay in step.)
+          const bool tail = step_needs_zeros(k, tile.rows);
+          constexpr uint32_t bytes = A_STEP_BYTES + TN_B_STEP;
+          uint32_t bar = full0_leader + 8u * stage;
+          if (tail) {
+            if (rank == 0) mbar_arrive(full0 + 8u * stage);
+            bar = tail0 + 8u * stage;
+            mbar_arrive_expect_tx(bar, bytes);
+          } else if (rank == 0) {
+            mbar_arrive_expect_tx(full0 + 8u * stage, 2 * bytes);
+          }
+          const uint32_t dA = sA + stage * A_STEP_BYTES, dB = sB + stage * TN_B_STEP;
+          const int row = tile.r0 + k * BK;
+          for (int h = 0; h < 2; ++h) {
+            if (tail) {
+              tma_load_2d(dA + h * 8192, &tmA, bar, a_col + h * 64, row);
+              tma_load_2d(dB + h * 8192, &tmB, bar, b_col + h * 64, row);
+            } else {
+              tma_load_2d_pair(dA + h * 8192, &tmA, bar, a_col + h * 64, row);
+              tma_load_2d_pair(dB + h * 8192, &tmB, bar, b_col + h * 64, row);
+            }
+          }
+          if (++stage == STAGES) { stage = 0; ph ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------- MMA issuer (leader)
+    if (lane == 0 && rank == 0) {
+      int stage = 0;
+      uint32_t ph = 0, nseg = 0, tail_ph = 0;
+      bool ok = true;
+      const uint64_t hi = umma_desc_sw128_hi(8192u, 1024);   // MN-major: 64-wide chunks 8 KB apart, 8 rows 1 KB apart
+      const uint32_t a_lo0 = umma_desc_lo(sA), b_lo0 = umma_desc_lo(sB);
+      const uint32_t full0 = smem_u32(&ctrl->full[0]), empty0 = smem_u32(&ctrl->empty[0]);
+      const uint32_t ready0 = smem_u32(&ctrl->tail_ready[0]);
+      const uint32_t idesc = p.idesc | (static_cast<uint32_t>(MAX_BN >> 3) << 17);
+      while (ok && walk.next(p, start, units, tile)) {
+        const int I = (tile.rows + BK - 1) / BK;
+        if (I == 0) continue;   // (the epilogue writes zeros)
+        const uint32_t buf = nseg & 1u;
+        if (!sk_wait_bar(smem_u32(&ctrl->tmem_empty[buf]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf, 1)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * MAX_BN;
+        uint32_t accumulate = 0u;
+        for (int k = 0; k < I; ++k) {
+          if (!sk_wait_bar(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
+            ok = false;
+            break;
+          }
+          if (step_needs_zeros(k, tile.rows)) {
+            if (!sk_wait_bar<true>(ready0 + 8u * stage, (tail_ph >> stage) & 1u, abort_flag, p, 48 + stage, 1)) {
+              ok = false;
+              break;
+            }
+            tail_ph ^= 1u << stage;
+          }
+          tc_fence_after();
+          const uint32_t a_lo = a_lo0 + stage * (A_STEP_BYTES >> 4), b_lo = b_lo0 + stage * (TN_B_STEP >> 4);
+          const int left = tile.rows - k * BK;              // rows of the group in this step
+          const int mmas = left >= BK ? BK / 16 : (left + 15) >> 4;
+          for (int kk = 0; kk < mmas; ++kk) {
+            umma_f16_ss_pair(d_tmem, hi | (a_lo + kk * 128), hi | (b_lo + kk * 128), idesc, accumulate);
+            accumulate = 1u;
+          }
+          umma_commit_pair(empty0 + 8u * stage);
+          if (++stage == STAGES) { stage = 0; ph ^= 1u; }
+        }
+        if (!ok) break;
+        umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));
+        ++nseg;
+      }
+    }
+  } else if (warp == 2 + EPI_WARPS) {
+    // ------------------------------------------------------------- zeroing warp (both CTAs)
+    int stage = 0;
+    uint32_t tail_ph = 0;
+    bool ok = true;
+    const uint32_t tail0 = smem_u32(&ctrl->tail_full[0]);
+    const uint32_t ready0_leader = mapa_shared(smem_u32(&ctrl->tail_ready[0]), 0);
+    while (ok && walk.next(p, start, units, tile)) {
+      const int I = (tile.rows + BK - 1) / BK;
+      for (int k = 0; k < I; ++k) {
+        if (step_needs_zeros(k, tile.rows)) {
+          const bool got = sk_wait_bar(tail0 + 8u * stage, (tail_ph >> stage) & 1u, abort_flag, p, 56 + stage, 5);
+          if (!__all_sync(0xffffffffu, got)) {
+            ok = false;
+            break;
+          }
+          tail_ph ^= 1u << stage;
+          // rows lo .. hi of the step's 64, 128 bytes in each of the four chunks (swizzling moves
+          // 16-byte pieces inside a row, so a whole row is a whole row)
+          const int lo = tile.rows - k * BK, hi = (lo + 15) & ~15;
+          const int pieces = (hi - lo) * 8;
+          for (int i = lane; i < 4 * pieces; i += 32) {
+            const int chunk = i / pieces, piece = i - chunk * pieces;
+            const uint32_t b = (chunk < 2 ? sA + stage * A_STEP_BYTES : sB + stage * TN_B_STEP) + (chunk & 1) * 8192;
+            st_shared_v4(b + lo * 128 + piece * 16, 0.f, 0.f, 0.f, 0.f);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(ready0_leader + 8u * stage);
+        }
+        if (++stage == STAGES) stage = 0;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------- epilogue (both CTAs)
+    const int q = warp & 3, sub = (warp - 2) >> 2;
+    const uint32_t tmem_full0 = smem_u32(&ctrl->tmem_full[0]);
+    const uint32_t tmem_empty0 = mapa_shared(smem_u32(&ctrl->tmem_empty[0]), 0);
+    const uint32_t buf_smem = cstage + static_cast<uint32_t>(warp - 2) * 4096u;
+    constexpr int gcols = F32 ? 32 : 64;            // columns of a 128-byte row of the staging buffer
+    uint32_t nseg = 0;
+    bool dead = false;
+    while (walk.next(p, start, units, tile)) {
+      const bool some = tile.rows > 0;
+      const uint32_t buf = nseg & 1u;
+      if (some) {
+        if (!dead) {
+          const bool got = sk_wait_bar(tmem_full0 + 8u * buf, (nseg >> 1) & 1u, abort_flag, p, 24 + buf, 2);
+          if (!__all_sync(0xffffffffu, got)) dead = true;
+        }
+        ++nseg;
+        tc_fence_after();
+      }
+      const uint32_t t_addr = tmem_base + buf * MAX_BN + (static_cast<uint32_t>(q * 32) << 16);
+      const int r0 = tile.f0 + rank * HALF_M + q * 32;      // first of this warp's 32 rows of C[e]
+      int valid = p.N - tile.c0;
+      if (valid > MAX_BN) valid = MAX_BN;
+      if (!dead && r0 < p.K) {
+        for (int c = sub * gcols; c < valid; c += 2 * gcols) {
+          float v[gcols / 32][32];
+#pragma unroll
+          for (int h = 0; h < gcols / 32; ++h) {
+            if (some) {
+              sk_load_acc(t_addr + c + h * 32, 0, v[h]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[h][j] = 0.f;
+            }
+          }
+          if (p.c_tma) {
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t a = buf_smem + static_cast<uint32_t>(lane) * 128u +
+                                 ((static_cast<uint32_t>(j) ^ (static_cast<uint32_t>(lane) & 7u)) << 4);
+              if constexpr (F32) {
+                st_shared_v4(a, v[0][4 * j], v[0][4 * j + 1], v[0][4 * j + 2], v[0][4 * j + 3]);
+              } else {
+                const float* w = &v[j >> 2][(j & 3) * 8];
+                const uint32_t h0 = sk_pack2(w[0], w[1], p.out_bf16), h1 = sk_pack2(w[2], w[3], p.out_bf16);
+                const uint32_t h2 = sk_pack2(w[4], w[5], p.out_bf16), h3 = sk_pack2(w[6], w[7], p.out_bf16);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(h0), "r"(h1), "r"(h2), "r"(h3)
+                             : "memory");
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&tmC, buf_smem, tile.c0 + c, r0, tile.e);   // clipped at the edges of C[e]
+              tma_store_commit();
+            }
+          } else if (r0 + lane < p.K) {
+            const long long at = tile.e * p.stride_c + static_cast<long long>(r0 + lane) * p.ldc + tile.c0 + c;
+#pragma unroll
+            for (int h = 0; h < gcols / 32; ++h) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (c + h * 32 + j < valid) {
+                  if constexpr (F32) static_cast<float*>(Cv)[at + h * 32 + j] = v[h][j];
+                  else static_cast<uint16_t*>(Cv)[at + h * 32 + j] = static_cast<uint16_t>(sk_pack2(v[h][j], 0.f, p.out_bf16));
+                }
+              }
+            }
+          }
+        }
+      }
+      if (some) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tmem_empty0 + 8u * buf);
+      }
+    }
+    if (lane == 0) tma_store_wait_read<0>();
+  }
+
+  // ------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    if (*abort_flag) {
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 200000ULL) __nanosleep(1000);
+    }
+    tc_fence_after();
+    __syncwarp();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// [batch, rows, cols] tensor map (batch 0: two-dimensional), 128-byte swizzle, box {box_cols, box_rows(, 1)}.
+int make_map(CUtensorMap* out, const void* ptr, bool f32, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld,
+             uint64_t batch_stride, uint32_t box_cols, uint32_t box_rows) {
+  static EncodeTiledFn enc = []() -> EncodeTiledFn {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) return nullptr;
+    return q == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiledFn>(f) : nullptr;
+  }();
+  if (!enc) return SK_ERR_LAUNCH;
+  const uint64_t esz = f32 ? 4 : 2;
+  cuuint64_t gdim[3] = {cols, rows, batch};
+  cuuint64_t gstride[2] = {ld * esz, batch_stride * esz};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, batch ? 3 : 2,
+                         const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SK_OK : sk_set_driver_error(static_cast<int>(r));
+}
+
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+}  // namespace
+
+extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const void* B, const void* offsets, void* C,
+                               void* ws, size_t ws_bytes, void* stream) {
+  if (!g || !A || !B || !C || !offsets) return SK_ERR_ARG;
+  if (g->kind < SK_GROUPED_NT || g->kind > SK_GROUPED_TN) return SK_ERR_ARG;
+  if (g->T <= 0 || g->E <= 0 || g->N <= 0 || g->K <= 0) return SK_ERR_SHAPE;
+  if (g->E > SK_GROUPED_MAX_GROUPS || g->T > SK_GROUPED_MAX_ROWS) return SK_ERR_LIMIT;
+  const bool tn = g->kind == SK_GROUPED_TN, nn = g->kind == SK_GROUPED_NN;
+  const bool f32 = (g->flags & SK_FLAG_OUT_F32) != 0;
+  if (f32 && !tn) return SK_ERR_ARG;
+  if (g->lda < g->K || g->ldb < (g->kind == SK_GROUPED_NT ? g->K : g->N) || g->ldc < g->N) return SK_ERR_SHAPE;
+  const long long b_rows = g->kind == SK_GROUPED_NT ? g->N : g->K;
+  if (!tn && g->E > 1 && g->stride_b < b_rows * g->ldb) return SK_ERR_SHAPE;
+  if (tn && g->E > 1 && g->stride_c < static_cast<long long>(g->K) * g->ldc) return SK_ERR_SHAPE;
+  // TMA: 16-byte aligned bases and pitches
+  if (!aligned(A, 16) || !aligned(B, 16) || (g->lda & 7) != 0 || (g->ldb & 7) != 0) return SK_ERR_ALIGN;
+  if (!tn && g->E > 1 && (g->stride_b & 7) != 0) return SK_ERR_ALIGN;
+  if (!aligned(C, f32 ? 4 : 2) || !aligned(offsets, (g->flags & SK_FLAG_OFFSETS_64) ? 8 : 4)) return SK_ERR_ALIGN;
+  sk_problem any;
+  memset(&any, 0, sizeof(any));
+  any.num_sms = g->num_sms;
+  int sms = 0, dev_sms = 0;
+  int st = sk_resolve_grid(&any, &sms, &dev_sms);
+  if (st != SK_OK) return st;
+  if (sms < 2) return SK_ERR_LIMIT;   // CTA pairs
+  if (!ws || ws_bytes < sk_ws_total_bytes(dev_sms)) return SK_ERR_WORKSPACE;
+  if (!aligned(ws, 256)) return SK_ERR_ALIGN;
+
+  GroupedParams p;
+  memset(&p, 0, sizeof(p));
+  p.T = g->T; p.E = g->E; p.N = g->N; p.K = g->K;
+  p.ldc = g->ldc; p.stride_c = g->E > 1 ? g->stride_c : static_cast<long long>(g->K) * g->ldc;
+  p.offsets = offsets;
+  p.off64 = (g->flags & SK_FLAG_OFFSETS_64) ? 1 : 0;
+  p.out_bf16 = (g->flags & SK_FLAG_BF16) ? 1 : 0;
+  p.zero_rest = (g->flags & SK_FLAG_ZERO_REST) ? 1 : 0;
+  p.timeout_ns = (g->timeout_us > 0 ? static_cast<unsigned long long>(g->timeout_us) : 2000000ULL) * 1000ULL;
+  p.ws = sk_ws_carve(ws, dev_sms);
+  const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const bool pdl = (g->flags & SK_FLAG_PDL) != 0;
+  const uint64_t ldb = static_cast<uint64_t>(g->ldb), stride_b = g->E > 1 ? static_cast<uint64_t>(g->stride_b) : ldb * b_rows;
+  static SkPerDeviceOnce attrs;
+  cudaError_t e = attrs.run([]() {
+    cudaError_t r = cudaFuncSetAttribute(sk_grouped_rows_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+    if (r == cudaSuccess)
+      r = cudaFuncSetAttribute(sk_grouped_rows_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+    if (r == cudaSuccess)
+      r = cudaFuncSetAttribute(sk_grouped_sum_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+    if (r == cudaSuccess)
+      r = cudaFuncSetAttribute(sk_grouped_sum_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+    return r;
+  });
+  if (e != cudaSuccess) return sk_set_cuda_error(e);
+  const int units = sms / 2;
+  const uint32_t bf16_bits = p.out_bf16 ? 1u : 0u;
+
+  if (tn) {
+    p.bn_max = MAX_BN;
+    p.tiles_f = (g->K + 255) / 256;
+    p.tiles_n = (g->N + 255) / 256;
+    const long long total = static_cast<long long>(p.tiles_f) * p.tiles_n * g->E;
+    if (total > (1LL << 30)) return SK_ERR_LIMIT;
+    const int esz = f32 ? 4 : 2;
+    p.c_tma = aligned(C, 16) && (p.ldc * esz) % 16 == 0 && (p.stride_c * esz) % 16 == 0;
+    p.idesc = umma_idesc_f16(2 * HALF_M, 0, 1, bf16_bits) | (1u << 15);   // both operands MN-major
+    CUtensorMap tmA, tmB, tmC;
+    memset(&tmC, 0, sizeof(tmC));
+    st = make_map(&tmA, A, false, 0, g->T, g->K, g->lda, 0, 64, 64);
+    if (st == SK_OK) st = make_map(&tmB, B, false, 0, g->T, g->N, ldb, 0, 64, 64);
+    if (st == SK_OK && p.c_tma) st = make_map(&tmC, C, f32, g->E, g->K, g->N, p.ldc, p.stride_c, f32 ? 32 : 64, 32);
+    if (st != SK_OK) return st;
+    const int smem = 1024 + TN_PIPE + EPI_WARPS * 4096 + CTRL_BYTES + table_bytes(g->E);
+    if (smem > SMEM_LIMIT) return SK_ERR_LIMIT;
+    const int grid = 2 * static_cast<int>(total < units ? total : units);
+    if (f32) e = sk_launch(sk_grouped_sum_kernel<true>, grid, TN_THREADS, smem, cs, 2, pdl, tmA, tmB, tmC, C, p);
+    else e = sk_launch(sk_grouped_sum_kernel<false>, grid, TN_THREADS, smem, cs, 2, pdl, tmA, tmB, tmC, C, p);
+    return e == cudaSuccess ? SK_OK : sk_set_cuda_error(e);
+  }
+
+  const int t32 = g->T < MAX_BN ? (g->T + 31) & ~31 : MAX_BN;
+  p.bn_max = t32;
+  p.tiles_f = (g->N + 255) / 256;
+  // (row tiles: at most one ragged one per group besides the full ones)
+  if ((static_cast<long long>(g->T) / p.bn_max + g->E + 1) * p.tiles_f > (1LL << 30)) return SK_ERR_LIMIT;
+  p.c_vec_ok = aligned(C, 16) && (g->ldc & 7) == 0;
+  // the box that a tile of bn_max rows loads, see the producer
+  const int half = p.bn_max / 2;
+  p.b_step_bytes = (half <= 16 ? 16 : half <= 64 ? 64 : 128) * 128;
+  const int fixed = 1024 + CTRL_BYTES + table_bytes(g->E);
+  p.stages = (SMEM_LIMIT - fixed) / (KG * (A_STEP_BYTES + p.b_step_bytes));
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  const int smem = fixed + p.stages * KG * (A_STEP_BYTES + p.b_step_bytes);
+  p.idesc = umma_idesc_f16(2 * HALF_M, 0, 0, bf16_bits) | (nn ? (1u << 15) : 0u);
+  CUtensorMap tmW, tmX[3];
+  st = nn ? make_map(&tmW, B, false, g->E, g->K, g->N, ldb, stride_b, 64, 64)
+          : make_map(&tmW, B, false, g->E, g->N, g->K, ldb, stride_b, 64, HALF_M);
+  const uint32_t boxes[3] = {16, 64, 128};
+  for (int i = 0; i < 3 && st == SK_OK; ++i) st = make_map(&tmX[i], A, false, 0, g->T, g->K, g->lda, 0, 64, boxes[i]);
+  if (st != SK_OK) return st;
+  const int grid = 2 * units;
+  uint16_t* c = static_cast<uint16_t*>(C);
+  if (nn)
+    e = sk_launch(sk_grouped_rows_kernel<true>, grid, NT_THREADS, smem, cs, 2, pdl, tmW, tmX[0], tmX[1], tmX[2], c, p);
+  else
+    e = sk_launch(sk_grouped_rows_kernel<false>, grid, NT_THREADS, smem, cs, 2, pdl, tmW, tmX[0], tmX[1], tmX[2], c, p);
+  return e == cudaSuccess ? SK_OK : sk_set_cuda_error(e);
+}

@@ -22,7 +22,8 @@ __all__ = [
     "streamk_fp32", "streamk_fp16_nn", "streamk_fp16_nt", "streamk_fp16_nt_host", "streamk_fp16_atomic",
     "streamk_fp16_block_reduce", "ladder_prepack", "streamk_fp16_ladder",
     "streamk_fp16_ladder_block_reduce", "q4_prepack", "dequant_w4",
-    "streamk_fp16_ladder_block_reduce_q4", "int8_quantize", "streamk_int8_nt", "schedule_info", "check_status",
+    "streamk_fp16_ladder_block_reduce_q4", "int8_quantize", "streamk_int8_nt",
+    "streamk_grouped_nt", "streamk_grouped_nn", "streamk_grouped_tn", "schedule_info", "check_status",
     "SCHEDULE_NAMES", "reset_workspace", "release_cached_memory", "cached_memory_bytes", "device_info", "LadderWeight", "PackedQ4", "StreamKError", "SCHEDULES", "FIXUPS",
 ]
 
@@ -664,3 +665,96 @@ def streamk_int8_nt(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, sca
                                     Cout.data_ptr(), ws.buf.data_ptr(), ws.nbytes, _stream_ptr(A.device)),
                 "sk_gemm_i8")
     return Cout
+
+
+# --------------------------------------------------------------------------- grouped by expert
+def _aligned16_batch(t: torch.Tensor) -> torch.Tensor:
+    """[E, R, C] 16-bit weights with 16-byte aligned rows (TMA), copied only if they have none."""
+    E, R, Cc = t.shape
+    if (t.stride(2) == 1 and t.stride(1) >= Cc and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0
+            and (E == 1 or (t.stride(0) >= R * t.stride(1) and t.stride(0) % 8 == 0))):
+        return t
+    n = torch.empty((E, R, -(-Cc // 8) * 8), dtype=t.dtype, device=t.device)
+    n[:, :, :Cc].copy_(t)
+    return n[:, :, :Cc]
+
+
+def _grouped(kind, A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl):
+    _check_matrix("A", A, HALF_TYPES)
+    if not isinstance(B, torch.Tensor) or not B.is_cuda:
+        raise ValueError("B must be a CUDA tensor (this library has no CPU path)")
+    if B.dtype != A.dtype:
+        raise TypeError(f"B must be {A.dtype} like A, got {B.dtype}")
+    if not isinstance(offsets, torch.Tensor) or offsets.device != A.device or B.device != A.device:
+        raise ValueError("A, B and offsets must be CUDA tensors on the same device")
+    if offsets.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"offsets must be int32 or int64, got {offsets.dtype}")
+    if offsets.dim() != 1 or offsets.shape[0] < 2:
+        raise ValueError(f"offsets must be 1-D with one more element than there are groups, got shape {tuple(offsets.shape)}")
+    T, K = A.shape
+    E = offsets.shape[0] - 1
+    dtype = A.dtype
+    if kind == "tn":
+        if B.dim() != 2 or B.shape[0] != T:
+            raise ValueError(f"Incompatible dimensions: A {tuple(A.shape)} B {tuple(B.shape)}")
+        N = B.shape[1]
+        dtype = dtype if out_dtype is None else out_dtype
+        if dtype not in (A.dtype, torch.float32):
+            raise TypeError(f"out_dtype must be {A.dtype} or torch.float32, got {dtype}")
+        shape = (E, K, N)
+    else:
+        if B.dim() != 3 or B.shape[0] != E or B.shape[2 if kind == "nt" else 1] != K:
+            raise ValueError(f"Incompatible dimensions: A {tuple(A.shape)} B {tuple(B.shape)} and {E} groups")
+        N = B.shape[1 if kind == "nt" else 2]
+        shape = (T, N)
+    _check_extents(N=N, K=K)
+    if out is not None and (out.shape != shape or out.dtype != dtype or out.device != A.device or out.stride(-1) != 1
+                            or out.stride(-2) < N or (kind == "tn" and E > 1 and out.stride(0) < K * out.stride(1))):
+        raise ValueError(f"out must be a row-major {list(shape)} tensor of type {dtype} on A's device")
+    with torch.cuda.device(A.device):
+        Cout = torch.empty(shape, dtype=dtype, device=A.device) if out is None else out
+        if T == 0:
+            return Cout.zero_() if kind == "tn" else Cout
+        A = _aligned16(_rowmajor(A))
+        B = _aligned16(_rowmajor(B)) if kind == "tn" else _aligned16_batch(B)
+        offsets = offsets.contiguous()
+        flags = ((L.SK_FLAG_BF16 if A.dtype == torch.bfloat16 else 0) | (L.SK_FLAG_PDL if pdl else 0)
+                 | (L.SK_FLAG_OFFSETS_64 if offsets.dtype == torch.int64 else 0)
+                 | (L.SK_FLAG_OUT_F32 if dtype == torch.float32 else 0)
+                 | (L.SK_FLAG_ZERO_REST if out is None and kind != "tn" else 0))
+        prob = L.SkGroupedProblem(L.GROUPED_KINDS[kind], T, E, N, K, int(num_sms or 0), int(timeout_us or 0), flags,
+                                  A.stride(0), B.stride(-2), Cout.stride(-2), B.stride(0) if kind != "tn" else 0,
+                                  Cout.stride(0) if kind == "tn" else 0)
+        ws = _workspace(A.device)
+        L.check(L.load().sk_gemm_grouped(C.byref(prob), A.data_ptr(), B.data_ptr(), offsets.data_ptr(), Cout.data_ptr(),
+                                         ws.buf.data_ptr(), ws.nbytes, _stream_ptr(A.device)), "sk_gemm_grouped")
+    return Cout
+
+
+def streamk_grouped_nt(A, B, offsets, *, out=None, num_sms=None, timeout_us=None, pdl=False):
+    """C[t] = B[e] @ A[t] for the group e that row t belongs to: the linear layers of a set of
+    experts.  A [T,K] and B [E,N,K] fp16 (or bf16), C [T,N] of the same type, fp32 accumulation.
+
+    The rows of A are sorted by group: group e holds rows offsets[e] .. offsets[e+1]; offsets is
+    an int32 or int64 CUDA tensor of E + 1 ascending numbers (nothing is read back by the host, so
+    the call can be captured and replayed with other sizes).  Groups may be empty.  Rows before
+    offsets[0] and from offsets[E] on belong to no group: zero in a fresh result, left as they
+    are in `out`.  Offsets out of order are clamped on the device and reported by check_status().
+    Its gradients: streamk_grouped_nn(dC, B, offsets) for A, streamk_grouped_tn(dC, A, offsets)
+    for B.  Operands whose rows are not 16-byte aligned are copied first.  No counterpart in the
+    reference."""
+    return _grouped("nt", A, B, offsets, out, None, num_sms, timeout_us, pdl)
+
+
+def streamk_grouped_nn(A, B, offsets, *, out=None, num_sms=None, timeout_us=None, pdl=False):
+    """C[t] = A[t] @ B[e]: A [T,K], B [E,K,N], C [T,N].  The input gradient of streamk_grouped_nt
+    (dA = streamk_grouped_nn(dC, B, offsets) with the same B [E,N,K]); otherwise the same rules."""
+    return _grouped("nn", A, B, offsets, out, None, num_sms, timeout_us, pdl)
+
+
+def streamk_grouped_tn(A, B, offsets, *, out=None, out_dtype=None, num_sms=None, timeout_us=None, pdl=False):
+    """C[e] = sum over the rows t of group e of outer(A[t], B[t]): A [T,K], B [T,N], C [E,K,N], zero
+    for an empty group.  The weight gradient of streamk_grouped_nt (dB = streamk_grouped_tn(dC, A,
+    offsets)).  out_dtype: the operands' type (default) or torch.float32 (unrounded sums).
+    Offsets as in streamk_grouped_nt; rows of no group, whatever they hold, do not count."""
+    return _grouped("tn", A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl)
