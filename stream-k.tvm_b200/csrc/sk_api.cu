@@ -194,12 +194,11 @@ void sk_resolve_auto(sk_problem* q, int kernel_kind, int num_sms) {
       }
     }
   }
-  const bool i8 = (q->flags & SK_FLAG_INTERNAL_I8) != 0;
   const int gemv_kind = sk_gemv_kind(kernel_kind, q->flags);
   // (W4A16: 9 to 16 rows cost the small-M kernel twice the instructions of 1 to 8: only where the
   // launch is short enough to be bound by latencies, at most one 32-row CTA per SM)
-  const int gemv_m = gemv_kind != 2 ? SK_GEMV_AUTO_M : (q->N <= 32LL * num_sms ? SK_GEMV_Q4_MAX_M : 8);
-  if (!i8 && tiles_open && q->M <= gemv_m && (kernel_kind == 2 || q->layout == SK_LAYOUT_NT)) {
+  const int gemv_m = gemv_kind == 4 ? SK_GEMV_I8_MAX_M : gemv_kind != 2 ? SK_GEMV_AUTO_M : (q->N <= 32LL * num_sms ? SK_GEMV_Q4_MAX_M : 8);
+  if (tiles_open && q->M <= gemv_m && (kernel_kind == 2 || q->layout == SK_LAYOUT_NT)) {
     // Few rows of activations: the weights stream once through a kernel without the tensor-core
     // kernels' fixed costs (tensor-memory allocation, mbarrier rings, a cluster exchange or a
     // workspace fix-up).  W4A16 with scale groups of 128 and more, whose small-M kernel takes
@@ -478,7 +477,7 @@ static int schedule_for(const sk_problem* p, int kernel_kind, int num_sms, int n
   }
   const int st = sk_make_sched(&q, kernel_kind, num_sms, out, nullptr, nullptr);
   if (st == SK_OK) out->schedule = q.schedule;
-  if (st == SK_OK && i8 && q.schedule != SK_SCHED_GEMV) out->tile_k *= 2;   // (bytes of K -> elements)
+  if (st == SK_OK && i8) out->tile_k *= 2;   // (bytes of K -> elements)
   return st;
 }
 

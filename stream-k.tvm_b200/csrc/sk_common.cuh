@@ -128,7 +128,8 @@ struct alignas(64) SkPeers {
 
 // ---------------------------------------------------------------------------------------
 // Small-M path (SK_SCHED_GEMV, sk_gemv.cu): how the grid is cut.  kernel_kind 1: fp16 / bf16;
-// 2: W4A16 with scale groups of 128 and more (M <= 16); 3: W4A16 with groups of 32 or 64 (M <= 4).
+// 2: W4A16 with scale groups of 128 and more (M <= 16); 3: W4A16 with groups of 32 or 64 (M <= 4);
+// 4: 8-bit integers (M <= 16; K counted in pairs of elements, see sk_i8_problem).
 //   fp16 / bf16: a row group is 128 weight rows; K is split across CTAs so that about four CTAs
 //     per SM are in flight, in units of 256 (one warp-wide 16-byte load per row), at most 2048
 //     per CTA (its activations sit in shared memory as fp32).
@@ -152,8 +153,42 @@ struct SkGemvPlan {
   int groups, splits, k_per_split, grid;
   int rows, slices, k_per_slice, threads;   // W4A16; fp16: 128, 1, k_per_split, 256
 };
+//   8-bit integers: a CTA takes 32 weight rows over all of K, its warps take steps of 128 bytes in
+//     turn, each with a ring of SK_GEMV_I8_DEPTH steps (4 KB each) in flight.  As many warps per
+//     CTA as let every CTA be resident at once, up to 16: all of the weights are then being
+//     asked for from the start, and an SM with one CTA more than another simply draws more of
+//     the bandwidth.  Few rows: K split across CTAs, at least eight steps each.
+constexpr int SK_GEMV_I8_MAX_M = 16;
+constexpr int SK_GEMV_I8_DEPTH = 3;
+constexpr int SK_GEMV_I8_STEP_BYTES = 32 * 128;
+inline bool sk_gemv_plan_i8(int M, int N, int K, int num_sms, SkGemvPlan* out) {
+  if (M < 1 || M > SK_GEMV_I8_MAX_M || N < 1 || K < 1 || num_sms < 1) return false;
+  const long long groups = (static_cast<long long>(N) + 31) / 32;
+  if (groups > 0x7fffffffLL / 64) return false;
+  const int steps = (K - 1) / 64 + 1;
+  int splits = 1;
+  if (2 * groups <= num_sms) {
+    splits = static_cast<int>(num_sms / groups);
+    if (splits > steps / 8) splits = steps / 8 > 1 ? steps / 8 : 1;
+  }
+  const int per_split = (steps + splits - 1) / splits;
+  splits = (steps + per_split - 1) / per_split;
+  const long long ctas = groups * splits;
+  int warps = ctas <= num_sms ? 16 : ctas <= 2LL * num_sms ? 8 : 4;
+  while (warps > 1 && warps > per_split) warps /= 2;
+  out->groups = static_cast<int>(groups);
+  out->splits = splits;
+  out->k_per_split = per_split * 64;
+  out->grid = static_cast<int>(ctas);
+  out->rows = 32;
+  out->slices = warps;
+  out->k_per_slice = (per_split + warps - 1) / warps * 64;
+  out->threads = 32 * warps;
+  return true;
+}
 inline bool sk_gemv_plan(int kernel_kind, int M, int N, int K, int num_sms, SkGemvPlan* out) {
-  if (kernel_kind < 1 || kernel_kind > 3) return false;
+  if (kernel_kind < 1 || kernel_kind > 4) return false;
+  if (kernel_kind == 4) return sk_gemv_plan_i8(M, N, K, num_sms, out);
   if (M < 1 || M > (kernel_kind == 2 ? SK_GEMV_Q4_MAX_M : SK_GEMV_MAX_M) || N < 1 || K < 1 || num_sms < 1) return false;
   if (kernel_kind != 1) {
     const long long groups = (static_cast<long long>(N) + 31) / 32;
@@ -213,12 +248,15 @@ inline bool sk_gemv_plan(int kernel_kind, int M, int N, int K, int num_sms, SkGe
   return true;
 }
 // The plan kind of an entry point's kernel kind (1: fp16, 2: W4A16) and problem flags.
+constexpr int SK_FLAG_INTERNAL_I8 = 1 << 30;   // see sk_i8_problem
 inline int sk_gemv_kind(int kernel_kind, int flags) {
-  if (kernel_kind != 2) return 1;
+  if (kernel_kind != 2) return (flags & SK_FLAG_INTERNAL_I8) ? 4 : 1;
   const int grp = flags & SK_FLAG_Q4_GROUP_MASK;
   return (grp == SK_FLAG_Q4_GROUP_32 || grp == SK_FLAG_Q4_GROUP_64) ? 3 : 2;
 }
 struct SkWorkspace;
+int sk_launch_gemv_i8(const sk_problem* prob, const void* A, const void* B, const float* scale_a, const float* scale_b,
+                      void* C, int k_elems, const SkWorkspace& ws, int num_sms, int dev_sms, void* stream);
 int sk_launch_gemv_f16(const sk_problem* prob, const void* A, const void* B, void* C, const SkWorkspace& ws,
                        int num_sms, int dev_sms, void* stream);
 int sk_launch_gemv_q4(const sk_problem* prob, const void* A, const void* qblocks, const void* szblocks, void* C,
@@ -285,7 +323,6 @@ unsigned long long* sk_trace_buffer();
 // 8-bit integer products (sk_gemm_i8) are planned as 16-bit ones of half the K: a K step, a
 // stage and a tile then hold the same bytes, which is what the scheduler's rules go by.
 // SK_FLAG_INTERNAL_I8 marks such a problem (the table of tuned 16-bit shapes is not for it).
-constexpr int SK_FLAG_INTERNAL_I8 = 1 << 30;
 inline sk_problem sk_i8_problem(const sk_problem* p) {
   sk_problem q = *p;
   q.K = p->K / 2 + (p->K & 1);

@@ -87,14 +87,21 @@ __device__ __forceinline__ void stage_activations(float* sA, const uint16_t* A, 
 
 // Partial sums of CTA (g, s) are at parts[((g * S + s) * M + m) * rows + row]; the last CTA of
 // group g to arrive adds them over s = 0 .. S-1 in that order and stores C[m][g * rows + row].
+// I8: the sums are 32-bit integers (bit patterns in float words), scaled where they become results.
+template <bool I8 = false>
 __device__ __forceinline__ void finish_group(const float* sums /* shared: [M][rows] */, int M, int rows, float* parts,
                                              uint32_t* counters, uint16_t* C, int ldc, int N, int g, int s,
-                                             int S, int bf16, int tid, int nthreads, uint32_t* s_last) {
+                                             int S, int bf16, int tid, int nthreads, uint32_t* s_last,
+                                             const float* scale_a = nullptr, const float* scale_b = nullptr) {
+  auto result = [&](float sum, int m, int n) {
+    if constexpr (I8) sum = (__int2float_rn(__float_as_int(sum)) * __ldg(scale_a + m)) * __ldg(scale_b + n);
+    return static_cast<uint16_t>(pack_out(sum, bf16));
+  };
   const int row0 = g * rows, items = M * rows;
   if (S == 1) {
     for (int i = tid; i < items; i += nthreads) {
       const int m = i / rows, r = i - m * rows;
-      if (row0 + r < N) C[static_cast<size_t>(m) * ldc + row0 + r] = static_cast<uint16_t>(pack_out(sums[i], bf16));
+      if (row0 + r < N) C[static_cast<size_t>(m) * ldc + row0 + r] = result(sums[i], m, row0 + r);
     }
     return;
   }
@@ -120,9 +127,12 @@ __device__ __forceinline__ void finish_group(const float* sums /* shared: [M][ro
         v[u] = __ldcg(all + static_cast<size_t>(j0 + u < S ? j0 + u : S - 1) * items + i);
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (j0 + u < S) acc += v[u];
+        if (j0 + u < S) {
+          if constexpr (I8) acc = __int_as_float(__float_as_int(acc) + __float_as_int(v[u]));
+          else acc += v[u];
+        }
     }
-    if (row0 + r < N) C[static_cast<size_t>(m) * ldc + row0 + r] = static_cast<uint16_t>(pack_out(acc, bf16));
+    if (row0 + r < N) C[static_cast<size_t>(m) * ldc + row0 + r] = result(acc, m, row0 + r);
   }
   if (tid == 0) counters[g] = 0u;   // zero between launches, like every counter of the workspace
 }
@@ -618,7 +628,174 @@ sk_gemv_q4_mma_kernel(const uint16_t* __restrict__ A, int lda, int M, const uint
   finish_group(sums, M, 32, parts, counters, C, ldc, N, g, s, S, 0, tid, nthreads, &s_last);
 }
 
+// ------------------------------------------------------------------------------ 8-bit integers
+// C[m][n] = sa[m] sb[n] sum_k A[m,k] B[n,k] for M <= 16, weights [N, K] row-major int8, through
+// register-level mma.sync (m16n8k32, 32-bit integer accumulators; exact, so any split of K gives
+// the same bits).  CTA (g, s) takes 32 weight rows over K range s; its warps take steps of 128
+// bytes of K in turn (warp w steps w, w + warps, ...: neighbouring lines of a row are asked for at
+// the same time), each through a ring of its own, filled by 16-byte asynchronous copies: eight
+// lanes to the 128 bytes of a row.
+//
+// Operand layout.  K may be dealt to the instruction's slots in any order that the weights and
+// the activations share.  Lane (g8 = lane / 4, t = lane % 4) takes the 16-byte pieces t and t + 4
+// of a row's 128: the words of a piece are, two by two, its slots of two instructions.  Rows g8,
+// g8 + 8 (and + 16, + 24 for the second operand tile) of the weights come from the ring; the
+// activations' pieces (row g8 of A) straight from global memory through L1, where every CTA of
+// the SM finds the same few KB.  Piece c of row r sits at c ^ 4 (r & 1), so that the eight lanes of
+// a quarter-warp, two rows of four pieces, read different banks.
+__device__ __forceinline__ void mma_16832_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// copies `bytes` (0 .. 16) and fills the rest of the 16 with zeros
+__device__ __forceinline__ void cp_async_16z(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+template <int NT>   // column tiles (eight rows of A each)
+__global__ void __launch_bounds__(GEMV_THREADS_Q4)
+sk_gemv_i8_kernel(const int8_t* __restrict__ A, int lda, int M, const int8_t* __restrict__ B, int ldb,
+                  const float* __restrict__ scale_a, const float* __restrict__ scale_b, uint16_t* __restrict__ C, int ldc,
+                  int N, int K, int steps, int per_split, int S, int bf16, float* parts, uint32_t* counters) {
+  constexpr int DEPTH = SK_GEMV_I8_DEPTH, STEP = SK_GEMV_I8_STEP_BYTES;
+  extern __shared__ __align__(128) uint8_t ring[];   // [warp][DEPTH][32 rows][128]; then red and sums
+  __shared__ uint32_t s_last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g8 = lane >> 2, t = lane & 3;
+  const int nthreads = blockDim.x, warps = nthreads >> 5;
+  const int g = blockIdx.x / S, s = blockIdx.x - g * S;
+  const int row0 = g * 32;
+  const int lo = s * per_split + warp;
+  const int hi = (s + 1) * per_split < steps ? (s + 1) * per_split : steps;
+  const uint32_t ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + warp * (DEPTH * STEP);
+  int acc[NT][2][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int T = 0; T < 2; ++T)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][T][e] = 0;
+  // copies: lane = (row of four, piece); instruction j takes rows 4 j + lane / 8
+  const int cr = lane >> 3, cp = lane & 7;
+  const int8_t* src[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int r = row0 + 4 * j + cr;
+    src[j] = B + static_cast<size_t>(r < N ? r : N - 1) * ldb + cp * 16;   // (rows past the end: never stored)
+  }
+  const uint32_t dst0 = ring_s + cr * 128 + ((cp ^ ((cr & 1) << 2)) << 4);
+  auto issue = [&](int i, int slot) {
+    const int k = i * 128 + cp * 16;
+    const int left = K - k, bytes = left >= 16 ? 16 : left > 0 ? left : 0;
+    const int off = left > 0 ? i * 128 : 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) cp_async_16z(dst0 + slot * STEP + j * 512, src[j] + off, bytes);
+  };
+  skptx::griddep_wait();
+  int next = lo, fill = 0;
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) {
+    if (next < hi) issue(next, d);
+    cp_async_commit();
+    next += warps;
+  }
+  const int8_t* a[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) a[n] = A + static_cast<size_t>(8 * n + g8 < M ? 8 * n + g8 : M - 1) * lda + t * 16;
+  const uint32_t frag = ring_s + g8 * 128 + ((t ^ ((g8 & 1) << 2)) << 4);
+  for (int i = lo; i < hi; i += warps) {
+    // (a piece past K meets zero weights: any readable address will do)
+    uint4 x[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = i * 128 + h * 64;
+        x[n][h] = ld_cached_v4(a[n] + (k + t * 16 < K ? k : -t * 16));
+      }
+    cp_async_wait<DEPTH - 1>();
+    __syncwarp();
+    uint4 w[2][4];   // piece t / t + 4, rows g8 + 8 j
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[h][j] = lds_v4((frag ^ (h << 6)) + fill * STEP + j * 1024);
+    __syncwarp();
+    if (next < hi) issue(next, fill);
+    cp_async_commit();
+    next += warps;
+    if (++fill == DEPTH) fill = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          const uint4 &u = w[h][2 * T], &v = w[h][2 * T + 1];
+          mma_16832_s8(acc[n][T], u.x, v.x, u.y, v.y, x[n][h].x, x[n][h].y);
+          mma_16832_s8(acc[n][T], u.z, v.z, u.w, v.w, x[n][h].z, x[n][h].w);
+        }
+  }
+  cp_async_wait<0>();
+  skptx::griddep_launch_dependents();
+  int* red = reinterpret_cast<int*>(ring + warps * (DEPTH * STEP));    // [warp][m][row of the CTA]
+  float* sums = reinterpret_cast<float*>(red + warps * M * 32);        // [m][row]
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int T = 0; T < 2; ++T)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int m = 8 * n + 2 * t + (e & 1);
+        if (m < M) red[(warp * M + m) * 32 + 16 * T + 8 * (e >> 1) + g8] = acc[n][T][e];
+      }
+  __syncthreads();
+  for (int i = tid; i < M * 32; i += nthreads) {
+    int v = red[i];
+    for (int j = 1; j < warps; ++j) v += red[j * M * 32 + i];
+    sums[i] = __int_as_float(v);
+  }
+  __syncthreads();
+  finish_group<true>(sums, M, 32, parts, counters, C, ldc, N, g, s, S, bf16, tid, nthreads, &s_last, scale_a, scale_b);
+}
+
 }  // namespace
+
+int sk_launch_gemv_i8(const sk_problem* prob, const void* A, const void* B, const float* scale_a, const float* scale_b,
+                      void* C, int k_elems, const SkWorkspace& ws, int num_sms, int dev_sms, void* stream) {
+  SkGemvPlan pl;
+  if (!sk_gemv_plan(4, prob->M, prob->N, prob->K, num_sms, &pl)) return SK_ERR_SHAPE;
+  if (pl.splits > 1 && pl.groups > 4 * dev_sms) return SK_ERR_LIMIT;   // (splits > 1: at most half an SM count of groups)
+  if (static_cast<size_t>(pl.splits > 1 ? pl.grid : 0) * prob->M * 32 * sizeof(float) >
+      2 * static_cast<size_t>(dev_sms) * SK_SLOT_BYTES)
+    return SK_ERR_LIMIT;
+  const bool pdl = (prob->flags & SK_FLAG_PDL) != 0;
+  const int warps = pl.slices;
+  const size_t smem = static_cast<size_t>(warps) * SK_GEMV_I8_DEPTH * SK_GEMV_I8_STEP_BYTES +
+                      static_cast<size_t>(warps + 1) * prob->M * 32 * sizeof(int);
+  constexpr size_t smem_max = static_cast<size_t>(16) * SK_GEMV_I8_DEPTH * SK_GEMV_I8_STEP_BYTES +
+                              static_cast<size_t>(17) * SK_GEMV_I8_MAX_M * 32 * sizeof(int);
+  static_assert(smem_max + 64 <= 232448, "shared memory of the largest CTA");
+  static SkPerDeviceOnce attrs;
+  cudaError_t e = attrs.run([]() {
+    cudaError_t r = cudaFuncSetAttribute(sk_gemv_i8_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_max);
+    if (r == cudaSuccess)
+      r = cudaFuncSetAttribute(sk_gemv_i8_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_max);
+    return r;
+  });
+  if (e != cudaSuccess) return sk_set_cuda_error(e);
+  const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const int steps = (prob->K - 1) / 64 + 1, per_split = pl.k_per_split / 64;
+  const int bf16 = (prob->flags & SK_FLAG_BF16) ? 1 : 0;
+  auto kernel = prob->M <= 8 ? sk_gemv_i8_kernel<1> : sk_gemv_i8_kernel<2>;
+  e = sk_launch(kernel, pl.grid, pl.threads, smem, cs, 1, pdl, static_cast<const int8_t*>(A), 2 * prob->lda, prob->M,
+                static_cast<const int8_t*>(B), 2 * prob->ldb, scale_a, scale_b, static_cast<uint16_t*>(C), prob->ldc,
+                prob->N, k_elems, steps, per_split, pl.splits, bf16, ws.part_slots, ws.counters);
+  return e == cudaSuccess ? SK_OK : sk_set_cuda_error(e);
+}
 
 // Launchers, called by sk_gemm_f16 / sk_gemm_w4a16 once the schedule has resolved to
 // SK_SCHED_GEMV (their argument checks have run).  ws: carved workspace of the device.

@@ -8,16 +8,18 @@
 // |x| order like the numbers do, so the maximum is one packed integer instruction per pair, and
 // NaN and infinity are whatever ends up at or above the infinity's pattern.
 //
-// The rounding goes by the exact quotient.  With b = a * 2^-e (between 1 and 4), x' = x * 2^-e
-// (exact: both are 11-bit numbers or shorter, and what underflows rounds to zero anyway) and
-// r = 127 / b rounded, t = x' r is within 2^-23 of the quotient, relatively.  The quotient is
-// either half of an odd number or at least 2^-20 away from one, relatively: 254 x' and
-// (odd) b are multiples of x''s last place whose difference, if it is not zero, is at least that
-// place.  So rounding t rounds the quotient, except where the quotient IS a half: there t may
-// sit on either side, and the remainder 127 x' - q b, which fp32 holds exactly (18 bits less 18
-// bits of the same place), is plus or minus b / 2.  An odd q is then moved to the even side.
+// The rounding goes by the exact quotient Q = 127 x / a.  With r = 127 / a rounded, t = x r is
+// within 2^-22 of Q, relatively, i.e. 3.1e-5 at most: where t is not that near to a half, rounding
+// it rounds Q.  The rest (one element in ten thousand) goes through exact arithmetic: with
+// b = a 2^-e (between 1 and 4) and x' = x 2^-e (exact: both are 11-bit numbers or shorter, and what
+// underflows rounds to zero anyway) Q is either half of an odd number or at least 2^-20 away from
+// one, relatively: 254 x' and (odd) b are multiples of x's last place whose difference, if it is
+// not zero, is at least that place.  So rounding x' (127 / b) rounds Q, except where Q IS a half:
+// there it may fall on either side, and the remainder 127 x' - q b, which fp32 holds exactly (18
+// bits less 18 bits of the same place), is plus or minus b / 2.  An odd q is then moved to the
+// even side.  Rows whose a is so small that 127 / a overflows take the exact way throughout.
 //
-// Bound: memory (2 bytes read, 1 written per element; about nine instructions per element).
+// Bound: memory (2 bytes read, 1 written per element; about seven instructions per element).
 #include "sk_common.cuh"
 
 namespace {
@@ -63,14 +65,22 @@ __device__ __forceinline__ float widen(uint32_t bits16) {
   else return __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
 }
 
+template <bool BF16>
+__device__ __forceinline__ float widen_high(uint32_t pair) {
+  if constexpr (BF16) return __uint_as_float(pair & 0xFFFF0000u);
+  else return widen<false>(pair >> 16);
+}
+
 struct RowScale {
+  float q;            // 127 / a; negative: not usable, every element takes the exact way
   float pow2, b, r;   // 2^-e, a * 2^-e, 127 / b
 };
 
-// One element: 127 x / a to the nearest integer, halves to even; the low byte holds it.
+constexpr float ROUND = 12582912.f;   // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
+
+// One element, exactly: 127 x / a to the nearest integer, halves to even; the low byte holds it.
 template <bool BF16>
 __device__ __forceinline__ uint32_t quantize1(uint32_t bits16, const RowScale& s) {
-  constexpr float ROUND = 12582912.f;   // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
   const float x = widen<BF16>(bits16) * s.pow2;
   const float m = __fmaf_rn(x, s.r, ROUND);
   const float q = m - ROUND;
@@ -84,8 +94,19 @@ template <bool BF16>
 __device__ __forceinline__ uint2 quantize8(const uint4& v, const RowScale& s) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t u[8];
+  float off = s.q;   // the largest distance between an element's t and its integer
+  off = off < 0.f ? 1.f : 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) u[j] = quantize1<BF16>(w[j >> 1] >> (16 * (j & 1)) & 0xFFFFu, s);
+  for (int j = 0; j < 8; ++j) {
+    const float t = ((j & 1) ? widen_high<BF16>(w[j >> 1]) : widen<BF16>(w[j >> 1] & 0xFFFFu)) * s.q;
+    const float m = t + ROUND;
+    u[j] = __float_as_uint(m);
+    off = fmaxf(off, fabsf(t - (m - ROUND)));
+  }
+  if (off >= 0.49995f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = quantize1<BF16>(w[j >> 1] >> (16 * (j & 1)) & 0xFFFFu, s);
+  }
   uint2 q;
   q.x = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
   q.y = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
@@ -138,8 +159,9 @@ sk_quantize_i8_kernel(const uint16_t* __restrict__ X, int M, int K, int ldx, int
     s.pow2 = __uint_as_float(static_cast<uint32_t>(e > 1 ? e : 1) << 23);
     s.b = a * s.pow2;
     s.r = __fdiv_rn(127.f, s.b);
+    s.q = a >= 0x1p-100f ? __fdiv_rn(127.f, a) : -1.f;
   } else {
-    s.pow2 = 0.f; s.b = 1.f; s.r = 0.f;
+    s.q = 0.f; s.pow2 = 0.f; s.b = 1.f; s.r = 0.f;
   }
   int8_t* q = Q + row * ldq;
   if constexpr (NV > 0) {
@@ -173,6 +195,7 @@ cudaError_t dispatch(const uint16_t* X, int M, int K, int ldx, int8_t* Q, int ld
   const int vecs = K / 8 + ((K & 7) != 0);
   if (vecs <= 32 * 4) return launch<BF16, VEC, 32, 4>(X, M, K, ldx, Q, ldq, scale, pdl, stream);
   if (vecs <= 256 * 2) return launch<BF16, VEC, 256, 2>(X, M, K, ldx, Q, ldq, scale, pdl, stream);
+  if (vecs <= 256 * 4) return launch<BF16, VEC, 256, 4>(X, M, K, ldx, Q, ldq, scale, pdl, stream);
   if (vecs <= 256 * 6) return launch<BF16, VEC, 256, 6>(X, M, K, ldx, Q, ldq, scale, pdl, stream);
   if (vecs <= 1024 * 4) return launch<BF16, VEC, 1024, 4>(X, M, K, ldx, Q, ldq, scale, pdl, stream);
   return launch<BF16, VEC, 1024, 0>(X, M, K, ldx, Q, ldq, scale, pdl, stream);

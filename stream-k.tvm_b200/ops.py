@@ -11,6 +11,7 @@ Everything runs on the GPU through libstreamk_b200.so; there is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from dataclasses import dataclass
 
@@ -55,8 +56,24 @@ class _Workspace:
 _workspaces: dict[tuple[int, int], _Workspace] = {}
 
 
+# The host side of a call costs more than many of the kernels: the raw stream handle comes
+# straight from the runtime binding where torch has it (0.1 us against 2.4), and the device is
+# switched only if another one is current (1.5 us a switch).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device() if device.index is None else device.index)
     return int(torch.cuda.current_stream(device).cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Context manager: `device` is current inside."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _workspace(device: torch.device) -> _Workspace:
@@ -248,7 +265,7 @@ def streamk_fp32(A: torch.Tensor, B: torch.Tensor, *, fixup: str = "atomic",
     Cout = _out(o["out"], M, N, torch.float32, A.device)
     prob = _problem(M, N, K, A.stride(0), B.stride(0), Cout.stride(0), "nt" if trans_b else "nn",
                     schedule, fixup, o)
-    with torch.cuda.device(A.device):
+    with _on(A.device):
         ws = _workspace(A.device)
         L.check(L.load().sk_gemm_f32(C.byref(prob), A.data_ptr(), B.data_ptr(), Cout.data_ptr(),
                                      ws.buf.data_ptr(), ws.nbytes, _stream_ptr(A.device)),
@@ -291,7 +308,7 @@ def _gemm_f16(A, B, layout, fixup, schedule, kw):
         ldb = Bt.stride(0)
     Cout = _out(o["out"], M, N, dtype, A.device)
     prob = _problem(M, N, A.shape[1], A.stride(0), ldb, Cout.stride(0), layout, schedule, fixup, o)
-    with torch.cuda.device(A.device):
+    with _on(A.device):
         ws = _workspace(A.device)
         L.check(L.load().sk_gemm_f16(C.byref(prob), A.data_ptr(), Bt.data_ptr(), Cout.data_ptr(),
                                      ws.buf.data_ptr(), ws.nbytes, _stream_ptr(A.device)),
@@ -574,7 +591,7 @@ def streamk_fp16_ladder_block_reduce_q4(A, QLB: PackedQ4, *, fixup="block_reduce
     Cout = _out(o["out"], M, QLB.N, torch.float16, A.device)
     prob = _problem(M, QLB.N, K, A.stride(0), 0, Cout.stride(0), "nt", schedule, fixup, o)
     prob.flags |= L.SK_FLAG_Q4_GROUP[QLB.group_size]
-    with torch.cuda.device(A.device):
+    with _on(A.device):
         ws = _workspace(A.device)
         L.check(L.load().sk_gemm_w4a16(C.byref(prob), A.data_ptr(), QLB.data.data_ptr(),
                                        Cout.data_ptr(), ws.buf.data_ptr(), ws.nbytes,
@@ -601,16 +618,15 @@ def int8_quantize(X: torch.Tensor, *, pdl: bool = False) -> tuple[torch.Tensor, 
     Q = torch.empty((M, pitch), dtype=torch.int8, device=X.device)
     scale = torch.empty(M, dtype=torch.float32, device=X.device)
     flags = (L.SK_FLAG_BF16 if X.dtype == torch.bfloat16 else 0) | (L.SK_FLAG_PDL if pdl else 0)
-    with torch.cuda.device(X.device):
+    with _on(X.device):
         L.check(L.load().sk_quantize_i8(X.data_ptr(), M, K, X.stride(0) if M > 1 else K, flags, Q.data_ptr(), pitch,
                                         scale.data_ptr(), _stream_ptr(X.device)), "sk_quantize_i8")
-    return Q[:, :K], scale
+    return (Q if pitch == K else Q[:, :K]), scale
 
 
 def _check_extents(**extents) -> None:
-    for name, v in extents.items():
-        if v < 1:
-            raise ValueError(f"{name} must be at least 1, got {v}")
+    if min(extents.values()) < 1:
+        raise ValueError(f"extents must be at least 1, got {extents}")
 
 
 def _check_scale(name: str, s: torch.Tensor, n: int, device) -> torch.Tensor:
@@ -618,6 +634,8 @@ def _check_scale(name: str, s: torch.Tensor, n: int, device) -> torch.Tensor:
         raise ValueError(f"{name} must be a CUDA tensor on the operands' device")
     if s.dtype != torch.float32:
         raise TypeError(f"{name} must be torch.float32, got {s.dtype}")
+    if s.shape == (n,) and s.is_contiguous():
+        return s
     if s.shape not in ((n,), (n, 1), (1, n)):
         raise ValueError(f"{name} must have {n} elements, got shape {tuple(s.shape)}")
     return s.reshape(n).contiguous()
@@ -654,7 +672,7 @@ def streamk_int8_nt(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, sca
     if K != Kb:
         raise ValueError(f"Incompatible dimensions: A {tuple(A.shape)} B {tuple(B.shape)}")
     _check_extents(M=M, N=N, K=K)
-    with torch.cuda.device(A.device):
+    with _on(A.device):
         scale_a = _check_scale("scale_a", scale_a, M, A.device)
         scale_b = _check_scale("scale_b", scale_b, N, A.device)
         A, B = _rows16(A), _rows16(B)
@@ -711,7 +729,7 @@ def _grouped(kind, A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl):
     if out is not None and (out.shape != shape or out.dtype != dtype or out.device != A.device or out.stride(-1) != 1
                             or out.stride(-2) < N or (kind == "tn" and E > 1 and out.stride(0) < K * out.stride(1))):
         raise ValueError(f"out must be a row-major {list(shape)} tensor of type {dtype} on A's device")
-    with torch.cuda.device(A.device):
+    with _on(A.device):
         Cout = torch.empty(shape, dtype=dtype, device=A.device) if out is None else out
         if T == 0:
             return Cout.zero_() if kind == "tn" else Cout
