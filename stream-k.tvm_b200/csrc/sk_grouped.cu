@@ -12,7 +12,7 @@
 //
 // NT and NN: CTA pairs (cta_group::2).  The weights feed the UMMA M dimension (256 of the N output
 // features per pair, 128 per CTA) and the rows of a group the UMMA N dimension, whose extent the
-// instruction descriptor sets tile by tile in steps of 32: a group of 5 rows costs the tensor
+// instruction descriptor sets tile by tile in steps of 16: a group of 5 rows costs the tensor
 // cores 32 columns and a group of 300 two tiles of 160, where rows on the M side would cost whole
 // multiples of 128 or 256.  Groups of a few rows are then what they should be, a stream of the
 // weights.  A pair's accumulator is transposed (lane = feature, column = row of A): 32 lanes
@@ -48,10 +48,11 @@ struct GroupedParams {
   int bn_max;                // most rows of a group per tile (NT / NN): a multiple of 32
   int tiles_f;               // tiles along the UMMA M side (NT / NN: of N; TN: of K)
   int tiles_n;               // TN: tiles of N
+  int band;                  // TN: tiles of K that are walked side by side
+  SkDiv d_band, d_in, d_last;   // / (band * tiles_n), / band, / the last band's tiles
   int stages;
   int b_step_bytes;          // shared memory per step of this CTA's half of the UMMA N operand
   int zero_rest;             // NT / NN: rows of C that belong to no group are set to zero
-  int out_bf16;
   int c_vec_ok;              // rows of C can take 16-byte stores
   int c_tma;                 // TN: C leaves through TMA stores
   uint32_t idesc;            // with N = 0
@@ -72,7 +73,7 @@ static_assert(sizeof(Ctrl) <= CTRL_BYTES, "Ctrl must fit its reserved space");
 
 __host__ __device__ constexpr int align_up(int v, int a) { return (v + a - 1) / a * a; }
 // Group table in shared memory: start[E + 1], then (NT / NN) first[E + 1], the first row tile.
-__host__ __device__ constexpr int table_bytes(int E) { return align_up(2 * (E + 1) * 4, 16); }
+__host__ __device__ constexpr int table_bytes(int E, bool tiles) { return align_up((tiles ? 2 : 1) * (E + 1) * 4, 16); }
 
 // Fills the table.  Called by every thread; ends with the table visible to all.
 __device__ __forceinline__ void make_table(const GroupedParams& p, int* start, int* first) {
@@ -105,6 +106,9 @@ __device__ __forceinline__ void make_table(const GroupedParams& p, int* start, i
       if (s < top) s = top;
       int before = __shfl_up_sync(0xffffffffu, s, 1);
       if (lane == 0) before = prev_start;
+      if (i <= p.E) start[i] = s;
+      top = prev_start = __shfl_sync(0xffffffffu, s, 31);
+      if (first == nullptr) continue;
       // tiles of group i - 1 (rows before .. s): first[i] = tiles of groups 0 .. i - 1
       int t = i > 0 && i <= p.E ? (s - before + p.bn_max - 1) / p.bn_max : 0;
 #pragma unroll
@@ -113,11 +117,7 @@ __device__ __forceinline__ void make_table(const GroupedParams& p, int* start, i
         if (lane >= d) t += o;
       }
       t += sum;
-      if (i <= p.E) {
-        start[i] = s;
-        first[i] = t;
-      }
-      top = prev_start = __shfl_sync(0xffffffffu, s, 31);
+      if (i <= p.E) first[i] = t;
       sum = __shfl_sync(0xffffffffu, t, 31);
     }
   }
@@ -129,7 +129,7 @@ struct RowTile {
   int e;          // group
   int f0;         // first output feature of the pair's 256
   int r0, rows;   // rows of A
-  int bn;         // UMMA N: rows rounded up to 32
+  int bn;         // UMMA N: rows rounded up to 16, at least 32
 };
 
 // Walks the tiles unit, unit + grid, ...: group by group, inside a group bands of up to eight row
@@ -155,7 +155,7 @@ struct RowWalk {
     o.f0 = f * (2 * HALF_M);
     o.r0 = start[e] + m * per;
     o.rows = rows - m * per < per ? rows - m * per : per;
-    o.bn = o.rows > 0 ? (o.rows + 31) & ~31 : 32;
+    o.bn = o.rows > 16 ? (o.rows + 15) & ~15 : 32;
     t += units;
     return true;
   }
@@ -163,8 +163,8 @@ struct RowWalk {
 
 constexpr int NT_THREADS = 64 + 32 * EPI_WARPS;   // warp 0 producer, 1 MMA issuer, 2..9 epilogue
 
-// W_MN: the weights are MN-major (NN): two boxes of 64 features x 64 of K per step.
-template <bool W_MN>
+// W_MN: the weights are MN-major (NN): two boxes of 64 features x 64 of K per step.  BF16: C's type.
+template <bool W_MN, bool BF16>
 __global__ void __launch_bounds__(NT_THREADS, 1)
 sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX16,
                        const __grid_constant__ CUtensorMap tmX64, const __grid_constant__ CUtensorMap tmX128,
@@ -179,7 +179,7 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
   int* start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ctrl) + CTRL_BYTES);
   int* first = start + p.E + 1;
   volatile uint32_t* abort_flag = &ctrl->abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
 
@@ -198,8 +198,8 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
     fence_proxy_async_smem();
     prefetch_tensormap(&tmW);
     prefetch_tensormap(&tmX16);
-    prefetch_tensormap(&tmX64);
-    prefetch_tensormap(&tmX128);
+    if (p.bn_max > 32) prefetch_tensormap(&tmX64);
+    if (p.bn_max > 128) prefetch_tensormap(&tmX128);
   }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(&ctrl->tmem_base), TMEM_COLS);
@@ -216,9 +216,12 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
   RowWalk walk{unit, 0};
   RowTile tile;
 
+  // (The single-thread roles are run by their whole warp, with the TMA, mbarrier and tcgen05
+  // instructions behind an elected lane: warp-uniform code issues them at half the cost.)
   if (warp == 0) {
     // ------------------------------------------------------------- producer (both CTAs)
-    if (lane == 0) {
+    {
+      const bool leader = elect_one();
       int stage = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -237,8 +240,8 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
             break;
           }
           const uint32_t bar = full0_leader + 8u * stage;
-          if (rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, n * tx);
-          for (int j = 0; j < n; ++j) {
+          if (leader && rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, n * tx);
+          for (int j = 0; leader && j < n; ++j) {
             const uint32_t dW = sW + (stage * KG + j) * A_STEP_BYTES;
             if constexpr (W_MN) {
               tma_load_3d_pair(dW, &tmW, bar, f_row, (k + j) * BK, tile.e);
@@ -255,7 +258,8 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA issuer (leader)
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool leader = elect_one();
       int stage = 0;
       uint32_t ph = 0, nseg = 0;
       bool ok = true;
@@ -282,16 +286,17 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
             const uint32_t x_lo = x_lo0 + (stage * KG + j) * (static_cast<uint32_t>(p.b_step_bytes) >> 4);
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
-              umma_f16_ss_pair(d_tmem, w_hi | (w_lo + kk * w_kstep16), x_hi | (x_lo + kk * 2), idesc, accumulate);
+              if (leader)
+                umma_f16_ss_pair(d_tmem, w_hi | (w_lo + kk * w_kstep16), x_hi | (x_lo + kk * 2), idesc, accumulate);
               accumulate = 1u;
             }
           }
-          umma_commit_pair(empty0 + 8u * stage);
+          if (leader) umma_commit_pair(empty0 + 8u * stage);
           k += n;
           if (++stage == STAGES) { stage = 0; ph ^= 1u; }
         }
         if (!ok) break;
-        umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));
+        if (leader) umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));
         ++nseg;
       }
     }
@@ -335,12 +340,12 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
           const int nv = tile.rows - c;
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (f_ok && j < nv) dst[j * p.ldc] = static_cast<uint16_t>(sk_pack2(v[j], 0.f, p.out_bf16));
+            if (f_ok && j < nv) dst[j * p.ldc] = static_cast<uint16_t>(sk_pack2(v[j], 0.f, BF16));
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tmem_empty0 + 8u * buf);
+      if (lane == 0) mbar_arrive_cluster_relaxed(tmem_empty0 + 8u * buf);
     }
   }
 
@@ -366,18 +371,17 @@ struct SumTile {
 };
 
 struct SumWalk {
-  int t;
+  int t, e;   // tile of group e (it may still lie in a later group)
   __device__ __forceinline__ bool next(const GroupedParams& p, const int* start, int units, SumTile& o) {
     const int per_e = p.tiles_f * p.tiles_n;
-    if (t >= p.E * per_e) return false;
-    const int e = t / per_e;
-    int local = t - e * per_e;
-    const int band = local / (8 * p.tiles_n);
-    local -= band * 8 * p.tiles_n;
-    const int in_band = p.tiles_f - band * 8 < 8 ? p.tiles_f - band * 8 : 8;
-    const int n = local / in_band;
+    while (t >= per_e && e < p.E) { t -= per_e; ++e; }
+    if (e >= p.E) return false;
+    const int band = sk_div(t, p.d_band);
+    const int local = t - band * p.band * p.tiles_n;
+    const int left = p.tiles_f - band * p.band;
+    const int n = sk_div(local, left < p.band ? p.d_last : p.d_in);
     o.e = e;
-    o.f0 = (band * 8 + (local - n * in_band)) * (2 * HALF_M);
+    o.f0 = (band * p.band + (local - n * (left < p.band ? left : p.band))) * (2 * HALF_M);
     o.c0 = n * MAX_BN;
     o.r0 = start[e];
     o.rows = start[e + 1] - start[e];
@@ -387,16 +391,17 @@ struct SumWalk {
 };
 
 constexpr int TN_THREADS = NT_THREADS + 32;   // one warp more: it zeroes what lies past a group's end
-constexpr int TN_STAGES = 5;                  // one step each
 constexpr int TN_B_STEP = 128 * BK * 2;
-constexpr int TN_PIPE = TN_STAGES * (A_STEP_BYTES + TN_B_STEP);
+constexpr int TN_STEP = A_STEP_BYTES + TN_B_STEP;   // a stage holds one step
 
 // Does step k of a group of `rows` rows hold a UMMA that reaches past the group's end?
 __device__ __forceinline__ bool step_needs_zeros(int k, int rows) {
   return (k + 1) * BK > rows && (rows & 15) != 0;
 }
 
-template <bool F32>
+constexpr int OUT_F16 = 0, OUT_BF16 = 1, OUT_F32 = 2;   // type of C
+
+template <int OUT>
 __global__ void __launch_bounds__(TN_THREADS, 1)
 sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmC, void* __restrict__ Cv, const GroupedParams p) {
@@ -404,14 +409,13 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw_addr);
-  constexpr int STAGES = TN_STAGES;
+  const int STAGES = p.stages;
   const uint32_t sA = base, sB = base + STAGES * A_STEP_BYTES;
-  const uint32_t cstage = base + TN_PIPE;                    // 8 x 4 KB staging of the TMA stores
-  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + TN_PIPE + EPI_WARPS * 4096);
+  const uint32_t cstage = base + STAGES * TN_STEP;           // 8 x 4 KB staging of the TMA stores
+  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + STAGES * TN_STEP + EPI_WARPS * 4096);
   int* start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ctrl) + CTRL_BYTES);
-  int* first = start + p.E + 1;
   volatile uint32_t* abort_flag = &ctrl->abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
 
@@ -439,18 +443,19 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     tmem_relinquish_pair();
   }
   griddep_wait();
-  make_table(p, start, first);
+  make_table(p, start, nullptr);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&ctrl->tmem_base);
-  SumWalk walk{unit};
+  SumWalk walk{unit, 0};
   SumTile tile;
 
   if (warp == 0) {
     // ------------------------------------------------------------- producer (both CTAs)
-    if (lane == 0) {
+    {
+      const bool leader = elect_one();
       int stage = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -471,16 +476,18 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           const bool tail = step_needs_zeros(k, tile.rows);
           constexpr uint32_t bytes = A_STEP_BYTES + TN_B_STEP;
           uint32_t bar = full0_leader + 8u * stage;
-          if (tail) {
-            if (rank == 0) mbar_arrive(full0 + 8u * stage);
-            bar = tail0 + 8u * stage;
-            mbar_arrive_expect_tx(bar, bytes);
-          } else if (rank == 0) {
-            mbar_arrive_expect_tx(full0 + 8u * stage, 2 * bytes);
+          if (tail) bar = tail0 + 8u * stage;
+          if (leader) {
+            if (tail) {
+              if (rank == 0) mbar_arrive(full0 + 8u * stage);
+              mbar_arrive_expect_tx(bar, bytes);
+            } else if (rank == 0) {
+              mbar_arrive_expect_tx(full0 + 8u * stage, 2 * bytes);
+            }
           }
           const uint32_t dA = sA + stage * A_STEP_BYTES, dB = sB + stage * TN_B_STEP;
           const int row = tile.r0 + k * BK;
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; leader && h < 2; ++h) {
             if (tail) {
               tma_load_2d(dA + h * 8192, &tmA, bar, a_col + h * 64, row);
               tma_load_2d(dB + h * 8192, &tmB, bar, b_col + h * 64, row);
@@ -495,7 +502,8 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA issuer (leader)
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool leader = elect_one();
       int stage = 0;
       uint32_t ph = 0, nseg = 0, tail_ph = 0;
       bool ok = true;
@@ -527,16 +535,17 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           tc_fence_after();
           const uint32_t a_lo = a_lo0 + stage * (A_STEP_BYTES >> 4), b_lo = b_lo0 + stage * (TN_B_STEP >> 4);
           const int left = tile.rows - k * BK;              // rows of the group in this step
-          const int mmas = left >= BK ? BK / 16 : (left + 15) >> 4;
-          for (int kk = 0; kk < mmas; ++kk) {
-            umma_f16_ss_pair(d_tmem, hi | (a_lo + kk * 128), hi | (b_lo + kk * 128), idesc, accumulate);
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            if (leader && kk * 16 < left)
+              umma_f16_ss_pair(d_tmem, hi | (a_lo + kk * 128), hi | (b_lo + kk * 128), idesc, accumulate);
             accumulate = 1u;
           }
-          umma_commit_pair(empty0 + 8u * stage);
+          if (leader) umma_commit_pair(empty0 + 8u * stage);
           if (++stage == STAGES) { stage = 0; ph ^= 1u; }
         }
         if (!ok) break;
-        umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));
+        if (leader) umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));
         ++nseg;
       }
     }
@@ -579,6 +588,7 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     const uint32_t tmem_full0 = smem_u32(&ctrl->tmem_full[0]);
     const uint32_t tmem_empty0 = mapa_shared(smem_u32(&ctrl->tmem_empty[0]), 0);
     const uint32_t buf_smem = cstage + static_cast<uint32_t>(warp - 2) * 4096u;
+    constexpr bool F32 = OUT == OUT_F32;
     constexpr int gcols = F32 ? 32 : 64;            // columns of a 128-byte row of the staging buffer
     uint32_t nseg = 0;
     bool dead = false;
@@ -600,14 +610,20 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       if (!dead && r0 < p.K) {
         for (int c = sub * gcols; c < valid; c += 2 * gcols) {
           float v[gcols / 32][32];
+          if (some) {
+            uint32_t raw[gcols / 32][32];
 #pragma unroll
-          for (int h = 0; h < gcols / 32; ++h) {
-            if (some) {
-              sk_load_acc(t_addr + c + h * 32, 0, v[h]);
-            } else {
+            for (int h = 0; h < gcols / 32; ++h) tmem_ld_32x32(t_addr + c + h * 32, raw[h]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int h = 0; h < gcols / 32; ++h)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[h][j] = __uint_as_float(raw[h][j]);
+          } else {
+#pragma unroll
+            for (int h = 0; h < gcols / 32; ++h)
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[h][j] = 0.f;
-            }
           }
           if (p.c_tma) {
             if (lane == 0) tma_store_wait_read<0>();
@@ -620,8 +636,9 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
                 st_shared_v4(a, v[0][4 * j], v[0][4 * j + 1], v[0][4 * j + 2], v[0][4 * j + 3]);
               } else {
                 const float* w = &v[j >> 2][(j & 3) * 8];
-                const uint32_t h0 = sk_pack2(w[0], w[1], p.out_bf16), h1 = sk_pack2(w[2], w[3], p.out_bf16);
-                const uint32_t h2 = sk_pack2(w[4], w[5], p.out_bf16), h3 = sk_pack2(w[6], w[7], p.out_bf16);
+                constexpr int BF = OUT == OUT_BF16;
+                const uint32_t h0 = sk_pack2(w[0], w[1], BF), h1 = sk_pack2(w[2], w[3], BF);
+                const uint32_t h2 = sk_pack2(w[4], w[5], BF), h3 = sk_pack2(w[6], w[7], BF);
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(h0), "r"(h1), "r"(h2), "r"(h3)
                              : "memory");
               }
@@ -640,7 +657,7 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
               for (int j = 0; j < 32; ++j) {
                 if (c + h * 32 + j < valid) {
                   if constexpr (F32) static_cast<float*>(Cv)[at + h * 32 + j] = v[h][j];
-                  else static_cast<uint16_t*>(Cv)[at + h * 32 + j] = static_cast<uint16_t>(sk_pack2(v[h][j], 0.f, p.out_bf16));
+                  else static_cast<uint16_t*>(Cv)[at + h * 32 + j] = static_cast<uint16_t>(sk_pack2(v[h][j], 0.f, OUT == OUT_BF16));
                 }
               }
             }
@@ -650,7 +667,7 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       if (some) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tmem_empty0 + 8u * buf);
+        if (lane == 0) mbar_arrive_cluster_relaxed(tmem_empty0 + 8u * buf);
       }
     }
     if (lane == 0) tma_store_wait_read<0>();
@@ -735,7 +752,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
   p.ldc = g->ldc; p.stride_c = g->E > 1 ? g->stride_c : static_cast<long long>(g->K) * g->ldc;
   p.offsets = offsets;
   p.off64 = (g->flags & SK_FLAG_OFFSETS_64) ? 1 : 0;
-  p.out_bf16 = (g->flags & SK_FLAG_BF16) ? 1 : 0;
+  const bool bf16 = (g->flags & SK_FLAG_BF16) != 0;
   p.zero_rest = (g->flags & SK_FLAG_ZERO_REST) ? 1 : 0;
   p.timeout_ns = (g->timeout_us > 0 ? static_cast<unsigned long long>(g->timeout_us) : 2000000ULL) * 1000ULL;
   p.ws = sk_ws_carve(ws, dev_sms);
@@ -744,39 +761,49 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
   const uint64_t ldb = static_cast<uint64_t>(g->ldb), stride_b = g->E > 1 ? static_cast<uint64_t>(g->stride_b) : ldb * b_rows;
   static SkPerDeviceOnce attrs;
   cudaError_t e = attrs.run([]() {
-    cudaError_t r = cudaFuncSetAttribute(sk_grouped_rows_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
-    if (r == cudaSuccess)
-      r = cudaFuncSetAttribute(sk_grouped_rows_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
-    if (r == cudaSuccess)
-      r = cudaFuncSetAttribute(sk_grouped_sum_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
-    if (r == cudaSuccess)
-      r = cudaFuncSetAttribute(sk_grouped_sum_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+    const void* kernels[7] = {reinterpret_cast<const void*>(sk_grouped_rows_kernel<false, false>),
+                              reinterpret_cast<const void*>(sk_grouped_rows_kernel<false, true>),
+                              reinterpret_cast<const void*>(sk_grouped_rows_kernel<true, false>),
+                              reinterpret_cast<const void*>(sk_grouped_rows_kernel<true, true>),
+                              reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F16>),
+                              reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_BF16>),
+                              reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F32>)};
+    cudaError_t r = cudaSuccess;
+    for (int i = 0; i < 7 && r == cudaSuccess; ++i)
+      r = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
     return r;
   });
   if (e != cudaSuccess) return sk_set_cuda_error(e);
   const int units = sms / 2;
-  const uint32_t bf16_bits = p.out_bf16 ? 1u : 0u;
 
   if (tn) {
     p.bn_max = MAX_BN;
     p.tiles_f = (g->K + 255) / 256;
     p.tiles_n = (g->N + 255) / 256;
+    p.band = p.tiles_f < 8 ? p.tiles_f : 8;
     const long long total = static_cast<long long>(p.tiles_f) * p.tiles_n * g->E;
     if (total > (1LL << 30)) return SK_ERR_LIMIT;
+    p.d_band = sk_div_make(p.band * p.tiles_n);
+    p.d_in = sk_div_make(p.band);
+    p.d_last = sk_div_make(p.tiles_f % p.band ? p.tiles_f % p.band : p.band);
     const int esz = f32 ? 4 : 2;
     p.c_tma = aligned(C, 16) && (p.ldc * esz) % 16 == 0 && (p.stride_c * esz) % 16 == 0;
-    p.idesc = umma_idesc_f16(2 * HALF_M, 0, 1, bf16_bits) | (1u << 15);   // both operands MN-major
+    p.idesc = umma_idesc_f16(2 * HALF_M, 0, 1, bf16) | (1u << 15);   // both operands MN-major
     CUtensorMap tmA, tmB, tmC;
     memset(&tmC, 0, sizeof(tmC));
     st = make_map(&tmA, A, false, 0, g->T, g->K, g->lda, 0, 64, 64);
     if (st == SK_OK) st = make_map(&tmB, B, false, 0, g->T, g->N, ldb, 0, 64, 64);
     if (st == SK_OK && p.c_tma) st = make_map(&tmC, C, f32, g->E, g->K, g->N, p.ldc, p.stride_c, f32 ? 32 : 64, 32);
     if (st != SK_OK) return st;
-    const int smem = 1024 + TN_PIPE + EPI_WARPS * 4096 + CTRL_BYTES + table_bytes(g->E);
-    if (smem > SMEM_LIMIT) return SK_ERR_LIMIT;
+    // Stages: as many as fit, six for up to 383 groups, five above.
+    const int fixed = 1024 + EPI_WARPS * 4096 + CTRL_BYTES + table_bytes(g->E, false);
+    p.stages = (SMEM_LIMIT - fixed) / TN_STEP;
+    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+    const int smem = fixed + p.stages * TN_STEP;
     const int grid = 2 * static_cast<int>(total < units ? total : units);
-    if (f32) e = sk_launch(sk_grouped_sum_kernel<true>, grid, TN_THREADS, smem, cs, 2, pdl, tmA, tmB, tmC, C, p);
-    else e = sk_launch(sk_grouped_sum_kernel<false>, grid, TN_THREADS, smem, cs, 2, pdl, tmA, tmB, tmC, C, p);
+    auto kernel = f32 ? sk_grouped_sum_kernel<OUT_F32>
+                      : bf16 ? sk_grouped_sum_kernel<OUT_BF16> : sk_grouped_sum_kernel<OUT_F16>;
+    e = sk_launch(kernel, grid, TN_THREADS, smem, cs, 2, pdl, tmA, tmB, tmC, C, p);
     return e == cudaSuccess ? SK_OK : sk_set_cuda_error(e);
   }
 
@@ -789,22 +816,24 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
   // the box that a tile of bn_max rows loads, see the producer
   const int half = p.bn_max / 2;
   p.b_step_bytes = (half <= 16 ? 16 : half <= 64 ? 64 : 128) * 128;
-  const int fixed = 1024 + CTRL_BYTES + table_bytes(g->E);
+  const int fixed = 1024 + CTRL_BYTES + table_bytes(g->E, true);
   p.stages = (SMEM_LIMIT - fixed) / (KG * (A_STEP_BYTES + p.b_step_bytes));
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   const int smem = fixed + p.stages * KG * (A_STEP_BYTES + p.b_step_bytes);
-  p.idesc = umma_idesc_f16(2 * HALF_M, 0, 0, bf16_bits) | (nn ? (1u << 15) : 0u);
+  p.idesc = umma_idesc_f16(2 * HALF_M, 0, 0, bf16) | (nn ? (1u << 15) : 0u);
   CUtensorMap tmW, tmX[3];
   st = nn ? make_map(&tmW, B, false, g->E, g->K, g->N, ldb, stride_b, 64, 64)
           : make_map(&tmW, B, false, g->E, g->N, g->K, ldb, stride_b, 64, HALF_M);
   const uint32_t boxes[3] = {16, 64, 128};
-  for (int i = 0; i < 3 && st == SK_OK; ++i) st = make_map(&tmX[i], A, false, 0, g->T, g->K, g->lda, 0, 64, boxes[i]);
+  memset(tmX, 0, sizeof(tmX));
+  for (int i = 0; i < 3 && st == SK_OK; ++i)   // (only those that a tile can use)
+    if (i == 0 || boxes[i - 1] < static_cast<uint32_t>(half))
+      st = make_map(&tmX[i], A, false, 0, g->T, g->K, g->lda, 0, 64, boxes[i]);
   if (st != SK_OK) return st;
   const int grid = 2 * units;
   uint16_t* c = static_cast<uint16_t*>(C);
-  if (nn)
-    e = sk_launch(sk_grouped_rows_kernel<true>, grid, NT_THREADS, smem, cs, 2, pdl, tmW, tmX[0], tmX[1], tmX[2], c, p);
-  else
-    e = sk_launch(sk_grouped_rows_kernel<false>, grid, NT_THREADS, smem, cs, 2, pdl, tmW, tmX[0], tmX[1], tmX[2], c, p);
+  auto kernel = nn ? (bf16 ? sk_grouped_rows_kernel<true, true> : sk_grouped_rows_kernel<true, false>)
+                   : (bf16 ? sk_grouped_rows_kernel<false, true> : sk_grouped_rows_kernel<false, false>);
+  e = sk_launch(kernel, grid, NT_THREADS, smem, cs, 2, pdl, tmW, tmX[0], tmX[1], tmX[2], c, p);
   return e == cudaSuccess ? SK_OK : sk_set_cuda_error(e);
 }

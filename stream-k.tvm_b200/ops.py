@@ -142,6 +142,9 @@ _OPTION_KEYS = ("tile_m", "tile_n", "num_sms", "group_m", "out", "timeout_us", "
                 "_drop_flag_cta", "_bf16")
 
 
+_NO_OPTIONS = dict.fromkeys(_OPTION_KEYS)
+
+
 def _options(kw: dict) -> dict:
     """Common keyword arguments of every GEMM entry point:
     tile_m / tile_n  tile extents (None = choose; tile_m < 128 puts the weights on the UMMA
@@ -152,6 +155,8 @@ def _options(kw: dict) -> dict:
                      no_table (True: schedule "auto" by the built-in rules only, ignoring the table
                      of tuned shapes),
                      _drop_flag_cta (test hook: index of a CTA that withholds its flag)."""
+    if not kw:
+        return _NO_OPTIONS.copy()
     unknown = set(kw) - set(_OPTION_KEYS)
     if unknown:
         raise TypeError(f"unexpected keyword argument(s): {sorted(unknown)}")
@@ -163,15 +168,14 @@ def _problem(M, N, K, lda, ldb, ldc, layout, schedule, fixup, o: dict) -> L.SkPr
         raise ValueError(f"schedule must be one of {sorted(L.SCHEDULES)}, got {schedule!r}")
     if fixup not in L.FIXUPS:
         raise ValueError(f"fixup must be one of {sorted(L.FIXUPS)}, got {fixup!r}")
-    return L.SkProblem(M=M, N=N, K=K, lda=lda, ldb=ldb, ldc=ldc, layout=L.LAYOUTS[layout],
-                       schedule=L.SCHEDULES[schedule], fixup=L.FIXUPS[fixup],
-                       tile_m=int(o["tile_m"] or 0), tile_n=int(o["tile_n"] or 0),
-                       num_sms=int(o["num_sms"] or 0), group_m=int(o["group_m"] or 0),
-                       fixup_timeout_us=int(o["timeout_us"] or 0),
+    # (positional: the fields of sk_problem in order; half the time of keywords)
+    return L.SkProblem(M, N, K, lda, ldb, ldc, L.LAYOUTS[layout], L.SCHEDULES[schedule], L.FIXUPS[fixup],
+                       int(o["tile_m"] or 0), int(o["tile_n"] or 0), int(o["num_sms"] or 0), int(o["group_m"] or 0),
+                       int(o["timeout_us"] or 0),
                        # (the C field is 0 = off, n = CTA n - 1)
-                       test_drop_flag_cta=0 if o["_drop_flag_cta"] is None else int(o["_drop_flag_cta"]) + 1,
-                       flags=(L.SK_FLAG_PDL if o["pdl"] else 0) | (L.SK_FLAG_NO_TABLE if o["no_table"] else 0)
-                             | (L.SK_FLAG_BF16 if o["_bf16"] else 0))
+                       0 if o["_drop_flag_cta"] is None else int(o["_drop_flag_cta"]) + 1,
+                       (L.SK_FLAG_PDL if o["pdl"] else 0) | (L.SK_FLAG_NO_TABLE if o["no_table"] else 0)
+                       | (L.SK_FLAG_BF16 if o["_bf16"] else 0))
 
 
 def schedule_info(M: int, N: int, K: int, *, kind: str = "f16", schedule: str = "auto",
@@ -615,8 +619,8 @@ def int8_quantize(X: torch.Tensor, *, pdl: bool = False) -> tuple[torch.Tensor, 
     _check_extents(M=M, K=K)
     X = _rowmajor(X)
     pitch = -(-K // 16) * 16
-    Q = torch.empty((M, pitch), dtype=torch.int8, device=X.device)
-    scale = torch.empty(M, dtype=torch.float32, device=X.device)
+    Q = X.new_empty((M, pitch), dtype=torch.int8)
+    scale = X.new_empty(M, dtype=torch.float32)
     flags = (L.SK_FLAG_BF16 if X.dtype == torch.bfloat16 else 0) | (L.SK_FLAG_PDL if pdl else 0)
     with _on(X.device):
         L.check(L.load().sk_quantize_i8(X.data_ptr(), M, K, X.stride(0) if M > 1 else K, flags, Q.data_ptr(), pitch,
@@ -643,7 +647,8 @@ def _check_scale(name: str, s: torch.Tensor, n: int, device) -> torch.Tensor:
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """An int8 matrix with 16-byte aligned rows (TMA), copied only if it has none."""
-    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0:
+    ld, unit = t.stride()
+    if unit == 1 and ld % 16 == 0 and ld >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
     n = torch.empty((t.shape[0], -(-t.shape[1] // 16) * 16), dtype=t.dtype, device=t.device)
     n[:, : t.shape[1]].copy_(t)
