@@ -13,10 +13,11 @@
 // NT and NN: CTA pairs (cta_group::2).  The weights feed the UMMA M dimension (256 of the N output
 // features per pair, 128 per CTA) and the rows of a group the UMMA N dimension, whose extent the
 // instruction descriptor sets tile by tile in steps of 16: a group of 5 rows costs the tensor
-// cores 32 columns and a group of 300 two tiles of 160, where rows on the M side would cost whole
+// cores 32 columns and a group of 300 two tiles of 160 (150 rounded up), where rows on the M side would cost whole
 // multiples of 128 or 256.  Groups of a few rows are then what they should be, a stream of the
-// weights.  A pair's accumulator is transposed (lane = feature, column = row of A): 32 lanes
-// store 64 contiguous bytes of a row of C.
+// weights.  A pair's accumulator is transposed (lane = feature, column = row of A); a warp turns
+// 32 x 32 of it through shared memory (ldmatrix.trans) and stores 64 contiguous bytes of a row of
+// C with every four lanes.
 //
 // TN: the sum runs over a group's rows, so both operands are MN-major (TMA boxes of 64 columns x
 // 64 rows) and a group's last step holds rows of the next group.  Those must not count, whatever
@@ -162,6 +163,16 @@ struct RowWalk {
 };
 
 constexpr int NT_THREADS = 64 + 32 * EPI_WARPS;   // warp 0 producer, 1 MMA issuer, 2..9 epilogue
+constexpr int TURN_BYTES = 2048;                  // an epilogue warp's 32 features x 32 rows of A, 16 bits each
+
+// Where a warp keeps piece k (8 rows of A, 16 bytes) of feature f while it turns a block: two
+// features to 128 bytes, the pieces permuted so that neither the lanes that write (eight
+// consecutive features, one piece) nor the matrices read back (features 8 j + 2 m and + 1 for
+// j = 0..3) meet on a bank.
+__device__ __forceinline__ uint32_t turn_at(int f, int k) {
+  const int swap = ((f >> 1) ^ (f >> 3)) & 3;
+  return static_cast<uint32_t>((f >> 1) * 128 + ((f & 1) * 4 + (k ^ swap)) * 16);
+}
 
 // W_MN: the weights are MN-major (NN): two boxes of 64 features x 64 of K per step.  BF16: C's type.
 template <bool W_MN, bool BF16>
@@ -176,7 +187,7 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
   const int STAGES = p.stages;
   const uint32_t sW = base, sX = base + STAGES * KG * A_STEP_BYTES;
   Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + STAGES * KG * (A_STEP_BYTES + p.b_step_bytes));
-  int* start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ctrl) + CTRL_BYTES);
+  int* start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ctrl) + CTRL_BYTES + EPI_WARPS * TURN_BYTES);
   int* first = start + p.E + 1;
   volatile uint32_t* abort_flag = &ctrl->abort;
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
@@ -319,6 +330,8 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
     }
     const uint32_t tmem_full0 = smem_u32(&ctrl->tmem_full[0]);
     const uint32_t tmem_empty0 = mapa_shared(smem_u32(&ctrl->tmem_empty[0]), 0);
+    const uint32_t turn = smem_u32(ctrl) + CTRL_BYTES + (warp - 2) * TURN_BYTES;
+    const int turn_f = 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);   // the feature whose piece this lane names
     uint32_t nseg = 0;
     bool dead = false;
     while (walk.next(p, start, first, units, tile)) {
@@ -330,17 +343,42 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
       ++nseg;
       tc_fence_after();
       const uint32_t t_addr = tmem_base + buf * MAX_BN + (static_cast<uint32_t>(q * 32) << 16);
-      const int f = tile.f0 + rank * HALF_M + q * 32 + lane;
-      const bool f_ok = f < p.N;
-      if (!dead && tile.f0 + rank * HALF_M + q * 32 < p.N) {
+      const int f0 = tile.f0 + rank * HALF_M + q * 32;      // the warp's 32 features
+      if (!dead && f0 < p.N) {
+        const int f = f0 + 8 * (lane & 3);                  // the eight that this lane stores
         for (int c = sub * 32; c < tile.rows; c += 64) {
-          float v[32];
-          sk_load_acc(t_addr + c, 0, v);
-          uint16_t* dst = C + static_cast<long long>(tile.r0 + c) * p.ldc + f;
-          const int nv = tile.rows - c;
+          uint32_t v[32];
+          tmem_ld_32x32(t_addr + c, v);
+          tmem_ld_wait();
+          __syncwarp();                                     // the block before has been read
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (f_ok && j < nv) dst[j * p.ldc] = static_cast<uint16_t>(sk_pack2(v[j], 0.f, BF16));
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = sk_pack2(__uint_as_float(v[8 * k + 2 * i]), __uint_as_float(v[8 * k + 2 * i + 1]), BF16);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(turn + turn_at(lane, k)), "r"(w[0]), "r"(w[1]),
+                         "r"(w[2]), "r"(w[3])
+                         : "memory");
+          }
+          __syncwarp();
+          uint16_t* dst = C + static_cast<long long>(tile.r0 + c + (lane >> 2)) * p.ldc + f;
+          const int left = tile.rows - c - (lane >> 2);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[4];
+            ldmatrix_x4_trans(turn + turn_at(turn_f, k), w);
+            uint16_t* d = dst + 8 * k * p.ldc;
+            if (8 * k < left) {
+              if (p.c_vec_ok && f + 8 <= p.N) {
+                *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (f + i < p.N) d[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+              }
+            }
+          }
         }
       }
       tc_fence_before();
@@ -816,7 +854,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
   // the box that a tile of bn_max rows loads, see the producer
   const int half = p.bn_max / 2;
   p.b_step_bytes = (half <= 16 ? 16 : half <= 64 ? 64 : 128) * 128;
-  const int fixed = 1024 + CTRL_BYTES + table_bytes(g->E, true);
+  const int fixed = 1024 + CTRL_BYTES + EPI_WARPS * TURN_BYTES + table_bytes(g->E, true);
   p.stages = (SMEM_LIMIT - fixed) / (KG * (A_STEP_BYTES + p.b_step_bytes));
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   const int smem = fixed + p.stages * KG * (A_STEP_BYTES + p.b_step_bytes);
