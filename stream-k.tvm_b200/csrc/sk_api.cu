@@ -175,6 +175,36 @@ const SkTuned kTuned[] = {
     {-1, 0, 0, 0, 0, 0, 0, 0}};
 }  // namespace
 
+// 8-bit integers: a K step takes half the time per element that it takes 16-bit operands, and a split
+// tile's fix-up takes the same, so whole tiles (data-parallel) are ahead nearly everywhere.
+// Measured over M = 100 .. 6400 at (N, K) = (512, 512) .. (28672, 8192), against the 16-bit rules'
+// Stream-K and hybrid choices: 1.0x to 2.1x, 1.3x in the geometric mean; within 5 % of the best
+// plan tried on all but a few.  The tile:
+//   128 x 64 while those fit on the SMs at once (the latency of one tile is all there is), then
+//   128 x 128 likewise, 128 x 256 for a single row of tiles beyond that; otherwise CTA pairs, 256 x
+//   256, or 256 x 192 where the waves then take a tenth less (200 x 11008 x 2048: 12.9 us against
+//   13.7; 400 x 12288 x 4096: 26.4 against 28.7).
+// M <= 64 keeps the rules below (weights on the UMMA M side, split over clusters), but for short K
+// (48 x 512 x 512: 5.5 us against 11.5) and for more than a wave of tiles (48 x 28672 x 1024: 13.2
+// against 16.9).  False: not decided here.
+static bool resolve_auto_i8(sk_problem* q, int num_sms) {
+  const int steps = (q->K - 1) / 64 + 1;          // (K in pairs of elements)
+  auto tiles = [&](int m, int n) {
+    return ((static_cast<long long>(q->M) + m - 1) / m) * ((static_cast<long long>(q->N) + n - 1) / n);
+  };
+  auto plan = [&](int m, int n) {
+    q->schedule = SK_SCHED_DP; q->tile_m = m; q->tile_n = n;
+    return true;
+  };
+  if (q->M <= 64 && !(steps < 8 && tiles(128, 64) <= num_sms) && !(q->M > 32 && tiles(128, 128) > num_sms)) return false;
+  if (tiles(128, 64) <= num_sms) return plan(128, 64);
+  if (tiles(128, 128) <= num_sms) return plan(128, 128);
+  if (q->M <= 128 || (num_sms & 1) != 0) return plan(128, 256);
+  const int pairs = num_sms / 2;
+  const long long w256 = (tiles(256, 256) + pairs - 1) / pairs, w192 = (tiles(256, 192) + pairs - 1) / pairs;
+  return plan(256, 11 * w192 * 192 < 10 * w256 * 256 ? 192 : 256);
+}
+
 void sk_resolve_auto(sk_problem* q, int kernel_kind, int num_sms) {
   if (q->schedule != SK_SCHED_AUTO) return;
   q->schedule = SK_SCHED_HYBRID;
@@ -197,7 +227,10 @@ void sk_resolve_auto(sk_problem* q, int kernel_kind, int num_sms) {
   const int gemv_kind = sk_gemv_kind(kernel_kind, q->flags);
   // (W4A16: 9 to 16 rows cost the small-M kernel twice the instructions of 1 to 8: only where the
   // launch is short enough to be bound by latencies, at most one 32-row CTA per SM)
-  const int gemv_m = gemv_kind == 4 ? SK_GEMV_I8_MAX_M : gemv_kind != 2 ? SK_GEMV_AUTO_M : (q->N <= 32LL * num_sms ? SK_GEMV_Q4_MAX_M : 8);
+  // (8-bit integers: 9 to 16 rows take a second column tile and a second set of activations; ahead of
+  // the tensor-memory kernels, 12.4 against 13.7 us at 16 x 11008 x 4096, until the weights are
+  // many waves of CTAs: 53.6 against 44.5 at 16 x 28672 x 8192)
+  const int gemv_m = gemv_kind == 4 ? (q->N <= 96LL * num_sms ? SK_GEMV_I8_MAX_M : 8) : gemv_kind != 2 ? SK_GEMV_AUTO_M : (q->N <= 32LL * num_sms ? SK_GEMV_Q4_MAX_M : 8);
   if (tiles_open && q->M <= gemv_m && (kernel_kind == 2 || q->layout == SK_LAYOUT_NT)) {
     // Few rows of activations: the weights stream once through a kernel without the tensor-core
     // kernels' fixed costs (tensor-memory allocation, mbarrier rings, a cluster exchange or a
@@ -213,6 +246,7 @@ void sk_resolve_auto(sk_problem* q, int kernel_kind, int num_sms) {
       return;
     }
   }
+  if (kernel_kind == 1 && tiles_open && (q->flags & SK_FLAG_INTERNAL_I8) != 0 && resolve_auto_i8(q, num_sms)) return;
   const long long t256 = static_cast<long long>((q->M + 255) / 256) * ((q->N + 255) / 256);
   if (t256 >= num_sms) return;                       // large: hybrid (CTA pairs when eligible)
   // (W4A16 beyond 112 rows: the cluster schedule would need two narrower tiles per 128 weight

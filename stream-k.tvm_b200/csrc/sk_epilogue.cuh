@@ -53,6 +53,15 @@ __device__ __forceinline__ bool sk_wait_bar(uint32_t bar, uint32_t parity, volat
   }
 }
 
+// The same for a role that a whole warp runs: one answer for all lanes, which leave the wait
+// together (a lane that fell behind could mistake a barrier's phase, and after a time-out lanes
+// that disagree would miss one another at the next warp-wide instruction).
+template <bool CLUSTER = false, typename Params>
+__device__ __forceinline__ bool sk_wait_bar_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                 const Params& p, uint32_t bar_id, uint32_t role) {
+  return __all_sync(0xffffffffu, sk_wait_bar<CLUSTER>(bar, parity, abort_flag, p, bar_id, role)) != 0;
+}
+
 // fp32 -> the 16-bit result type: fp16, or bfloat16 when the problem carries SK_FLAG_BF16
 // (p.out_bf16).  C is addressed as 16-bit words either way.
 __device__ __forceinline__ uint32_t sk_pack2(float a, float b, int bf16) {

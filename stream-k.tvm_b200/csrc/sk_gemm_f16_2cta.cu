@@ -65,7 +65,8 @@ static_assert(sizeof(Ctrl) <= CTRL_BYTES, "Ctrl must fit its reserved space");
 constexpr int OUT_PLAIN = 0, OUT_GATHER = 1, OUT_SCATTER = 2;
 
 // I8: 8-bit integer operands, 32-bit integer accumulators (see sk_gemm_f16.cu); OUT_PLAIN only.
-template <int OUT, bool I8 = false>
+// WIDE: the schedule has 256 x 512 units (p.wide_units > 0); never with OUT_SCATTER.
+template <int OUT, bool I8, bool WIDE>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmC, __half* __restrict__ C, const SkParams p,
@@ -86,7 +87,17 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + PIPE_BYTES);
   volatile uint32_t* abort_flag = &ctrl->abort;
 
-  const int warp = threadIdx.x >> 5;
+  // Without wide units the producer and the MMA issuer are run by their whole warp, with the TMA,
+  // mbarrier and tcgen05 instructions behind an elected lane: warp-uniform code issues them at
+  // about half the cost, and issued by a lone lane the four UMMAs of a K step take longer than a
+  // step of a tile narrower than 256 columns (256 x 11008 x 4096: 31.7 -> 29.9 us).  With wide units
+  // (eight UMMAs of 256 columns to a barrier) the lone lane is ahead (9472 x 8192 x 4096: 426 us
+  // against 430).
+  auto wait_bar = [](uint32_t bar, uint32_t parity, volatile uint32_t* flag, const SkParams& prm, uint32_t id, uint32_t role) {
+    if constexpr (WIDE) return sk_wait_bar(bar, parity, flag, prm, id, role);
+    else return sk_wait_bar_warp(bar, parity, flag, prm, id, role);
+  };
+  const int warp = uniform_warp_idx();
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());   // 0 = leader of the pair
   const int unit = blockIdx.x >> 1;                        // the pair's index in the schedule
@@ -135,7 +146,8 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 
   if (warp == 0) {
     // ------------------------------------------------------------- producer (both CTAs)
-    if (lane == 0) {
+    if (!WIDE || lane == 0) {
+      const bool leader = WIDE || elect_one();
       SkCursor cur;
       sk_cursor_init(s, unit, cur);
       SkSeg seg;
@@ -152,26 +164,26 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const int b_row0 = tc * p.bn + rank * (p.bn / 2);   // this CTA's half of the tile's rows of B
         for (int k = seg.k0; k < seg.k1;) {
           const int n = (seg.k1 - k) < KG ? (seg.k1 - k) : KG;
-          if (!sk_wait_bar(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0)) {
+          if (!wait_bar(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0)) {
             ok = false;
             break;
           }
           // Both CTAs' loads complete on the leader's barrier; the leader expects all of them.
           const uint32_t full_leader = full0_leader + 8u * stage;
-          if (rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, n * 2 * (A_STAGE_BYTES + p.col_tx_bytes));
-          for (int j = 0; j < n; ++j) {
+          if (leader && rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, n * 2 * (A_STAGE_BYTES + p.col_tx_bytes));
+          for (int j = 0; leader && j < n; ++j) {
             tma_load_2d_pair(sA + (stage * KG + j) * A_STAGE_BYTES, &tmA, full_leader, (k + j) * XK, a_row0);
             tma_load_2d_pair(sB + (stage * KG + j) * B_STAGE_BYTES, &tmB, full_leader, (k + j) * XK, b_row0);
           }
           k += n;
           if (++stage == STAGES) { stage = 0; ph ^= 1u; }
-          if (!traced) { sk_trace(p, 2); traced = true; }
+          if (leader && !traced) { sk_trace(p, 2); traced = true; }
         }
       }
-      if (ok && p.wide_units > 0) {
+      if (WIDE && ok) {
         // ---- wide units.  First let the tiles' last stages drain: the wide ring reuses their memory.
         for (int i = 0; i < STAGES && ok; ++i) {
-          ok = sk_wait_bar(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0);
+          ok = wait_bar(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0);
           if (++stage == STAGES) { stage = 0; ph ^= 1u; }
         }
         const uint32_t fullw0_leader = mapa_shared(smem_u32(&ctrl->fullw[0]), 0);
@@ -184,16 +196,18 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           const int a_row0 = (tm * 2 + rank) * BM;
           const int b_row0 = tnw * (2 * BN) + rank * (BN / 2);   // half 0; half 1 is BN rows further
           for (int k = 0; k < s.iters_per_tile; ++k) {
-            if (!sk_wait_bar(emptyw0 + 8u * ws, wph ^ 1u, abort_flag, p, 8 + ws, 0)) {
+            if (!wait_bar(emptyw0 + 8u * ws, wph ^ 1u, abort_flag, p, 8 + ws, 0)) {
               ok = false;
               break;
             }
             const uint32_t dst = base + ws * W_STAGE_BYTES;
             const uint32_t full_leader = fullw0_leader + 8u * ws;
-            if (rank == 0) mbar_arrive_expect_tx(fullw0 + 8u * ws, 2 * W_STAGE_BYTES);
-            tma_load_2d_pair(dst, &tmA, full_leader, k * XK, a_row0);
-            tma_load_2d_pair(dst + A_STAGE_BYTES, &tmB, full_leader, k * XK, b_row0);
-            tma_load_2d_pair(dst + A_STAGE_BYTES + B_STAGE_BYTES, &tmB, full_leader, k * XK, b_row0 + BN);
+            if (leader) {
+              if (rank == 0) mbar_arrive_expect_tx(fullw0 + 8u * ws, 2 * W_STAGE_BYTES);
+              tma_load_2d_pair(dst, &tmA, full_leader, k * XK, a_row0);
+              tma_load_2d_pair(dst + A_STAGE_BYTES, &tmB, full_leader, k * XK, b_row0);
+              tma_load_2d_pair(dst + A_STAGE_BYTES + B_STAGE_BYTES, &tmB, full_leader, k * XK, b_row0 + BN);
+            }
             if (++ws == WSTAGES) { ws = 0; wph ^= 1u; }
           }
         }
@@ -201,7 +215,8 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA issuer (leader only)
-    if (lane == 0 && rank == 0) {
+    if (rank == 0 && (!WIDE || lane == 0)) {
+      const bool leader = WIDE || elect_one();
       SkCursor cur;
       sk_cursor_init(s, unit, cur);
       SkSeg seg;
@@ -216,37 +231,37 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
       while (ok && sk_next(s, unit, cur, seg)) {
         const uint32_t buf = nseg & 1u;
         const uint32_t acc_ph = (nseg >> 1) & 1u;
-        if (!sk_wait_bar(smem_u32(&ctrl->tmem_empty[buf]), acc_ph ^ 1u, abort_flag, p, 16 + buf, 1))
+        if (!wait_bar(smem_u32(&ctrl->tmem_empty[buf]), acc_ph ^ 1u, abort_flag, p, 16 + buf, 1))
           break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * BN;
         uint32_t accumulate = 0u;
         for (int k = seg.k0; k < seg.k1;) {
           const int n = (seg.k1 - k) < KG ? (seg.k1 - k) : KG;
-          if (!sk_wait_bar(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
+          if (!wait_bar(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          if (nseg == 0 && k == seg.k0) sk_trace(p, 3);
+          if (leader && nseg == 0 && k == seg.k0) sk_trace(p, 3);
           for (int j = 0; j < n; ++j) {
             const uint32_t a_lo = a_lo0 + (stage * KG + j) * (A_STAGE_BYTES >> 4);
             const uint32_t b_lo = b_lo0 + (stage * KG + j) * (B_STAGE_BYTES >> 4);
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
-              umma(d_tmem, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc, accumulate);
+              if (leader) umma(d_tmem, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc, accumulate);
               accumulate = 1u;
             }
           }
-          umma_commit_pair(empty0 + 8u * stage);   // frees the stage in both CTAs
+          if (leader) umma_commit_pair(empty0 + 8u * stage);   // frees the stage in both CTAs
           k += n;
           if (++stage == STAGES) { stage = 0; ph ^= 1u; }
         }
         if (!ok) break;
-        umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));   // accumulator ready in both CTAs
+        if (leader) umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));   // accumulator ready in both CTAs
         ++nseg;
       }
-      if (ok && p.wide_units > 0) {
+      if (WIDE && ok) {
         // ---- wide units: every A stage feeds two accumulators (25 % fewer bytes into the SM
         // per flop, which is what bounds this kernel and what costs it power)
         const uint32_t fullw0 = smem_u32(&ctrl->fullw[0]), emptyw0 = smem_u32(&ctrl->emptyw[0]);
@@ -257,7 +272,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           const uint32_t buf0 = nseg & 1u, buf1 = buf0 ^ 1u;
           const uint32_t empty1 = smem_u32(&ctrl->tmem_empty[buf1]);
           const uint32_t empty1_ph = (((nseg + 1) >> 1) & 1u) ^ 1u;
-          if (!sk_wait_bar(smem_u32(&ctrl->tmem_empty[buf0]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf0, 1)) {
+          if (!wait_bar(smem_u32(&ctrl->tmem_empty[buf0]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf0, 1)) {
             ok = false;
             break;
           }
@@ -278,7 +293,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           bool h1_ready = false;
           while (ok && k1 < I) {
             if (k0 < I && (h1_ready ? k0 - k1 <= lag : k0 - k1 < WSTAGES - 1)) {
-              if (!sk_wait_bar(fullw0 + 8u * ws, wph, abort_flag, p, 40 + ws, 1)) {
+              if (!wait_bar(fullw0 + 8u * ws, wph, abort_flag, p, 40 + ws, 1)) {
                 ok = false;
                 break;
               }
@@ -287,17 +302,17 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
               const uint32_t b_lo = a_lo + (A_STAGE_BYTES >> 4);
 #pragma unroll
               for (int kk = 0; kk < BK / 16; ++kk)
-                umma(d0, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc,
-                                 (k0 | kk) ? 1u : 0u);
+                if (leader)
+                  umma(d0, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc, (k0 | kk) ? 1u : 0u);
               ++k0;
               if (++ws == WSTAGES) { ws = 0; wph ^= 1u; }
-              if (k0 == I) umma_commit_pair(smem_u32(&ctrl->tmem_full[buf0]));   // first half complete
+              if (leader && k0 == I) umma_commit_pair(smem_u32(&ctrl->tmem_full[buf0]));   // first half complete
             }
             if (!h1_ready) {
               if (mbar_try_wait(empty1, empty1_ph, 0u)) {
                 h1_ready = true;
               } else if (k0 == I || k0 - k1 >= WSTAGES - 1) {   // cannot run further ahead: wait
-                if (!sk_wait_bar(empty1, empty1_ph, abort_flag, p, 16 + buf1, 1)) {
+                if (!wait_bar(empty1, empty1_ph, abort_flag, p, 16 + buf1, 1)) {
                   ok = false;
                   break;
                 }
@@ -310,19 +325,19 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
               const uint32_t b_lo = a_lo + ((A_STAGE_BYTES + B_STAGE_BYTES) >> 4);
 #pragma unroll
               for (int kk = 0; kk < BK / 16; ++kk)
-                umma(d1, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc,
-                                 (k1 | kk) ? 1u : 0u);
-              umma_commit_pair(emptyw0 + 8u * ws1);   // both halves have read the stage
+                if (leader)
+                  umma(d1, desc_hi | (a_lo + kk * 2), desc_hi | (b_lo + kk * 2), idesc, (k1 | kk) ? 1u : 0u);
+              if (leader) umma_commit_pair(emptyw0 + 8u * ws1);   // both halves have read the stage
               ++k1;
               if (++ws1 == WSTAGES) ws1 = 0;
             }
           }
           if (!ok) break;
-          umma_commit_pair(smem_u32(&ctrl->tmem_full[buf1]));
+          if (leader) umma_commit_pair(smem_u32(&ctrl->tmem_full[buf1]));
           nseg += 2;
         }
       }
-      sk_trace(p, 4);
+      if (leader) sk_trace(p, 4);
     }
   } else {
     // ------------------------------------------------------------- epilogue (both CTAs)
@@ -365,7 +380,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     sk_epilogue_loop<I8 ? SK_EPI_BLOCK_REDUCE : SK_EPI_ANY, EPI_WARPS, 1, I8>(p, C, unit, rank, warp, lane, tmem_base, tmem_full0, tmem_empty0,
                                             &ctrl->bcast, abort_flag, ctrl->pend, &tmC, cstage, &nseg, peers);
     }
-    if (OUT != OUT_SCATTER && p.wide_units > 0) {
+    if (WIDE) {
       // ---- wide units: the two halves are two whole tiles in the two accumulator buffers
       const int q = warp & 3;
       const int sub = (warp - 2) >> 2;   // the quadrant's two warps take alternate column groups
@@ -526,36 +541,32 @@ int sk_launch_f16_2cta(const sk_problem* prob, const void* A, const void* B, voi
   p->wide_lag = 1;
 
   static SkPerDeviceOnce attrs;
-  cudaError_t e = attrs.run([]() {
-    cudaError_t r = cudaFuncSetAttribute(sk_gemm_f16_2cta_kernel<OUT_PLAIN>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
-    if (r == cudaSuccess)
-      r = cudaFuncSetAttribute(sk_gemm_f16_2cta_kernel<OUT_PLAIN, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               SMEM_BYTES);
-    if (r == cudaSuccess)
-      r = cudaFuncSetAttribute(sk_gemm_f16_2cta_kernel<OUT_GATHER>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               SMEM_BYTES);
-    if (r == cudaSuccess)
-      r = cudaFuncSetAttribute(sk_gemm_f16_2cta_kernel<OUT_SCATTER>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               SMEM_BYTES);
+  const void* const kernels[7] = {reinterpret_cast<const void*>(sk_gemm_f16_2cta_kernel<OUT_PLAIN, false, false>),
+                                  reinterpret_cast<const void*>(sk_gemm_f16_2cta_kernel<OUT_PLAIN, false, true>),
+                                  reinterpret_cast<const void*>(sk_gemm_f16_2cta_kernel<OUT_PLAIN, true, false>),
+                                  reinterpret_cast<const void*>(sk_gemm_f16_2cta_kernel<OUT_PLAIN, true, true>),
+                                  reinterpret_cast<const void*>(sk_gemm_f16_2cta_kernel<OUT_GATHER, false, false>),
+                                  reinterpret_cast<const void*>(sk_gemm_f16_2cta_kernel<OUT_GATHER, false, true>),
+                                  reinterpret_cast<const void*>(sk_gemm_f16_2cta_kernel<OUT_SCATTER, false, false>)};
+  cudaError_t e = attrs.run([&kernels]() {
+    cudaError_t r = cudaSuccess;
+    for (int i = 0; i < 7 && r == cudaSuccess; ++i)
+      r = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     return r;
   });
   if (e != cudaSuccess) return sk_set_cuda_error(e);
   const bool pdl = (prob->flags & SK_FLAG_PDL) != 0;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   __half* Ch = static_cast<__half*>(C);
-  if (k_i8)
-    e = sk_launch(sk_gemm_f16_2cta_kernel<OUT_PLAIN, true>, p->sched.grid * 2, NUM_THREADS, SMEM_BYTES, cs, 2, pdl,
-                  tmA, tmB, tmC, Ch, *p, peer_set);
-  else if (n_blocks)
-    e = sk_launch(sk_gemm_f16_2cta_kernel<OUT_SCATTER>, p->sched.grid * 2, NUM_THREADS, SMEM_BYTES, cs, 2, pdl,
-                  tmA, tmB, tmC, Ch, *p, peer_set);
-  else if (n_peers > 0)
-    e = sk_launch(sk_gemm_f16_2cta_kernel<OUT_GATHER>, p->sched.grid * 2, NUM_THREADS, SMEM_BYTES, cs, 2, pdl,
-                  tmA, tmB, tmC, Ch, *p, peer_set);
-  else
-    e = sk_launch(sk_gemm_f16_2cta_kernel<OUT_PLAIN>, p->sched.grid * 2, NUM_THREADS, SMEM_BYTES, cs, 2, pdl,
-                  tmA, tmB, tmC, Ch, *p, peer_set);
+  const bool wide = p->wide_units > 0;
+  if (n_blocks && wide) return SK_ERR_SHAPE;   // (whole tiles only: the data-parallel schedule has no units)
+  auto kernel = n_blocks ? sk_gemm_f16_2cta_kernel<OUT_SCATTER, false, false>
+              : n_peers > 0 ? (wide ? sk_gemm_f16_2cta_kernel<OUT_GATHER, false, true>
+                                    : sk_gemm_f16_2cta_kernel<OUT_GATHER, false, false>)
+              : k_i8 ? (wide ? sk_gemm_f16_2cta_kernel<OUT_PLAIN, true, true> : sk_gemm_f16_2cta_kernel<OUT_PLAIN, true, false>)
+                     : (wide ? sk_gemm_f16_2cta_kernel<OUT_PLAIN, false, true>
+                             : sk_gemm_f16_2cta_kernel<OUT_PLAIN, false, false>);
+  e = sk_launch(kernel, p->sched.grid * 2, NUM_THREADS, SMEM_BYTES, cs, 2, pdl, tmA, tmB, tmC, Ch, *p, peer_set);
   if (e != cudaSuccess) return sk_set_cuda_error(e);
   return SK_OK;
 }

@@ -246,7 +246,7 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
         const int f_row = tile.f0 + rank * HALF_M, x_row = tile.r0 + rank * half;
         for (int k = 0; k < I;) {
           const int n = I - k < KG ? I - k : KG;
-          if (!sk_wait_bar(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0)) {
+          if (!sk_wait_bar_warp(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0)) {
             ok = false;
             break;
           }
@@ -280,14 +280,14 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
       const uint32_t full0 = smem_u32(&ctrl->full[0]), empty0 = smem_u32(&ctrl->empty[0]);
       while (ok && walk.next(p, start, first, units, tile)) {
         const uint32_t buf = nseg & 1u;
-        if (!sk_wait_bar(smem_u32(&ctrl->tmem_empty[buf]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf, 1)) break;
+        if (!sk_wait_bar_warp(smem_u32(&ctrl->tmem_empty[buf]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf, 1)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * MAX_BN;
         const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tile.bn >> 3) << 17);
         uint32_t accumulate = 0u;
         for (int k = 0; k < I;) {
           const int n = I - k < KG ? I - k : KG;
-          if (!sk_wait_bar(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
+          if (!sk_wait_bar_warp(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
             ok = false;
             break;
           }
@@ -504,7 +504,7 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         const int I = (tile.rows + BK - 1) / BK;
         const int a_col = tile.f0 + rank * HALF_M, b_col = tile.c0 + rank * (MAX_BN / 2);
         for (int k = 0; k < I; ++k) {
-          if (!sk_wait_bar(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0)) {
+          if (!sk_wait_bar_warp(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0)) {
             ok = false;
             break;
           }
@@ -554,17 +554,17 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         const int I = (tile.rows + BK - 1) / BK;
         if (I == 0) continue;   // (the epilogue writes zeros)
         const uint32_t buf = nseg & 1u;
-        if (!sk_wait_bar(smem_u32(&ctrl->tmem_empty[buf]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf, 1)) break;
+        if (!sk_wait_bar_warp(smem_u32(&ctrl->tmem_empty[buf]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf, 1)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * MAX_BN;
         uint32_t accumulate = 0u;
         for (int k = 0; k < I; ++k) {
-          if (!sk_wait_bar(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
+          if (!sk_wait_bar_warp(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
             ok = false;
             break;
           }
           if (step_needs_zeros(k, tile.rows)) {
-            if (!sk_wait_bar<true>(ready0 + 8u * stage, (tail_ph >> stage) & 1u, abort_flag, p, 48 + stage, 1)) {
+            if (!sk_wait_bar_warp<true>(ready0 + 8u * stage, (tail_ph >> stage) & 1u, abort_flag, p, 48 + stage, 1)) {
               ok = false;
               break;
             }
