@@ -189,6 +189,24 @@ def test_halves_go_to_even(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_every_mantissa(dtype):
+    """Every mantissa of the row's maximum against every mantissa of x down to 2^-8 of it."""
+    n = 1024 if dtype == torch.float16 else 128
+    a = torch.arange(n, 2 * n)                                   # row maxima, a / n in [1, 2)
+    X, shift = torch.meshgrid(torch.arange(n, 2 * n), torch.arange(0, 9), indexing="ij")
+    X, den = X.flatten(), (1 << shift).flatten()                 # x = X / (n den)
+    num = torch.where(X[None, :] <= a[:, None] * den[None, :], X[None, :], 0)
+    x = torch.cat([a[:, None].double() / n, num.double() / den / n], dim=1).to(dtype)
+    x[:, 1::2] *= -1
+    q, _ = sk.int8_quantize(x.to(DEV))
+    d = (a[:, None] * den[None, :])                              # |Q| = 127 num / d
+    f, r = torch.div(127 * num, d, rounding_mode="floor"), (127 * num) % d
+    want = f + ((2 * r > d) | ((2 * r == d) & (f % 2 == 1))).long()
+    assert torch.equal(q[:, 1:].cpu().long().abs(), want)
+    assert bool((q[:, 0] == 127).all()) and not bool((q[:, 1::2] > 0).any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_extreme_rows(dtype):
     big, tiny = torch.finfo(dtype).max, float(torch.finfo(dtype).smallest_normal) * torch.finfo(dtype).eps
     g = torch.Generator().manual_seed(2)
