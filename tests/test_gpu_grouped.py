@@ -97,6 +97,23 @@ def test_weight_gradient_in_fp32(case, dtype):
     _verify("tn", A, B, sizes, lead, got, torch.float32)
 
 
+@pytest.mark.parametrize("kind,sizes,N,K", [
+    ("nt", [5], 256, 1536), ("nt", [5, 0, 40], 300, 2504), ("nt", [300, 7], 520, 4096), ("nn", [130, 0, 0, 9], 264, 8192),
+    ("nn", [16], 8, 20000), ("nn", [1, 31, 33], 776, 1600), ("nt", [1000], 256, 1536),
+    ("tn", [4000], 256, 256), ("tn", [3001, 0, 700], 264, 300), ("tn", [1025, 2049, 511, 17], 72, 520), ("tn", [9999], 40, 64)])
+def test_sums_split_over_pairs(kind, sizes, N, K):
+    """Few tiles and long sums: several CTA pairs share a tile; twice the same bits."""
+    A, B = _operands(sum(sizes), len(sizes), N, K, torch.bfloat16, N + K, kind)
+    off = _offsets(sizes)
+    got = RUN[kind](A, B, off)
+    sk.check_status()
+    _verify(kind, A, B, sizes, 0, got)
+    for _ in range(5):
+        assert torch.equal(RUN[kind](A, B, off), got)
+    if kind == "tn":
+        _verify(kind, A, B, sizes, 0, RUN[kind](A, B, off, out_dtype=torch.float32), torch.float32)
+
+
 @pytest.mark.parametrize("kind", ["nt", "nn", "tn"])
 @pytest.mark.parametrize("E", [32, 33, 300, 1024])
 def test_many_groups(E, kind):
