@@ -405,12 +405,15 @@ constexpr int SK_CSTAGE_BYTES = 4 * 2 * 4096;
 // groups g_first, g_first + g_step, ... (the warps that share a TMEM lane quadrant split the
 // columns).  NBUF: staging buffers per warp.  Returns the number of columns the warps handle
 // together (a multiple of 64; the rest of the tile goes through sk_store_chunk).
-template <int NBUF = 2, bool I8 = false>
+// ROWS: C's rows are not what TMA can address (a pitch or a base off the 16-byte grid): the warp
+// stores the staged box itself, a row at a time and consecutive lanes to consecutive columns
+// (4-byte words where the rows allow them), instead of every lane walking a row of its own.
+template <int NBUF = 2, bool I8 = false, bool ROWS = false>
 __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtensorMap* tmC, uint32_t cstage,
                                                  int warp_slot, int lane, uint32_t t_addr, uint32_t b_off,
                                                  int grow0, int gcol0, int valid_cols, uint32_t& groups,
                                                  const SkPeers* peers = nullptr, int g_first = 0,
-                                                 int g_step = 1) {
+                                                 int g_step = 1, __half* C = nullptr) {
   using namespace skptx;
   const int full = valid_cols >> 6;
   float rs = 0.f;
@@ -418,7 +421,7 @@ __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtens
   for (int g = g_first; g < full; g += g_step, ++groups) {
     const uint32_t buf = cstage + static_cast<uint32_t>(warp_slot * NBUF + (NBUF == 2 ? (groups & 1u) : 0u)) * 4096u;
     // the store issued from this buffer NBUF groups ago must have read it
-    if (lane == 0) tma_store_wait_read<NBUF - 1>();
+    if (!ROWS && lane == 0) tma_store_wait_read<NBUF - 1>();
     __syncwarp();
     // both 32-column reads of the group in flight before the one wait
     uint32_t raw[2][32];
@@ -452,6 +455,35 @@ __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtens
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(h0), "r"(h1), "r"(h2), "r"(h3)
                      : "memory");
       }
+    }
+    if constexpr (ROWS) {
+      __syncwarp();
+      int rows = p.rows - grow0;
+      if (rows > 32) rows = 32;
+      const bool words = (p.ldc & 1) == 0 && (reinterpret_cast<uintptr_t>(C) & 3u) == 0;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(C) + static_cast<size_t>(grow0) * p.ldc + gcol0 + g * 64;
+      if (words) {
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r) {
+          uint32_t w;
+          asm volatile("ld.shared.u32 %0, [%1];"
+                       : "=r"(w) : "r"(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
+          reinterpret_cast<uint32_t*>(dst + static_cast<size_t>(r) * p.ldc)[lane] = w;
+        }
+      } else {
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int c = h * 32 + lane;
+            uint16_t w;
+            asm volatile("ld.shared.u16 %0, [%1];"
+                         : "=h"(w) : "r"(buf + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2) : "memory");
+            dst[static_cast<size_t>(r) * p.ldc + c] = w;
+          }
+        }
+      }
+      continue;
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -571,6 +603,10 @@ __device__ __forceinline__ void sk_epilogue_loop(const SkParams& p, __half* __re
     if (whole && p.c_tma && cstage != 0 && warp_ok && !dead)
       c_first = sk_store_tile_tma<NBUF, I8>(p, tmC, cstage, warp - 2, lane, t_addr, two ? p.acc_b_off : 0,
                                         r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB) >> 5;
+    if constexpr (I8)
+      if (whole && !p.c_tma && cstage != 0 && warp_ok && !dead)
+        c_first = sk_store_tile_tma<NBUF, I8, true>(p, tmC, cstage, warp - 2, lane, t_addr, two ? p.acc_b_off : 0,
+                                                    r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB, C) >> 5;
     if (warp_ok && !dead) {
       for (int c = c_first + sub; c < nchunks; c += NSUB) {
         float v[32];

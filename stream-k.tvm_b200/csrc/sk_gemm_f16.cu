@@ -354,7 +354,7 @@ sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_const
     else
       sk_epilogue_loop<MODE, 4, 2, I8>(p, C, pid, 0, warp, lane, tmem_base, smem_u32(&ctrl->tmem_full[0]),
                              smem_u32(&ctrl->tmem_empty[0]), &ctrl->bcast, abort_flag, ctrl->pend, &tmC,
-                             p.c_tma ? smem_u32(ctrl) + 1024u : 0u);   // staging behind the control block
+                             p.c_tma || (I8 && !p.transposed) ? smem_u32(ctrl) + 1024u : 0u);   // staging behind the control block
   }
 
   // ------------------------------------------------------------- teardown
@@ -556,7 +556,9 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
   // Whole tiles of a row-major C leave through shared memory and TMA stores (not the
   // transposed store of the swapped order, not the cluster schedule's reduction).
   p.c_tma = (!plan.swap && !split && p.c_vec_ok) ? 1 : 0;
-  const int recv_bytes = split ? sk_cluster_recv_bytes(plan.bn, split) : p.c_tma ? 512 + SK_CSTAGE_BYTES : 0;
+  // (8-bit integers: whole tiles are staged for rows that TMA cannot address, too)
+  const bool stage_c = p.c_tma || (i8 && !plan.swap && !split);
+  const int recv_bytes = split ? sk_cluster_recv_bytes(plan.bn, split) : stage_c ? 512 + SK_CSTAGE_BYTES : 0;
   p.cl_per = split ? sk_cluster_quads_per_cta(plan.bn, split) : 1;
   p.cl_per_div = sk_div_make(p.cl_per);
   sk_fill_tile_params(&p, plan.bn, ROW_STAGE_BYTES, MAX_STAGES, recv_bytes, true);

@@ -341,7 +341,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     }
   } else {
     // ------------------------------------------------------------- epilogue (both CTAs)
-    const uint32_t cstage = p.c_tma ? smem_u32(ctrl) + 1024u : 0u;
+    const uint32_t cstage = p.c_tma || I8 ? smem_u32(ctrl) + 1024u : 0u;   // (I8: staged even where TMA cannot store)
     const uint32_t tmem_full0 = smem_u32(&ctrl->tmem_full[0]);
     const uint32_t tmem_empty0 = mapa_shared(smem_u32(&ctrl->tmem_empty[0]), 0);
     uint32_t nseg = 0;
@@ -406,7 +406,10 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           const uint32_t t_addr = tmem_base + buf * BN + (static_cast<uint32_t>(q * 32) << 16);
           if (warp_ok && !dead && valid_cols > 0) {
             int c_first = 0;
-            if (cstage != 0)
+            if (I8 && !p.c_tma)
+              c_first = sk_store_tile_tma<1, I8, true>(p, &tmC, cstage, warp - 2, lane, t_addr, 0, r0 + q * 32, c0,
+                                                       valid_cols, groups, peers, sub, EPI_WARPS / 4, C) >> 5;
+            else if (cstage != 0)
               c_first = sk_store_tile_tma<1, I8>(p, &tmC, cstage, warp - 2, lane, t_addr, 0, r0 + q * 32, c0,
                                              valid_cols, groups, peers, sub, EPI_WARPS / 4) >> 5;
             for (int c = c_first + sub; c < ((valid_cols + 31) >> 5); c += EPI_WARPS / 4) {

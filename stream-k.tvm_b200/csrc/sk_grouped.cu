@@ -57,7 +57,7 @@ struct GroupedParams {
   int stages;
   int b_step_bytes;          // shared memory per step of this CTA's half of the UMMA N operand
   int zero_rest;             // NT / NN: rows of C that belong to no group are set to zero
-  int c_vec_ok;              // rows of C can take 16-byte stores
+  int c_vec_ok, c_words;     // rows of C can take 16-byte stores; 4-byte stores
   int c_tma;                 // TN: C leaves through TMA stores
   uint32_t idesc;            // with N = 0
   unsigned long long timeout_ns;
@@ -426,6 +426,9 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
       uint16_t* d = C + row * p.ldc + f;
       if (p.c_vec_ok && f + 8 <= p.N) {
         *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else if (p.c_words && f + 8 <= p.N) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(d)[i] = w[i];
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -805,45 +808,58 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     const uint32_t buf_smem = cstage + static_cast<uint32_t>(warp - 2) * 4096u;
     constexpr bool F32 = OUT == OUT_F32;
     constexpr int gcols = F32 ? 32 : 64;            // columns of a 128-byte row of the staging buffer
-    // 32 rows of gcols columns, this lane's row in v, to columns c.. of the tile.
+    // 32 rows of gcols columns, this lane's row in v, to columns c.. of the tile: staged as 32 x 128
+    // bytes, then one TMA store, or, where C's rows are not what TMA can address, a row at a time
+    // with consecutive lanes on consecutive columns.
     auto store_group = [&](const SumTile& tile, int r0, int c, int valid, const float (&v)[gcols / 32][32]) {
-                if (p.c_tma) {
-                  if (lane == 0) tma_store_wait_read<0>();
-                  __syncwarp();
-      #pragma unroll
-                  for (int j = 0; j < 8; ++j) {
-                    const uint32_t a = buf_smem + static_cast<uint32_t>(lane) * 128u +
-                                       ((static_cast<uint32_t>(j) ^ (static_cast<uint32_t>(lane) & 7u)) << 4);
-                    if constexpr (F32) {
-                      st_shared_v4(a, v[0][4 * j], v[0][4 * j + 1], v[0][4 * j + 2], v[0][4 * j + 3]);
-                    } else {
-                      const float* w = &v[j >> 2][(j & 3) * 8];
-                      constexpr int BF = OUT == OUT_BF16;
-                      const uint32_t h0 = sk_pack2(w[0], w[1], BF), h1 = sk_pack2(w[2], w[3], BF);
-                      const uint32_t h2 = sk_pack2(w[4], w[5], BF), h3 = sk_pack2(w[6], w[7], BF);
-                      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(h0), "r"(h1), "r"(h2), "r"(h3)
-                                   : "memory");
-                    }
-                  }
-                  fence_proxy_async_smem();
-                  __syncwarp();
-                  if (lane == 0) {
-                    tma_store_3d(&tmC, buf_smem, tile.c0 + c, r0, tile.e);   // clipped at the edges of C[e]
-                    tma_store_commit();
-                  }
-                } else if (r0 + lane < p.K) {
-                  const long long at = tile.e * p.stride_c + static_cast<long long>(r0 + lane) * p.ldc + tile.c0 + c;
-      #pragma unroll
-                  for (int h = 0; h < gcols / 32; ++h) {
-      #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                      if (c + h * 32 + j < valid) {
-                        if constexpr (F32) static_cast<float*>(Cv)[at + h * 32 + j] = v[h][j];
-                        else static_cast<uint16_t*>(Cv)[at + h * 32 + j] = static_cast<uint16_t>(sk_pack2(v[h][j], 0.f, OUT == OUT_BF16));
-                      }
-                    }
-                  }
-                }
+      if (lane == 0) tma_store_wait_read<0>();
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t a = buf_smem + static_cast<uint32_t>(lane) * 128u +
+                           ((static_cast<uint32_t>(j) ^ (static_cast<uint32_t>(lane) & 7u)) << 4);
+        if constexpr (F32) {
+          st_shared_v4(a, v[0][4 * j], v[0][4 * j + 1], v[0][4 * j + 2], v[0][4 * j + 3]);
+        } else {
+          const float* w = &v[j >> 2][(j & 3) * 8];
+          constexpr int BF = OUT == OUT_BF16;
+          const uint32_t h0 = sk_pack2(w[0], w[1], BF), h1 = sk_pack2(w[2], w[3], BF);
+          const uint32_t h2 = sk_pack2(w[4], w[5], BF), h3 = sk_pack2(w[6], w[7], BF);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(h0), "r"(h1), "r"(h2), "r"(h3)
+                       : "memory");
+        }
+      }
+      if (p.c_tma) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&tmC, buf_smem, tile.c0 + c, r0, tile.e);   // clipped at the edges of C[e]
+          tma_store_commit();
+        }
+        return;
+      }
+      __syncwarp();
+      const long long at = tile.e * p.stride_c + static_cast<long long>(r0) * p.ldc + tile.c0 + c;
+      const int rows = p.K - r0 < 32 ? p.K - r0 : 32;
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r) {
+        const uint32_t row = buf_smem + r * 128;
+        if constexpr (F32) {
+          float w;
+          asm volatile("ld.shared.f32 %0, [%1];"
+                       : "=f"(w) : "r"(row + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
+          if (c + lane < valid) static_cast<float*>(Cv)[at + r * p.ldc + lane] = w;
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int i = h * 32 + lane;
+            uint16_t w;
+            asm volatile("ld.shared.u16 %0, [%1];"
+                         : "=h"(w) : "r"(row + (((i >> 3) ^ (r & 7)) << 4) + (i & 7) * 2) : "memory");
+            if (c + i < valid) static_cast<uint16_t*>(Cv)[at + r * p.ldc + i] = w;
+          }
+        }
+      }
     };
     uint32_t nseg = 0;
     bool dead = false;
@@ -1111,6 +1127,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
   // (row tiles: at most one ragged one per group besides the full ones)
   if ((static_cast<long long>(g->T) / p.bn_max + g->E + 1) * p.tiles_f > (1LL << 30)) return SK_ERR_LIMIT;
   p.c_vec_ok = aligned(C, 16) && (g->ldc & 7) == 0;
+  p.c_words = aligned(C, 4) && (g->ldc & 1) == 0;
   // the box that a tile of bn_max rows loads, see the producer
   const int half = p.bn_max / 2;
   p.b_step_bytes = (half <= 16 ? 16 : half <= 64 ? 64 : 128) * 128;
