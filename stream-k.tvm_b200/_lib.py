@@ -138,6 +138,27 @@ def load(path: str | None = None):
     return lib
 
 
+_host = None
+
+
+def load_host():
+    """The CPython module of the host fast path (csrc/host/sk_torch_host.cpp), bound to the loaded
+    library; built if missing, like the library, and an error if it cannot be loaded."""
+    global _host
+    if _host is None:
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (its libraries have to be loaded first)
+        lib = load()
+        path = _build.HOST_LIB if os.path.exists(_build.HOST_LIB) else _build.build_host()
+        loader = importlib.machinery.ExtensionFileLoader("sk_torch_host", path)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("sk_torch_host", loader))
+        loader.exec_module(mod)
+        mod.bind(*(C.cast(f, C.c_void_p).value for f in (lib.sk_quantize_i8, lib.sk_gemm_i8, lib.sk_gemm_grouped)))
+        _host = mod
+    return _host
+
+
 def check(status: int, where: str) -> None:
     if status != SK_OK:
         raise StreamKError(status, where)

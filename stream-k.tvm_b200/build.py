@@ -1,7 +1,9 @@
 """Build recipe: compiles csrc/*.cu for sm_100a into lib/libstreamk_b200.so.
 
 The library is a plain C-ABI shared object (no torch, no pybind): nvcc only.
-Objects are rebuilt when a source or header is newer than the object.
+Objects are rebuilt when a source or header is newer than the object.  Beside it the host
+compiler makes lib/sk_torch_host.so from csrc/host/sk_torch_host.cpp, a small CPython module
+over torch's headers: the shortcut from tensors to the C ABI that ops.py takes in plain cases.
 
 STREAMK_B200_TRACE=1 builds a second library, lib/libstreamk_b200_trace.so, compiled with
 -DSK_TRACE: its kernels record per-CTA timestamps while sk_debug_set_trace() names a buffer.
@@ -13,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -21,6 +24,8 @@ LIBDIR = os.path.join(HERE, "lib")
 OBJDIR = os.path.join(HERE, "build")
 LIBNAME = "libstreamk_b200.so"
 TRACE_LIBNAME = "libstreamk_b200_trace.so"
+HOST_SRC = os.path.join(CSRC, "host", "sk_torch_host.cpp")
+HOST_LIB = os.path.join(LIBDIR, "sk_torch_host.so")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -56,8 +61,36 @@ def _stale(target: str, deps: list[str]) -> bool:
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def build_host(force: bool = False, verbose: bool = False) -> str:
+    """Compile (if needed) the CPython module of the host fast path and return its path."""
+    header = os.path.join(HERE, "..", "include", "streamk_b200.h")
+    if not force and not _stale(HOST_LIB, [HOST_SRC, header]):
+        return HOST_LIB
+    import torch
+    os.makedirs(LIBDIR, exist_ok=True)
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if not cxx:
+        raise RuntimeError("no C++ compiler found; set CXX")
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{d}" for d in (os.path.join(root, "include"),
+                                os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                                sysconfig.get_paths()["include"], os.path.join(cuda, "include"))),
+           HOST_SRC, "-o", HOST_LIB, f"-L{os.path.join(root, 'lib')}",
+           "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(f"--- {os.path.basename(HOST_SRC)}\n{r.stdout}{r.stderr}\n")
+    if r.returncode != 0:
+        raise RuntimeError(f"compiling {HOST_SRC} failed")
+    return HOST_LIB
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile (if needed) and return the path of the shared library."""
+    build_host(force, verbose)
     objdir = OBJDIR + ("_trace" if trace_build() else "")
     os.makedirs(LIBDIR, exist_ok=True)
     os.makedirs(objdir, exist_ok=True)

@@ -77,6 +77,20 @@ def _on(device: torch.device):
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+# The fast path from tensors to the C ABI (csrc/host/sk_torch_host.cpp): int8_quantize,
+# streamk_int8_nt and the grouped products offer it their arguments first; it returns None where
+# there is anything to check, copy or refuse, and the code below takes over.
+_fast = None
+
+
+def _load_fast():
+    global _fast
+    _fast = L.load_host()
+    for (device, stream), ws in _workspaces.items():
+        _fast.set_workspace(device, stream, ws.ptr, ws.nbytes)
+    return _fast
+
+
 def _workspace(device: torch.device) -> _Workspace:
     """One workspace per (device, stream): launches that may overlap never share one."""
     key = (device.index if device.index is not None else torch.cuda.current_device(),
@@ -86,6 +100,8 @@ def _workspace(device: torch.device) -> _Workspace:
         with torch.cuda.device(device):
             ws = _Workspace(device, key[1])
         _workspaces[key] = ws
+        if _fast is not None:
+            _fast.set_workspace(key[0], key[1], ws.ptr, ws.nbytes)
     return ws
 
 
@@ -111,6 +127,8 @@ def release_cached_memory() -> None:
     first, so nothing in flight still uses them; the next call allocates afresh."""
     for dev in {k[0] for k in _workspaces} | {k[0] for k in _host_pipes}:
         torch.cuda.synchronize(dev)
+    if _fast is not None:
+        _fast.clear_workspaces()
     _workspaces.clear()
     _host_pipes.clear()
 
@@ -615,6 +633,10 @@ def int8_quantize(X: torch.Tensor, *, pdl: bool = False) -> tuple[torch.Tensor, 
     Q = 0, so that products with it are NaN.  Q's row pitch is K rounded up to 16 bytes (what
     streamk_int8_nt reads without a copy).  Rows of X may be strided.  No counterpart in the
     reference."""
+    if not pdl:
+        r = (_fast or _load_fast()).quantize(X)
+        if r is not None:
+            return r
     _check_matrix("X", X, HALF_TYPES)
     M, K = X.shape
     if M < 1 or K < 1:
@@ -662,6 +684,10 @@ def streamk_int8_nt(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, sca
     C = (float(sum) * scale_a) * scale_b, then one rounding to out_dtype.  K at most 131071.
     Operands whose rows are not 16-byte aligned are copied first.  Same schedules and keyword
     options as streamk_fp16_nt (see _options()).  No counterpart in the reference."""
+    if not kw and schedule == "auto" and out_dtype in HALF_TYPES:
+        r = (_fast or _load_fast()).gemm_i8(A, B, scale_a, scale_b, out_dtype == torch.bfloat16)
+        if r is not None:
+            return r
     o = _options(kw)
     if out_dtype not in HALF_TYPES:
         raise TypeError(f"out_dtype must be one of {HALF_TYPES}, got {out_dtype}")
@@ -703,6 +729,12 @@ def _aligned16_batch(t: torch.Tensor) -> torch.Tensor:
 
 
 def _grouped(kind, A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl):
+    if out is None and not (num_sms or timeout_us or pdl) and isinstance(A, torch.Tensor):
+        fp32 = out_dtype is torch.float32
+        if fp32 or out_dtype is None or out_dtype is A.dtype:
+            r = (_fast or _load_fast()).grouped(L.GROUPED_KINDS[kind], A, B, offsets, fp32)
+            if r is not None:
+                return r
     _check_matrix("A", A, HALF_TYPES)
     dtype, device = A.dtype, A.device
     if not isinstance(B, torch.Tensor) or not B.is_cuda:
