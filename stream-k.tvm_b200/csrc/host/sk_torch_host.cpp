@@ -78,7 +78,7 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
   at::Tensor Q = empty({M, K}, {K, 1}, at::kChar, device);
   at::Tensor scale = empty({M}, {1}, at::kFloat, device);
-  const int flags = x->scalar_type() == at::kBFloat16 ? SK_FLAG_BF16 : 0;
+  const int flags = SK_FLAG_PDL | (x->scalar_type() == at::kBFloat16 ? SK_FLAG_BF16 : 0);
   if (g_quantize(x->const_data_ptr(), static_cast<int>(M), static_cast<int>(K), static_cast<int>(ld), flags,
                  Q.mutable_data_ptr(), static_cast<int>(K), static_cast<float*>(scale.mutable_data_ptr()), stream) != SK_OK)
     SK_MISS;
@@ -125,7 +125,7 @@ PyObject* gemm_i8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   p.M = static_cast<int32_t>(M); p.N = static_cast<int32_t>(N); p.K = static_cast<int32_t>(K);
   p.lda = static_cast<int32_t>(lda); p.ldb = static_cast<int32_t>(ldb); p.ldc = static_cast<int32_t>(N);
   p.layout = SK_LAYOUT_NT; p.schedule = SK_SCHED_AUTO; p.fixup = SK_FIXUP_BLOCK_REDUCE;
-  p.flags = bf16 ? SK_FLAG_BF16 : 0;
+  p.flags = SK_FLAG_PDL | (bf16 ? SK_FLAG_BF16 : 0);
   if (g_gemm_i8(&p, a->const_data_ptr(), b->const_data_ptr(), sa, sb, C.mutable_data_ptr(), ws->ptr, ws->bytes, stream) != SK_OK)
     SK_MISS;
   return THPVariable_Wrap(std::move(C));
@@ -170,7 +170,7 @@ PyObject* grouped(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g.kind = static_cast<int32_t>(kind);
   g.T = static_cast<int32_t>(T); g.E = static_cast<int32_t>(E);
   g.N = static_cast<int32_t>(N); g.K = static_cast<int32_t>(K);
-  g.flags = (a->scalar_type() == at::kBFloat16 ? SK_FLAG_BF16 : 0) | (off64 ? SK_FLAG_OFFSETS_64 : 0) |
+  g.flags = SK_FLAG_PDL | (a->scalar_type() == at::kBFloat16 ? SK_FLAG_BF16 : 0) | (off64 ? SK_FLAG_OFFSETS_64 : 0) |
             (fp32 ? SK_FLAG_OUT_F32 : 0) | (tn ? 0 : SK_FLAG_ZERO_REST);
   g.lda = lda; g.ldb = ldb; g.ldc = N; g.stride_b = stride_b; g.stride_c = tn ? K * N : 0;
   if (g_grouped(&g, a->const_data_ptr(), b->const_data_ptr(), off->const_data_ptr(), C.mutable_data_ptr(), ws->ptr, ws->bytes,

@@ -623,7 +623,7 @@ def streamk_fp16_ladder_block_reduce_q4(A, QLB: PackedQ4, *, fixup="block_reduce
 
 
 # --------------------------------------------------------------------------- 8-bit integers
-def int8_quantize(X: torch.Tensor, *, pdl: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+def int8_quantize(X: torch.Tensor, *, pdl: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows of X [M,K] (fp16 or bf16) as 8-bit integers: (Q int8 [M,K], scale fp32 [M]).
 
     With a = max_k |X[m,k]|: scale[m] = a / 127 and Q[m,k] = 127 X[m,k] / a rounded to the
@@ -631,9 +631,10 @@ def int8_quantize(X: torch.Tensor, *, pdl: bool = False) -> tuple[torch.Tensor, 
     One scale per row: tokens when X holds activations, output channels when it holds a weight
     [N,K].  A row of zeros has scale 0; a row that holds a NaN or an infinity has scale NaN and
     Q = 0, so that products with it are NaN.  Q's row pitch is K rounded up to 16 bytes (what
-    streamk_int8_nt reads without a copy).  Rows of X may be strided.  No counterpart in the
+    streamk_int8_nt reads without a copy).  Rows of X may be strided.  pdl: programmatic
+    dependent launch (see _options(); here on unless switched off).  No counterpart in the
     reference."""
-    if not pdl:
+    if pdl:
         r = (_fast or _load_fast()).quantize(X)
         if r is not None:
             return r
@@ -683,12 +684,15 @@ def streamk_int8_nt(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, sca
     32-bit integer sums, exact whatever the schedule: every schedule returns the same bits.
     C = (float(sum) * scale_a) * scale_b, then one rounding to out_dtype.  K at most 131071.
     Operands whose rows are not 16-byte aligned are copied first.  Same schedules and keyword
-    options as streamk_fp16_nt (see _options()).  No counterpart in the reference."""
+    options as streamk_fp16_nt (see _options(); pdl is on unless switched off).  No counterpart
+    in the reference."""
     if not kw and schedule == "auto" and out_dtype in HALF_TYPES:
         r = (_fast or _load_fast()).gemm_i8(A, B, scale_a, scale_b, out_dtype == torch.bfloat16)
         if r is not None:
             return r
     o = _options(kw)
+    if o["pdl"] is None:
+        o["pdl"] = True
     if out_dtype not in HALF_TYPES:
         raise TypeError(f"out_dtype must be one of {HALF_TYPES}, got {out_dtype}")
     o["_bf16"] = out_dtype == torch.bfloat16
@@ -729,7 +733,7 @@ def _aligned16_batch(t: torch.Tensor) -> torch.Tensor:
 
 
 def _grouped(kind, A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl):
-    if out is None and not (num_sms or timeout_us or pdl) and isinstance(A, torch.Tensor):
+    if out is None and pdl and not (num_sms or timeout_us) and isinstance(A, torch.Tensor):
         fp32 = out_dtype is torch.float32
         if fp32 or out_dtype is None or out_dtype is A.dtype:
             r = (_fast or _load_fast()).grouped(L.GROUPED_KINDS[kind], A, B, offsets, fp32)
@@ -794,7 +798,7 @@ def _grouped(kind, A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl):
     return Cout
 
 
-def streamk_grouped_nt(A, B, offsets, *, out=None, num_sms=None, timeout_us=None, pdl=False):
+def streamk_grouped_nt(A, B, offsets, *, out=None, num_sms=None, timeout_us=None, pdl=True):
     """C[t] = B[e] @ A[t] for the group e that row t belongs to: the linear layers of a set of
     experts.  A [T,K] and B [E,N,K] fp16 (or bf16), C [T,N] of the same type, fp32 accumulation.
 
@@ -804,18 +808,18 @@ def streamk_grouped_nt(A, B, offsets, *, out=None, num_sms=None, timeout_us=None
     offsets[0] and from offsets[E] on belong to no group: zero in a fresh result, left as they
     are in `out`.  Offsets out of order are clamped on the device and reported by check_status().
     Its gradients: streamk_grouped_nn(dC, B, offsets) for A, streamk_grouped_tn(dC, A, offsets)
-    for B.  Operands whose rows are not 16-byte aligned are copied first.  No counterpart in the
-    reference."""
+    for B.  Operands whose rows are not 16-byte aligned are copied first.  num_sms, timeout_us, pdl:
+    see _options() (pdl is on unless switched off).  No counterpart in the reference."""
     return _grouped("nt", A, B, offsets, out, None, num_sms, timeout_us, pdl)
 
 
-def streamk_grouped_nn(A, B, offsets, *, out=None, num_sms=None, timeout_us=None, pdl=False):
+def streamk_grouped_nn(A, B, offsets, *, out=None, num_sms=None, timeout_us=None, pdl=True):
     """C[t] = A[t] @ B[e]: A [T,K], B [E,K,N], C [T,N].  The input gradient of streamk_grouped_nt
     (dA = streamk_grouped_nn(dC, B, offsets) with the same B [E,N,K]); otherwise the same rules."""
     return _grouped("nn", A, B, offsets, out, None, num_sms, timeout_us, pdl)
 
 
-def streamk_grouped_tn(A, B, offsets, *, out=None, out_dtype=None, num_sms=None, timeout_us=None, pdl=False):
+def streamk_grouped_tn(A, B, offsets, *, out=None, out_dtype=None, num_sms=None, timeout_us=None, pdl=True):
     """C[e] = sum over the rows t of group e of outer(A[t], B[t]): A [T,K], B [T,N], C [E,K,N], zero
     for an empty group.  The weight gradient of streamk_grouped_nt (dB = streamk_grouped_tn(dC, A,
     offsets)).  out_dtype: the operands' type (default) or torch.float32 (unrounded sums).

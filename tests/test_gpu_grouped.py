@@ -251,6 +251,21 @@ def test_captured_and_replayed_with_other_sizes(kind):
         assert torch.equal(first, second)
 
 
+@pytest.mark.parametrize("kind", ["nt", "nn", "tn"])
+def test_the_fast_path_and_the_long_one_agree(kind):
+    sizes = [9, 0, 30]
+    A, B = _operands(45, 3, 136, 200, torch.bfloat16, 2, kind)
+    for off in (_offsets(sizes, 2), _offsets(sizes, 2, torch.int64)):
+        want = RUN[kind](A, B, off)
+        assert torch.equal(RUN[kind](A, B, off, pdl=False), want)
+        assert torch.equal(RUN[kind](torch.nn.Parameter(A), torch.nn.Parameter(B), off), want)
+        out = torch.zeros_like(want)
+        assert torch.equal(RUN[kind](A, B, off, out=out), want)
+    if kind == "tn":
+        f32 = sk.streamk_grouped_tn(A, B, off, out_dtype=torch.float32)
+        assert torch.equal(sk.streamk_grouped_tn(A, B, off, out_dtype=torch.float32, pdl=False), f32)
+
+
 def test_two_streams_at_once():
     sizes = [100, 0, 260, 40]
     A, B = _operands(400, 4, 520, 256, torch.float16, 5, "nt")

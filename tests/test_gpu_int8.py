@@ -147,6 +147,24 @@ def test_two_streams_and_a_captured_graph():
     assert torch.equal(_bits(out), _bits(sk.streamk_int8_nt(q1, B, s1, sb)))
 
 
+def test_the_fast_path_and_the_long_one_agree():
+    """Plain calls take a shortcut from tensors to the C ABI; options, copies and refusals do not."""
+    A, B, sa, sb = (t.to(DEV) for t in _case(70, 264, 512, seed=2))
+    want = _bits(_ref(*(t.cpu() for t in (A, B, sa, sb)), torch.float16))
+    for kw in ({}, {"pdl": False}, {"schedule": "dp"}, {"num_sms": 20}):
+        assert torch.equal(_bits(sk.streamk_int8_nt(A, B, sa, sb, **kw)), want), kw
+    P = torch.nn.Parameter(torch.randn(33, 512, device=DEV).half())     # a parameter is a plain tensor
+    for x in (P, P.detach()[::2], P.detach()[:, 16:272]):
+        (q, s), (q2, s2) = sk.int8_quantize(x), sk.int8_quantize(x, pdl=False)
+        assert torch.equal(q, q2) and torch.equal(s, s2) and not q.requires_grad and not s.requires_grad
+    held = sk.cached_memory_bytes()
+    assert held > 0
+    sk.release_cached_memory()                                          # the shortcut lets go of it, too
+    assert sk.cached_memory_bytes() == 0
+    assert torch.equal(_bits(sk.streamk_int8_nt(A, B, sa, sb)), want)
+    assert sk.cached_memory_bytes() > 0
+
+
 # ------------------------------------------------------------------------------------ quantiser
 def _codes(x):
     """Nearest integers (halves to even) of 127 x / a in exact rational arithmetic; x: 1-D."""
