@@ -202,6 +202,13 @@ int sk_tile_coords(const sk_schedule_info* s, int tile, int* tile_m, int* tile_n
  * reported device error call sk_workspace_init again.                        */
 size_t sk_workspace_bytes(int num_sms);
 int sk_workspace_init(void* ws, size_t bytes, void* stream);
+/* The part of a workspace that sk_gemm_i8 and sk_gemm_grouped need zeroed: sk_workspace_init over
+ * this many bytes is enough for a workspace that only they use (a few KB; what a captured graph
+ * re-zeroes at the start of every replay).                                                    */
+size_t sk_workspace_header_bytes(int num_sms);
+/* Identifies the capture that `stream` is being recorded into (the runtime's capture id, unique in
+ * the process); 0 if it is not capturing.                                                     */
+int sk_stream_capture_id(void* stream, unsigned long long* id);
 /* Asynchronously copies the 16-byte status word into host_out (pinned memory
  * recommended); valid after the stream is synchronised.                      */
 int sk_poll_status(const void* ws, sk_status* host_out, void* stream);

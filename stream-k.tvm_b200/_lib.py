@@ -75,6 +75,8 @@ SIGNATURES = {
     "sk_memcpy2d_async": (C.c_int, [_P, C.c_size_t, _P, C.c_size_t, C.c_size_t, C.c_size_t, _P]),
     "sk_workspace_bytes": (C.c_size_t, [C.c_int]),
     "sk_workspace_init": (C.c_int, [_P, C.c_size_t, _P]),
+    "sk_workspace_header_bytes": (C.c_size_t, [C.c_int]),
+    "sk_stream_capture_id": (C.c_int, [_P, C.POINTER(C.c_ulonglong)]),
     "sk_poll_status": (C.c_int, [_P, C.POINTER(SkStatus), _P]),
     "sk_gemm_f32": (C.c_int, [C.POINTER(SkProblem), _P, _P, _P, _P, C.c_size_t, _P]),
     "sk_gemm_f32_noalloc": (C.c_int, [C.POINTER(SkProblem), _P, _P, _P, C.POINTER(SkStatus), _P]),

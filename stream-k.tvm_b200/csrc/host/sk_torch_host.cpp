@@ -13,6 +13,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -57,7 +58,10 @@ at::Tensor empty(at::IntArrayRef sizes, at::IntArrayRef strides, at::ScalarType 
 
 bool half_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 
+// The workspace of an eager call; null while the stream captures (a graph has one of its own, which
+// the Python path makes).
 const Workspace* workspace(int device, void* stream) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return nullptr;
   const auto it = g_workspaces.find({device, stream});
   return it == g_workspaces.end() ? nullptr : &it->second;
 }

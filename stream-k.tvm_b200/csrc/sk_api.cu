@@ -229,8 +229,10 @@ void sk_resolve_auto(sk_problem* q, int kernel_kind, int num_sms) {
   // launch is short enough to be bound by latencies, at most one 32-row CTA per SM)
   // (8-bit integers: 9 to 16 rows take a second column tile and a second set of activations; ahead of
   // the tensor-memory kernels, 12.4 against 13.7 us at 16 x 11008 x 4096, until the weights are
-  // many waves of CTAs: 53.6 against 44.5 at 16 x 28672 x 8192)
-  const int gemv_m = gemv_kind == 4 ? (q->N <= 96LL * num_sms ? SK_GEMV_I8_MAX_M : 8) : gemv_kind != 2 ? SK_GEMV_AUTO_M : (q->N <= 32LL * num_sms ? SK_GEMV_Q4_MAX_M : 8);
+  // many waves of CTAs: 53.6 against 44.5 at 16 x 28672 x 8192.
+  // And every CTA reads all the activations, half as many bytes as its weights at N = 4096: with a
+  // deep K the cluster schedule is ahead, 11.4 against 12.2 us at 16 x 4096 x 11008.)
+  const int gemv_m = gemv_kind == 4 ? (q->N > 96LL * num_sms || (q->N <= 32LL * num_sms && q->K > 4096) ? 8 : SK_GEMV_I8_MAX_M) : gemv_kind != 2 ? SK_GEMV_AUTO_M : (q->N <= 32LL * num_sms ? SK_GEMV_Q4_MAX_M : 8);
   if (tiles_open && q->M <= gemv_m && (kernel_kind == 2 || q->layout == SK_LAYOUT_NT)) {
     // Few rows of activations: the weights stream once through a kernel without the tensor-core
     // kernels' fixed costs (tensor-memory allocation, mbarrier rings, a cluster exchange or a
@@ -574,6 +576,18 @@ extern "C" int sk_workspace_init(void* ws, size_t bytes, void* stream) {
   if (bytes < SK_WS_HEADER) return SK_ERR_WORKSPACE;
   cudaError_t e = cudaMemsetAsync(ws, 0, bytes, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return sk_set_cuda_error(e);
+  return SK_OK;
+}
+
+extern "C" size_t sk_workspace_header_bytes(int num_sms) { return num_sms <= 0 ? 0 : sk_ws_acc_offset(num_sms); }
+
+extern "C" int sk_stream_capture_id(void* stream, unsigned long long* id) {
+  if (!id) return SK_ERR_ARG;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long found = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &found);
+  if (e != cudaSuccess) return sk_set_cuda_error(e);
+  *id = status == cudaStreamCaptureStatusNone ? 0ull : found;
   return SK_OK;
 }
 

@@ -105,6 +105,35 @@ def _workspace(device: torch.device) -> _Workspace:
     return ws
 
 
+# Captured calls of the 8-bit integer and grouped products do not use the stream's workspace: graphs
+# are often captured on one stream and replayed on several at a time, and would share it.  Each
+# capture gets a workspace of its own, allocated while capturing and therefore in the graph's
+# memory pool, whose counters a node of the graph zeroes at the start of every replay.  It is held
+# until another capture begins or a call is made outside one; from then on it belongs to the graph
+# like any tensor that its capture made and let go.  (Errors that a replayed kernel reports stay in
+# it: check_status() sees those of eager calls.)
+_capture_ws: dict[int, tuple[int, torch.Tensor]] = {}     # device -> capture id, workspace
+
+
+def _call_workspace(device: torch.device) -> tuple[int, int]:
+    """Address and size of the workspace of a call that may be captured."""
+    stream = _stream_ptr(device)
+    lib = L.load()
+    cid = C.c_ulonglong(0)
+    L.check(lib.sk_stream_capture_id(stream, C.byref(cid)), "sk_stream_capture_id")
+    if cid.value == 0:
+        _capture_ws.pop(device.index, None)
+        ws = _workspace(device)
+        return ws.ptr, ws.nbytes
+    held = _capture_ws.get(device.index)
+    if held is None or held[0] != cid.value:
+        sms = torch.cuda.get_device_properties(device).multi_processor_count
+        buf = torch.empty(int(lib.sk_workspace_bytes(sms)), dtype=torch.uint8, device=device)
+        L.check(lib.sk_workspace_init(buf.data_ptr(), int(lib.sk_workspace_header_bytes(sms)), stream), "sk_workspace_init")
+        held = _capture_ws[device.index] = (cid.value, buf)
+    return held[1].data_ptr(), held[1].numel()
+
+
 def reset_workspace(device=None) -> None:
     """Re-zero the workspace of the current stream (needed after a device-reported error)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
@@ -642,6 +671,7 @@ def int8_quantize(X: torch.Tensor, *, pdl: bool = True) -> tuple[torch.Tensor, t
     M, K = X.shape
     if M < 1 or K < 1:
         raise ValueError(f"X must not be empty, got shape {(M, K)}")
+    _check_int32(M=M, K=K, pitch=X.stride(0))
     X = _rowmajor(X)
     device = X.device
     pitch = -(-K // 16) * 16
@@ -652,6 +682,12 @@ def int8_quantize(X: torch.Tensor, *, pdl: bool = True) -> tuple[torch.Tensor, t
         L.check(L.load().sk_quantize_i8(X.data_ptr(), M, K, X.stride(0) if M > 1 else K, flags, Q.data_ptr(), pitch,
                                         scale.data_ptr(), _stream_ptr(device)), "sk_quantize_i8")
     return (Q if pitch == K else Q[:, :K]), scale
+
+
+def _check_int32(**extents) -> None:
+    for name, v in extents.items():
+        if v > 0x7fffffff:
+            raise ValueError(f"{name} is {v}: extents and pitches are 32-bit numbers")
 
 
 def _check_scale(name: str, s: torch.Tensor, n: int, device) -> torch.Tensor:
@@ -707,6 +743,7 @@ def streamk_int8_nt(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, sca
         raise ValueError(f"Incompatible dimensions: A {tuple(A.shape)} B {tuple(B.shape)}")
     if M < 1 or N < 1 or K < 1:
         raise ValueError(f"operands must not be empty: A {tuple(A.shape)} B {tuple(B.shape)}")
+    _check_int32(M=M, N=N, K=K, pitch_a=A.stride(0), pitch_b=B.stride(0))
     with _on(device):
         scale_a = _check_scale("scale_a", scale_a, M, device)
         scale_b = _check_scale("scale_b", scale_b, N, device)
@@ -714,9 +751,9 @@ def streamk_int8_nt(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, sca
         B, ldb = _rows16(B)
         Cout = _out(o["out"], M, N, out_dtype, device)
         prob = _problem(M, N, K, lda, ldb, Cout.stride(0), "nt", schedule, "block_reduce", o)
-        ws = _workspace(device)
+        ws, ws_bytes = _call_workspace(device)
         L.check(L.load().sk_gemm_i8(C.byref(prob), A.data_ptr(), B.data_ptr(), scale_a.data_ptr(), scale_b.data_ptr(),
-                                    Cout.data_ptr(), ws.ptr, ws.nbytes, _stream_ptr(device)), "sk_gemm_i8")
+                                    Cout.data_ptr(), ws, ws_bytes, _stream_ptr(device)), "sk_gemm_i8")
     return Cout
 
 
@@ -770,6 +807,7 @@ def _grouped(kind, A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl):
         shape = (T, N)
     if N < 1 or K < 1:
         raise ValueError(f"operands must not be empty: A {tuple(A.shape)} B {tuple(B.shape)}")
+    _check_int32(T=T, N=N, K=K)
     if out is not None and (out.shape != shape or out.dtype != dtype or out.device != A.device or out.stride(-1) != 1
                             or out.stride(-2) < N or (kind == "tn" and E > 1 and out.stride(0) < K * out.stride(1))):
         raise ValueError(f"out must be a row-major {list(shape)} tensor of type {dtype} on A's device")
@@ -792,9 +830,9 @@ def _grouped(kind, A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl):
         bs, cs = B.stride(), Cout.stride()
         prob = L.SkGroupedProblem(L.GROUPED_KINDS[kind], T, E, N, K, num_sms or 0, timeout_us or 0, flags,
                                   A.stride(0), bs[-2], cs[-2], 0 if kind == "tn" else bs[0], cs[0] if kind == "tn" else 0)
-        ws = _workspace(device)
+        ws, ws_bytes = _call_workspace(device)
         L.check(L.load().sk_gemm_grouped(C.byref(prob), A.data_ptr(), B.data_ptr(), offsets.data_ptr(), Cout.data_ptr(),
-                                         ws.ptr, ws.nbytes, _stream_ptr(device)), "sk_gemm_grouped")
+                                         ws, ws_bytes, _stream_ptr(device)), "sk_gemm_grouped")
     return Cout
 
 

@@ -282,6 +282,40 @@ def test_two_streams_at_once():
         assert torch.equal(o, want2 if i & 1 else want)
 
 
+def test_two_captured_graphs_replayed_at_once():
+    """Graphs captured on one stream and replayed on two: each has a workspace of its own (the sums
+    here are split, so the counters and the parts in it matter)."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    cases = []
+    for i, (sizes, N, K) in enumerate((([5, 40], 300, 6400), ([130], 264, 8192))):
+        A, B = _operands(sum(sizes), len(sizes), N, K, torch.bfloat16, i, "nt")
+        q = torch.randint(-127, 128, (7, 8192), generator=g, device=DEV, dtype=torch.int8)
+        w = torch.randint(-127, 128, (512, 8192), generator=g, device=DEV, dtype=torch.int8)
+        s, t = torch.rand(7, generator=g, device=DEV), torch.rand(512, generator=g, device=DEV)
+        run = lambda A=A, B=B, off=_offsets(sizes), q=q, w=w, s=s, t=t: [
+            sk.streamk_grouped_nt(A, B, off), sk.streamk_int8_nt(q, w, s, t), sk.streamk_grouped_nt(A, B, off)]
+        want = [r.clone() for r in run()]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run()
+        cases.append((graph, got, want, run))        # (run holds the operands that the graph reads)
+    sk.check_status()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(20):
+        for _, got, _, _ in cases:
+            for r in got:
+                r.fill_(7.0)
+        torch.cuda.synchronize()
+        for (graph, *_), stream in zip(cases, streams):
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for _, got, want, _ in cases:
+            for r, x in zip(got, want):
+                assert torch.equal(r, x)
+
+
 def test_few_sms():
     sizes = [100, 0, 260, 40]
     for kind in ("nt", "nn", "tn"):

@@ -90,8 +90,14 @@ def test_the_shortcut_hands_back_what_it_does_not_take():
         m.grouped("nt", h, h, h, False)
 
 
+def test_workspace_header(lib):
+    assert lib.sk_workspace_header_bytes(0) == 0
+    assert 256 + 16 * 148 <= lib.sk_workspace_header_bytes(148) < 1 << 16
+    assert lib.sk_stream_capture_id(None, None) == L.SK_ERR_ARG
+
+
 @pytest.mark.parametrize("shape,name,tile", [
-    ((1, 11008, 4096), "gemv", None), ((16, 4096, 11008), "gemv", None), ((16, 28672, 8192), "dp", None),
+    ((1, 11008, 4096), "gemv", None), ((16, 4096, 11008), "cluster", (16, 128)), ((16, 11008, 4096), "gemv", None), ((8, 4096, 11008), "gemv", None), ((16, 28672, 8192), "dp", None),
     ((24, 4096, 4096), "cluster", None), ((48, 512, 512), "dp", (128, 64)), ((48, 28672, 1024), "dp", (128, 256)),
     ((100, 4096, 4096), "dp", (128, 64)), ((400, 4096, 4096), "dp", (128, 128)), ((128, 28672, 1024), "dp", (128, 256)),
     ((200, 12288, 4096), "dp", (256, 192)), ((800, 12288, 4096), "dp", (256, 256)), ((8192, 28672, 8192), "dp", (256, 256))])
