@@ -26,12 +26,13 @@ constexpr int BN = 256;              // tile columns (both CTAs see all of them 
 constexpr int BK = 64;
 constexpr int A_STAGE_BYTES = BM * BK * 2;         // 16 KB
 constexpr int B_STAGE_BYTES = (BN / 2) * BK * 2;   // 16 KB: this CTA's half of the B tile
-constexpr int KG = 2;                  // K steps that share a pipeline stage (one barrier round trip)
-constexpr int STAGES = 3;              // 3 x 2 x 32 KB = 192 KB
+// The ring holds six K steps (192 KB).  With wide units two of them share a stage (one barrier round
+// trip); without, each is a stage of its own, refilled as soon as it has been read.
+constexpr int RING_STEPS = 6;
 constexpr int EPI_WARPS = 8;
 constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;   // warp 0 producer, warp 1 MMA issuer, warps 2..9 epilogue
 constexpr int TMEM_COLS = 512;
-constexpr int PIPE_BYTES = STAGES * KG * (A_STAGE_BYTES + B_STAGE_BYTES);
+constexpr int PIPE_BYTES = RING_STEPS * (A_STAGE_BYTES + B_STAGE_BYTES);
 constexpr int CTRL_BYTES = 512;
 constexpr int SMEM_BYTES = PIPE_BYTES + 1024 + CTRL_BYTES + 512 + SK_CSTAGE_BYTES;   // ... + TMA-store staging
 static_assert(SMEM_BYTES <= 232448, "shared memory budget");
@@ -43,8 +44,8 @@ constexpr int W_STAGE_BYTES = A_STAGE_BYTES + 2 * B_STAGE_BYTES;   // 48 KB: A |
 static_assert(WSTAGES * W_STAGE_BYTES <= PIPE_BYTES, "the wide ring lives in the pipeline's memory");
 
 struct Ctrl {
-  uint64_t full[STAGES];      // used in the leader CTA: both CTAs' loads complete here
-  uint64_t empty[STAGES];     // one per CTA, released by the leader's multicast commit
+  uint64_t full[RING_STEPS];    // used in the leader CTA: both CTAs' loads complete here
+  uint64_t empty[RING_STEPS];   // one per CTA, released by the leader's multicast commit
   uint64_t fullw[WSTAGES];    // the same pair for the wide ring
   uint64_t emptyw[WSTAGES];
   uint64_t tmem_full[2];      // one per CTA, multicast commit
@@ -72,6 +73,8 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                         const __grid_constant__ CUtensorMap tmC, __half* __restrict__ C, const SkParams p,
                         const __grid_constant__ SkPeers peer_set) {
   constexpr bool PEERS = OUT == OUT_GATHER;
+  constexpr int KG = WIDE ? 2 : 1;              // K steps that share a pipeline stage
+  constexpr int STAGES = RING_STEPS / KG;
   constexpr int XK = I8 ? 2 * BK : BK;   // elements of K per step
   auto umma = [](uint32_t d, uint64_t da, uint64_t db, uint32_t id, uint32_t acc) {
     if constexpr (I8) umma_i8_ss_pair(d, da, db, id, acc);
@@ -536,7 +539,7 @@ int sk_launch_f16_2cta(const sk_problem* prob, const void* A, const void* B, voi
   p->acc_stride = BN;           // (the accumulator buffers stay 256 columns apart)
   p->col_tx_bytes = (bn / 2) * BK * 2;   // bytes of this CTA's half of a B stage
   p->tmem_cols = TMEM_COLS;
-  p->stages = STAGES;
+  p->stages = RING_STEPS;
   p->idesc = k_i8 ? umma_idesc_i8(2 * BM, bn) : umma_idesc_f16(2 * BM, bn, 0, p->out_bf16);
   // K steps the second half of a 256 x 512 unit stays behind the first (see the MMA issuer).
   // Measured on configuration 5, sustained loop: 1278 TFLOP/s with 0, 1291 with 1, 1137 with 2
