@@ -34,8 +34,7 @@ constexpr int BK = 64;                  // K per step: 128 bytes of a row
 constexpr int HALF_M = 128;             // UMMA M rows per CTA of a pair
 constexpr int A_STEP_BYTES = HALF_M * BK * 2;   // 16 KB
 constexpr int MAX_BN = 256;
-constexpr int KG = 2;                   // steps that share a stage
-constexpr int MAX_STAGES = 6;
+constexpr int MAX_STAGES = 12;
 constexpr int EPI_WARPS = 8;
 constexpr int TMEM_COLS = 512;
 constexpr int SMEM_LIMIT = 232448;
@@ -271,8 +270,8 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw_addr);
   const int STAGES = p.stages;
-  const uint32_t sW = base, sX = base + STAGES * KG * A_STEP_BYTES;
-  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + STAGES * KG * (A_STEP_BYTES + p.b_step_bytes));
+  const uint32_t sW = base, sX = base + STAGES * A_STEP_BYTES;
+  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + STAGES * (A_STEP_BYTES + p.b_step_bytes));
   int* start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ctrl) + CTRL_BYTES + EPI_WARPS * TURN_BYTES);
   int* first = start + p.E + 1;
   volatile uint32_t* abort_flag = &ctrl->abort;
@@ -331,25 +330,23 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
         const int box = half <= 16 ? 16 : half <= 64 ? 64 : 128;
         const uint32_t tx = 2u * (A_STEP_BYTES + static_cast<uint32_t>(box) * 128u);   // of both CTAs
         const int f_row = tile.f0 + rank * HALF_M, x_row = tile.r0 + rank * half;
-        for (int k = tile.k0; k < tile.k1;) {
-          const int n = tile.k1 - k < KG ? tile.k1 - k : KG;
+        for (int k = tile.k0; k < tile.k1; ++k) {
           if (!sk_wait_bar_warp(empty0 + 8u * stage, ph ^ 1u, abort_flag, p, stage, 0)) {
             ok = false;
             break;
           }
           const uint32_t bar = full0_leader + 8u * stage;
-          if (leader && rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, n * tx);
-          for (int j = 0; leader && j < n; ++j) {
-            const uint32_t dW = sW + (stage * KG + j) * A_STEP_BYTES;
+          if (leader) {
+            if (rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, tx);
+            const uint32_t dW = sW + stage * A_STEP_BYTES;
             if constexpr (W_MN) {
-              tma_load_3d_pair(dW, &tmW, bar, f_row, (k + j) * BK, tile.e);
-              tma_load_3d_pair(dW + 8192, &tmW, bar, f_row + 64, (k + j) * BK, tile.e);
+              tma_load_3d_pair(dW, &tmW, bar, f_row, k * BK, tile.e);
+              tma_load_3d_pair(dW + 8192, &tmW, bar, f_row + 64, k * BK, tile.e);
             } else {
-              tma_load_3d_pair(dW, &tmW, bar, (k + j) * BK, f_row, tile.e);
+              tma_load_3d_pair(dW, &tmW, bar, k * BK, f_row, tile.e);
             }
-            tma_load_2d_pair(sX + (stage * KG + j) * p.b_step_bytes, tmX, bar, (k + j) * BK, x_row);
+            tma_load_2d_pair(sX + stage * p.b_step_bytes, tmX, bar, k * BK, x_row);
           }
-          k += n;
           if (++stage == STAGES) { stage = 0; ph ^= 1u; }
         }
       }
@@ -372,25 +369,21 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
         const uint32_t d_tmem = tmem_base + buf * MAX_BN;
         const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tile.bn >> 3) << 17);
         uint32_t accumulate = 0u;
-        for (int k = tile.k0; k < tile.k1;) {
-          const int n = tile.k1 - k < KG ? tile.k1 - k : KG;
+        for (int k = tile.k0; k < tile.k1; ++k) {
           if (!sk_wait_bar_warp(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          for (int j = 0; j < n; ++j) {
-            const uint32_t w_lo = w_lo0 + (stage * KG + j) * (A_STEP_BYTES >> 4);
-            const uint32_t x_lo = x_lo0 + (stage * KG + j) * (static_cast<uint32_t>(p.b_step_bytes) >> 4);
+          const uint32_t w_lo = w_lo0 + stage * (A_STEP_BYTES >> 4);
+          const uint32_t x_lo = x_lo0 + stage * (static_cast<uint32_t>(p.b_step_bytes) >> 4);
 #pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk) {
-              if (leader)
-                umma_f16_ss_pair(d_tmem, w_hi | (w_lo + kk * w_kstep16), x_hi | (x_lo + kk * 2), idesc, accumulate);
-              accumulate = 1u;
-            }
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            if (leader)
+              umma_f16_ss_pair(d_tmem, w_hi | (w_lo + kk * w_kstep16), x_hi | (x_lo + kk * 2), idesc, accumulate);
+            accumulate = 1u;
           }
           if (leader) umma_commit_pair(empty0 + 8u * stage);
-          k += n;
           if (++stage == STAGES) { stage = 0; ph ^= 1u; }
         }
         if (!ok) break;
@@ -1132,9 +1125,11 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
   const int half = p.bn_max / 2;
   p.b_step_bytes = (half <= 16 ? 16 : half <= 64 ? 64 : 128) * 128;
   const int fixed = 1024 + CTRL_BYTES + EPI_WARPS * TURN_BYTES + table_bytes(g->E, true);
-  p.stages = (SMEM_LIMIT - fixed) / (KG * (A_STEP_BYTES + p.b_step_bytes));
+  // Stages of one step each, as many as fit (six for tiles of 256 rows, eleven for the fewest;
+  // three of two steps were 2-5 % slower).
+  p.stages = (SMEM_LIMIT - fixed) / (A_STEP_BYTES + p.b_step_bytes);
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-  const int smem = fixed + p.stages * KG * (A_STEP_BYTES + p.b_step_bytes);
+  const int smem = fixed + p.stages * (A_STEP_BYTES + p.b_step_bytes);
   p.idesc = umma_idesc_f16(2 * HALF_M, 0, 0, bf16) | (nn ? (1u << 15) : 0u);
   p.steps = (g->K + BK - 1) / BK;
   p.d_steps = sk_div_make(p.steps);
