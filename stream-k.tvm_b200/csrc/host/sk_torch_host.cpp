@@ -74,17 +74,18 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor* x = cuda_tensor(args[0]);
   if (x == nullptr || x->dim() != 2 || !half_type(x->scalar_type())) SK_MISS;
   const int64_t M = x->size(0), K = x->size(1);
-  if (!fits_int(M) || !fits_int(K) || K % 16 != 0 || x->stride(1) != 1) SK_MISS;
+  const int64_t pitch = (K + 15) / 16 * 16;
+  if (!fits_int(M) || !fits_int(pitch) || x->stride(1) != 1) SK_MISS;
   const int64_t ld = M > 1 ? x->stride(0) : K;
   if (ld < K || !fits_int(ld)) SK_MISS;
   const at::Device device = x->device();
   const c10::cuda::CUDAGuard guard(device);
   void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-  at::Tensor Q = empty({M, K}, {K, 1}, at::kChar, device);
+  at::Tensor Q = empty({M, K}, {pitch, 1}, at::kChar, device);
   at::Tensor scale = empty({M}, {1}, at::kFloat, device);
   const int flags = SK_FLAG_PDL | (x->scalar_type() == at::kBFloat16 ? SK_FLAG_BF16 : 0);
   if (g_quantize(x->const_data_ptr(), static_cast<int>(M), static_cast<int>(K), static_cast<int>(ld), flags,
-                 Q.mutable_data_ptr(), static_cast<int>(K), static_cast<float*>(scale.mutable_data_ptr()), stream) != SK_OK)
+                 Q.mutable_data_ptr(), static_cast<int>(pitch), static_cast<float*>(scale.mutable_data_ptr()), stream) != SK_OK)
     SK_MISS;
   PyObject* q = THPVariable_Wrap(std::move(Q));
   PyObject* s = THPVariable_Wrap(std::move(scale));

@@ -675,13 +675,13 @@ def int8_quantize(X: torch.Tensor, *, pdl: bool = True) -> tuple[torch.Tensor, t
     X = _rowmajor(X)
     device = X.device
     pitch = -(-K // 16) * 16
-    Q = torch.empty_strided((M, pitch), (pitch, 1), dtype=torch.int8, device=device)
+    Q = torch.empty_strided((M, K), (pitch, 1), dtype=torch.int8, device=device)
     scale = torch.empty_strided((M,), (1,), dtype=torch.float32, device=device)
     flags = (L.SK_FLAG_BF16 if X.dtype == torch.bfloat16 else 0) | (L.SK_FLAG_PDL if pdl else 0)
     with _on(device):
         L.check(L.load().sk_quantize_i8(X.data_ptr(), M, K, X.stride(0) if M > 1 else K, flags, Q.data_ptr(), pitch,
                                         scale.data_ptr(), _stream_ptr(device)), "sk_quantize_i8")
-    return (Q if pitch == K else Q[:, :K]), scale
+    return Q, scale
 
 
 def _check_int32(**extents) -> None:
