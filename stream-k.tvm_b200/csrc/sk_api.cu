@@ -175,6 +175,14 @@ const SkTuned kTuned[] = {
     {-1, 0, 0, 0, 0, 0, 0, 0}};
 }  // namespace
 
+// Clusters of `size` CTAs (one per SM) that can be resident at once: a cluster stays inside a GPC, so
+// not every SM is reached.  Measured on 148 SMs (100 rows, K = 8192, 128 x 64 tiles): up to 15
+// clusters of eight and 32 of four in one wave (8.2 and 9.9 us), one more costs a second (14.1,
+// 17.3).  A little less is assumed, for devices whose SMs are spread differently.
+static long long sk_i8_cluster_cap(int size, int num_sms) {
+  return size == 8 ? num_sms * 10LL / 13 / 8 : size == 4 ? num_sms * 7LL / 8 / 4 : num_sms / 2;
+}
+
 // 8-bit integers: a K step takes half the time per element that it takes 16-bit operands, and a split
 // tile's fix-up takes the same, so whole tiles (data-parallel) are ahead nearly everywhere.
 // Measured over M = 100 .. 6400 at (N, K) = (512, 512) .. (28672, 8192), against the 16-bit rules'
@@ -184,6 +192,8 @@ const SkTuned kTuned[] = {
 //   128 x 128 likewise, 128 x 256 for a single row of tiles beyond that; otherwise CTA pairs, 256 x
 //   256, or 256 x 192 where the waves then take a tenth less (200 x 11008 x 2048: 12.9 us against
 //   13.7; 400 x 12288 x 4096: 26.4 against 28.7).
+// Few tiles and a deep K: 128 x 64 tiles split over clusters (100 x 512 x 8192: 7.4 us against 10.9;
+// 32 tiles, K = 8192: 9.9 against 12.5; with clusters of two, or fewer steps, no gain).
 // M <= 64 keeps the rules below (weights on the UMMA M side, split over clusters), but for short K
 // (48 x 512 x 512: 5.5 us against 11.5) and for more than a wave of tiles (48 x 28672 x 1024: 13.2
 // against 16.9).  False: not decided here.
@@ -196,7 +206,14 @@ static bool resolve_auto_i8(sk_problem* q, int num_sms) {
     q->schedule = SK_SCHED_DP; q->tile_m = m; q->tile_n = n;
     return true;
   };
-  if (q->M <= 64 && !(steps < 8 && tiles(128, 64) <= num_sms) && !(q->M > 32 && tiles(128, 128) > num_sms)) return false;
+  const bool short_k = steps < 8 && tiles(128, 64) <= num_sms;
+  if (q->M <= 64 && !short_k && !(q->M > 32 && tiles(128, 128) > num_sms)) return false;
+  if ((steps >= 32 && tiles(128, 64) <= sk_i8_cluster_cap(8, num_sms)) ||
+      (steps >= 48 && tiles(128, 64) <= sk_i8_cluster_cap(4, num_sms))) {
+    plan(128, 64);
+    q->schedule = SK_SCHED_CLUSTER;
+    return true;
+  }
   if (tiles(128, 64) <= num_sms) return plan(128, 64);
   if (tiles(128, 128) <= num_sms) return plan(128, 128);
   if (q->M <= 128 || (num_sms & 1) != 0) return plan(128, 256);
@@ -389,6 +406,10 @@ int sk_make_sched(const sk_problem* p, int kernel_kind, int num_sms, sk_schedule
     if (plan.bn > (kernel_kind == 2 ? 112 : 192)) return SK_ERR_SHAPE;
     split = 2;
     while (split < 8 && 2 * split * total <= P) split *= 2;
+    // (8-bit integers, whose launches are the shortest: no more clusters than are resident at once,
+    // see sk_i8_cluster_cap; the others keep the sizes, and with them the bits, that they have had)
+    if ((p->flags & SK_FLAG_INTERNAL_I8) != 0)
+      while (split > 2 && total > sk_i8_cluster_cap(split, P)) split /= 2;
     grid = total * split;
   }
   int gm = p->group_m;

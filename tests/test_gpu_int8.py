@@ -35,7 +35,7 @@ def _bits(t):
     return t.cpu().view(torch.int16)
 
 
-SHAPES = [(1, 1, 1), (1, 128, 128), (1, 1000, 333), (2, 300, 1024), (7, 11008, 512), (16, 512, 4096), (17, 129, 640), (33, 4096, 1024),
+SHAPES = [(100, 500, 5000), (70, 1900, 6200), (1, 1, 1), (1, 128, 128), (1, 1000, 333), (2, 300, 1024), (7, 11008, 512), (16, 512, 4096), (17, 129, 640), (33, 4096, 1024),
           (64, 384, 8192), (65, 640, 2048), (100, 1000, 1000), (128, 1024, 1040), (250, 1536, 1024), (384, 384, 8192),
           (513, 1030, 257), (1024, 2048, 512), (2049, 4104, 384), (4096, 4096, 256)]
 

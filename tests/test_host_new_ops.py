@@ -98,7 +98,8 @@ def test_workspace_header(lib):
 
 @pytest.mark.parametrize("shape,name,tile", [
     ((1, 11008, 4096), "gemv", None), ((16, 4096, 11008), "cluster", (16, 128)), ((16, 11008, 4096), "gemv", None), ((8, 4096, 11008), "gemv", None), ((16, 28672, 8192), "dp", None),
-    ((24, 4096, 4096), "cluster", None), ((48, 512, 512), "dp", (128, 64)), ((48, 28672, 1024), "dp", (128, 256)),
+    ((24, 4096, 4096), "cluster", None), ((48, 512, 512), "dp", (128, 64)), ((44, 2176, 2208), "cluster", (48, 128)),
+    ((100, 512, 8192), "cluster", (128, 64)), ((100, 2048, 8192), "cluster", (128, 64)), ((100, 2048, 4096), "dp", (128, 64)), ((48, 28672, 1024), "dp", (128, 256)),
     ((100, 4096, 4096), "dp", (128, 64)), ((400, 4096, 4096), "dp", (128, 128)), ((128, 28672, 1024), "dp", (128, 256)),
     ((200, 12288, 4096), "dp", (256, 192)), ((800, 12288, 4096), "dp", (256, 256)), ((8192, 28672, 8192), "dp", (256, 256))])
 def test_auto_plans(shape, name, tile):
@@ -106,6 +107,11 @@ def test_auto_plans(shape, name, tile):
     assert sk.SCHEDULE_NAMES[p["schedule"]] == name
     if tile:
         assert (p["tile_m"], p["tile_n"]) == tile
+
+
+def test_no_more_clusters_than_are_resident():
+    for N, size in ((14 * 64, 8), (15 * 64, 4), (32 * 64, 4), (33 * 64, 2)):
+        assert sk.schedule_info(100, N, 8192, kind="int8", schedule="cluster", tile_m=128, tile_n=64)["cluster"] == size
 
 
 def test_every_tile_is_walked_once_under_every_schedule():
