@@ -85,24 +85,26 @@ __device__ __forceinline__ float sk_acc_add(float a, float b) {
   if constexpr (I8) return __int_as_float(__float_as_int(a) + __float_as_int(b));
   else return a + b;
 }
+__device__ __forceinline__ float sk_scaled(float raw, float scale_a, float scale_b) {
+  return (__int2float_rn(__float_as_int(raw)) * scale_a) * scale_b;
+}
 __device__ __forceinline__ float sk_scaled(const SkParams& p, float raw, float row_scale, float col_scale) {
-  const float x = __int2float_rn(__float_as_int(raw));
-  return p.transposed ? (x * col_scale) * row_scale : (x * row_scale) * col_scale;
+  return p.transposed ? sk_scaled(raw, col_scale, row_scale) : sk_scaled(raw, row_scale, col_scale);
 }
 
-// Scales of the 32 columns from gcol0 on (a multiple of 32), `valid` of them inside the matrix.
-__device__ __forceinline__ void sk_load_col_scales(const SkParams& p, int gcol0, int valid, float (&cs)[32]) {
-  const float* src = p.col_scale + gcol0;
-  if (valid >= 32 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(src) + j);
-      cs[4 * j] = x.x; cs[4 * j + 1] = x.y; cs[4 * j + 2] = x.z; cs[4 * j + 3] = x.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) cs[j] = j < valid ? __ldg(src + j) : 0.f;
-  }
+// The scales that a warp needs for the first 64 columns it stores of a whole tile: its lane's row and
+// columns lane, lane + 32 of the group.  Fetched while the tile is still being multiplied (a read
+// from L2 in line with every group cost as much as the group's arithmetic); what the group's 32
+// columns share then goes round the lanes through 128 bytes of shared memory per warp.
+struct SkScales {
+  float row, c0, c1;
+};
+__device__ __forceinline__ SkScales sk_fetch_scales(const SkParams& p, int grow, int gcol) {
+  SkScales s;
+  s.row = grow < p.rows ? __ldg(p.row_scale + grow) : 0.f;
+  s.c0 = gcol < p.cols ? __ldg(p.col_scale + gcol) : 0.f;
+  s.c1 = gcol + 32 < p.cols ? __ldg(p.col_scale + gcol + 32) : 0.f;
+  return s;
 }
 
 // nv (<= NC) fp32 values of tile row `grow`, columns gcol0.. -> 16-bit C  (NC = 16 or 32)
@@ -428,14 +430,13 @@ __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtens
                                                  int warp_slot, int lane, uint32_t t_addr, uint32_t b_off,
                                                  int grow0, int gcol0, int valid_cols, uint32_t& groups,
                                                  const SkPeers* peers = nullptr, int g_first = 0,
-                                                 int g_step = 1, __half* C = nullptr) {
+                                                 int g_step = 1, __half* C = nullptr, SkScales scales = SkScales{}) {
   using namespace skptx;
   // I8: a last group that the matrix ends in goes the same way (TMA clips it; the row stores mind the
   // edge), if the tile's own columns are whole groups.  (Through registers it cost 4 us more:
   // 531 x 696 x 2144 12.9 -> 8.2 us.)
   const int full = I8 && (p.bn & 63) == 0 ? (valid_cols + 63) >> 6 : valid_cols >> 6;
-  float rs = 0.f;
-  if constexpr (I8) rs = grow0 + lane < p.rows ? __ldg(p.row_scale + grow0 + lane) : 0.f;   // (rows past the end are clipped)
+  const uint32_t share = cstage + static_cast<uint32_t>(SK_CSTAGE_BYTES) + static_cast<uint32_t>(warp_slot) * 128u;
   for (int g = g_first; g < full; g += g_step, ++groups) {
     const uint32_t buf = cstage + static_cast<uint32_t>(warp_slot * NBUF + (NBUF == 2 ? (groups & 1u) : 0u)) * 4096u;
     // the store issued from this buffer NBUF groups ago must have read it
@@ -459,10 +460,20 @@ __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtens
         for (int j = 0; j < 32; ++j) v[j] = sk_acc_add<I8>(v[j], __uint_as_float(r2[j]));
       }
       if constexpr (I8) {
-        float cs[32];                            // the 32 columns' scales (the same for every lane)
-        sk_load_col_scales(p, gcol0 + g * 64 + h * 32, valid_cols - g * 64 - h * 32, cs);
+        __syncwarp();                            // (the half before has been read)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(share + lane * 4), "f"(h ? scales.c1 : scales.c0) : "memory");
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = sk_scaled(p, v[j], rs, cs[j]);
+        for (int j = 0; j < 8; ++j) {
+          const float4 cs = ld_shared_v4(share + j * 16);
+          v[4 * j + 0] = sk_scaled(v[4 * j + 0], scales.row, cs.x); v[4 * j + 1] = sk_scaled(v[4 * j + 1], scales.row, cs.y);
+          v[4 * j + 2] = sk_scaled(v[4 * j + 2], scales.row, cs.z); v[4 * j + 3] = sk_scaled(v[4 * j + 3], scales.row, cs.w);
+        }
+        if (h == 1 && g + g_step < full) {       // the next group's
+          const float row = scales.row;
+          scales = sk_fetch_scales(p, p.rows, gcol0 + (g + g_step) * 64 + lane);
+          scales.row = row;
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -615,6 +626,10 @@ __device__ __forceinline__ void sk_epilogue_loop(const SkParams& p, __half* __re
     if (!whole) sk_tile_ctas(s, seg.tile, first, last);
     const bool is_tail = !whole && seg.k0 == 0;   // this CTA starts the tile (its "owner")
 
+    SkScales scales{};
+    if constexpr (I8)
+      if (whole && cstage != 0 && warp_ok) scales = sk_fetch_scales(p, grow, c0 + sub * 64 + lane);
+
     // A wait that ran out must not leave the warps disagreeing: every epilogue
     // thread keeps walking the segment list (and meeting the named barriers) but
     // stops touching tensor memory.
@@ -636,11 +651,11 @@ __device__ __forceinline__ void sk_epilogue_loop(const SkParams& p, __half* __re
     int c_first = 0;   // first 32-column chunk that still has to go through the register path
     if (whole && p.c_tma && cstage != 0 && warp_ok && !dead)
       c_first = sk_store_tile_tma<NBUF, I8>(p, tmC, cstage, warp - 2, lane, t_addr, two ? p.acc_b_off : 0,
-                                        r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB) >> 5;
+                                        r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB, nullptr, scales) >> 5;
     if constexpr (I8)
       if (whole && !p.c_tma && cstage != 0 && warp_ok && !dead)
         c_first = sk_store_tile_tma<NBUF, I8, true>(p, tmC, cstage, warp - 2, lane, t_addr, two ? p.acc_b_off : 0,
-                                                    r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB, C) >> 5;
+                                                    r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB, C, scales) >> 5;
     if (warp_ok && !dead) {
       for (int c = c_first + sub; c < nchunks; c += NSUB) {
         float v[32];
@@ -670,7 +685,9 @@ __device__ __forceinline__ void sk_epilogue_loop(const SkParams& p, __half* __re
     __syncwarp();
     if (lane == 0) {
       // with CTA pairs the barrier lives in the leader CTA (a shared::cluster address)
-      if (p.unit_ctas == 2) mbar_arrive_cluster(tmem_empty_bar + 8u * buf);
+      // (relaxed: the accumulator's values are in registers, and a releasing arrival would wait for
+      // the stores in flight)
+      if (p.unit_ctas == 2) mbar_arrive_cluster_relaxed(tmem_empty_bar + 8u * buf);
       else mbar_arrive(tmem_empty_bar + 8u * buf);
     }
 

@@ -558,7 +558,7 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
   p.c_tma = (!plan.swap && !split && p.c_vec_ok) ? 1 : 0;
   // (8-bit integers: whole tiles are staged for rows that TMA cannot address, too)
   const bool stage_c = p.c_tma || (i8 && !plan.swap && !split);
-  const int recv_bytes = split ? sk_cluster_recv_bytes(plan.bn, split) : stage_c ? 512 + SK_CSTAGE_BYTES : 0;
+  const int recv_bytes = split ? sk_cluster_recv_bytes(plan.bn, split) : stage_c ? 512 + SK_CSTAGE_BYTES + (i8 ? 512 : 0) : 0;   // (i8: 128 bytes per epilogue warp, SkScales)
   p.cl_per = split ? sk_cluster_quads_per_cta(plan.bn, split) : 1;
   p.cl_per_div = sk_div_make(p.cl_per);
   sk_fill_tile_params(&p, plan.bn, ROW_STAGE_BYTES, MAX_STAGES, recv_bytes, true);

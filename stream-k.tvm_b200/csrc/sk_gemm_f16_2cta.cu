@@ -34,7 +34,7 @@ constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;   // warp 0 producer, warp 1 MM
 constexpr int TMEM_COLS = 512;
 constexpr int PIPE_BYTES = RING_STEPS * (A_STAGE_BYTES + B_STAGE_BYTES);
 constexpr int CTRL_BYTES = 512;
-constexpr int SMEM_BYTES = PIPE_BYTES + 1024 + CTRL_BYTES + 512 + SK_CSTAGE_BYTES;   // ... + TMA-store staging
+constexpr int SMEM_BYTES = PIPE_BYTES + 1024 + CTRL_BYTES + 512 + SK_CSTAGE_BYTES + 128 * EPI_WARPS;   // ... + TMA-store staging, SkScales
 static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 
 // Wide units (256 x 512: two column-adjacent tiles that share every A stage, one accumulator
@@ -398,6 +398,9 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const bool warp_ok = r0 + q * 32 < p.rows;
         for (int h = 0; h < 2; ++h, ++nseg) {
           const uint32_t buf = nseg & 1u;
+          SkScales scales{};
+          if constexpr (I8)
+            if (warp_ok) scales = sk_fetch_scales(p, r0 + row, (2 * tnw + h) * BN + sub * 64 + lane);
           if (!dead) {
             const bool got = sk_wait_bar(tmem_full0 + 8u * buf, (nseg >> 1) & 1u, abort_flag, p, 24 + buf, 2);
             if (!__all_sync(0xffffffffu, got)) dead = true;
@@ -411,10 +414,10 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             int c_first = 0;
             if (I8 && !p.c_tma)
               c_first = sk_store_tile_tma<1, I8, true>(p, &tmC, cstage, warp - 2, lane, t_addr, 0, r0 + q * 32, c0,
-                                                       valid_cols, groups, peers, sub, EPI_WARPS / 4, C) >> 5;
+                                                       valid_cols, groups, peers, sub, EPI_WARPS / 4, C, scales) >> 5;
             else if (cstage != 0)
               c_first = sk_store_tile_tma<1, I8>(p, &tmC, cstage, warp - 2, lane, t_addr, 0, r0 + q * 32, c0,
-                                             valid_cols, groups, peers, sub, EPI_WARPS / 4) >> 5;
+                                             valid_cols, groups, peers, sub, EPI_WARPS / 4, nullptr, scales) >> 5;
             for (int c = c_first + sub; c < ((valid_cols + 31) >> 5); c += EPI_WARPS / 4) {
               float v[32];
               sk_load_acc(t_addr + c * 32, 0, v);
@@ -425,7 +428,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(tmem_empty0 + 8u * buf);
+          if (lane == 0) mbar_arrive_cluster_relaxed(tmem_empty0 + 8u * buf);
         }
       }
       if (cstage != 0 && lane == 0) tma_store_wait_read<0>();
