@@ -58,6 +58,7 @@ struct GroupedParams {
   int zero_rest;             // NT / NN: rows of C that belong to no group are set to zero
   int c_vec_ok, c_words;     // rows of C can take 16-byte stores; 4-byte stores
   int c_tma;                 // TN: C leaves through TMA stores
+  int c_flat;                // TN: and every C[e] is one piece of memory
   uint32_t idesc;            // with N = 0
   unsigned long long timeout_ns;
   SkWorkspace ws;
@@ -558,6 +559,7 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
 struct SumTile {
   int e, f0, c0;    // group, first row (of K) and column (of N) of the pair's 256 x 256 tile of C[e]
   int r0, rows;     // the group's rows of A and B
+  int local;        // number of the tile inside its group
   int k0, k1;       // steps of 64 rows to add up: all of them, or part `part` of `parts`
   int part, parts;
 };
@@ -579,6 +581,7 @@ struct SumWalk {
     while (t >= per_e && e < p.E) { t -= per_e; ++e; }
     if (e >= p.E) return false;
     const int steps = (start[e + 1] - start[e] + BK - 1) / BK;
+    o.local = t;
     o.k0 = 0; o.k1 = steps; o.part = 0; o.parts = 1;
     if (SPLIT) {
       const int most = steps / SUM_MIN_RUN;
@@ -858,6 +861,17 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     bool dead = false;
     while (walk.next(p, start, units, tile)) {
       const bool some = tile.rows > 0;
+      if (!some && p.c_flat) {
+        // an empty group whose matrix is one piece of memory: its tiles zero equal contiguous
+        // shares of it, half a share per CTA
+        const long long quads = static_cast<long long>(p.K) * p.N * (F32 ? 4 : 2) / 16;
+        const long long tiles2 = 2LL * p.tiles_f * p.tiles_n, me = 2 * tile.local + rank;
+        float4* base = reinterpret_cast<float4*>(static_cast<uint8_t*>(Cv) + tile.e * p.stride_c * (F32 ? 4 : 2));
+        const long long end = quads * (me + 1) / tiles2;
+        for (long long i = quads * me / tiles2 + (threadIdx.x - 64); i < end; i += 32 * EPI_WARPS)
+          base[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        continue;
+      }
       const uint32_t buf = nseg & 1u;
       if (some) {
         if (!dead) {
@@ -1093,6 +1107,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
     p.d_last = sk_div_make(p.tiles_f % p.band ? p.tiles_f % p.band : p.band);
     const int esz = f32 ? 4 : 2;
     p.c_tma = aligned(C, 16) && (p.ldc * esz) % 16 == 0 && (p.stride_c * esz) % 16 == 0;
+    p.c_flat = p.c_tma && p.ldc == g->N;
     p.idesc = umma_idesc_f16(2 * HALF_M, 0, 1, bf16) | (1u << 15);   // both operands MN-major
     CUtensorMap tmA, tmB, tmC;
     memset(&tmC, 0, sizeof(tmC));
