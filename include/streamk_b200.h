@@ -59,7 +59,8 @@ enum { SK_SCHED_STREAMK = 0,        /* every tile is Stream-K'd                 
                                        clusters or workspace fix-ups.  fp16 / bf16 NT and W4A16 with
                                        scale groups of 32 or 64: M <= 4, on the CUDA cores.  W4A16
                                        with groups of 128 and more: M <= 16, register-level
-                                       tensor-core instructions on the packed nibbles.  Partial sums
+                                       tensor-core instructions on the packed nibbles; 8-bit
+                                       integers: M <= 16, the same on the integers.  Partial sums
                                        meet in a fixed order (bitwise reproducible); `fixup`,
                                        tile_m, tile_n, group_m and num_sms < device are ignored;
                                        fp16: N <= 512 x the SM count.  What SK_SCHED_AUTO picks for

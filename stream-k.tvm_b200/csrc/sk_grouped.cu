@@ -13,16 +13,25 @@
 // NT and NN: CTA pairs (cta_group::2).  The weights feed the UMMA M dimension (256 of the N output
 // features per pair, 128 per CTA) and the rows of a group the UMMA N dimension, whose extent the
 // instruction descriptor sets tile by tile in steps of 16: a group of 5 rows costs the tensor
-// cores 32 columns and a group of 300 two tiles of 160 (150 rounded up), where rows on the M side would cost whole
-// multiples of 128 or 256.  Groups of a few rows are then what they should be, a stream of the
+// cores 32 columns and a group of 300 two tiles of 160 (150 rounded up), where rows on the M side
+// would cost whole multiples of 128 or 256.  Groups of a few rows are then what they should be, a stream of the
 // weights.  A pair's accumulator is transposed (lane = feature, column = row of A); a warp turns
 // 32 x 32 of it through shared memory (ldmatrix.trans) and stores 64 contiguous bytes of a row of
-// C with every four lanes.
+// C with every four lanes.  (Stored straight from the registers, two bytes per lane, short sums paid
+// for it: 9472 x 8192 x 512 89 us, turned 63.)
+//
+// What bounds them.  Few rows per group: the stream of the weights (16 rows over eight groups of
+// 11008 x 4096: 112 us, 98 % of the rate of a copy).  Many rows: the tensor cores, 87 % of their
+// cycles at 4 x 8192 x 4096 with 1000 rows each, and under a long load the power limit (16384 rows,
+// 8 x 11008 x 4096: 0.97 ms, 1.52 PFLOP/s, alone; 1.13 ms among others like it).  In between: what an
+// SM can load, 32 KB per step and CTA.
 //
 // TN: the sum runs over a group's rows, so both operands are MN-major (TMA boxes of 64 columns x
 // 64 rows) and a group's last step holds rows of the next group.  Those must not count, whatever
 // they hold: UMMAs past the group's end are not issued (16 rows each), and the rows of the last
-// one that lie past it are zeroed in shared memory, in both operands (0 x NaN is NaN).
+// one that lie past it are zeroed in shared memory, in both operands (0 x NaN is NaN).  Long sums are
+// bound like the other two (16384 rows, 8 x 11008 x 4096: 0.98 ms), short ones by the writing of C
+// (32 groups of 128 rows, 4096 x 2048 in fp32: 208 us, 5.4 TB/s).
 #include "sk_common.cuh"
 #include "sk_epilogue.cuh"
 

@@ -22,10 +22,10 @@
 // of the same place), is plus or minus b / 2.  An odd q is then moved to the even side.
 //
 // Bound: memory (2 bytes read, 1 written per element; about four instructions per element).
-// Measured: 8192 x 11008 of normally distributed bf16 48.4 us, 5.6 TB/s (a copy: 6.6); 16 x 4096
-// 2.1 us, a launch.  Tried: looking again at elements near a half instead of whole rows (57 us: some
-// warp of nearly every row has one, and the row's CTA waits for it); 512 threads a row 65 us, 128
-// threads 62, registers capped for six or eight CTAs an SM no better.
+// Measured: 8192 x 11008 of normally distributed bf16 46.7 us, 5.8 TB/s (a copy: 6.6); 16 x 4096
+// 1.6 us, a launch.  Tried: looking again at the elements near a half instead of at whole rows (57 us:
+// some warp of nearly every row has one, and the row's CTA waits for it); 512 threads a row 65 us,
+// 128 threads 62; registers capped for five CTAs an SM are 3 % ahead of no cap, for six no better.
 #include "sk_common.cuh"
 
 namespace {
@@ -128,7 +128,7 @@ __device__ __forceinline__ uint2 quantize8(const uint4& v, const RowScale& s) {
 // and stays in registers; NV = 0: rows longer than that are read twice (the second time mostly
 // from L2).
 template <bool BF16, bool VEC, int G, int NV>
-__global__ void __launch_bounds__(G < 128 ? 128 : G)
+__global__ void __launch_bounds__(G < 128 ? 128 : G, G == 256 ? 5 : 1)
 sk_quantize_i8_kernel(const uint16_t* __restrict__ X, int M, int K, int ldx, int8_t* __restrict__ Q, int ldq,
                       float* __restrict__ scale) {
   constexpr int THREADS = G < 128 ? 128 : G;
