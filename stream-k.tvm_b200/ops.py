@@ -107,12 +107,13 @@ def _workspace(device: torch.device) -> _Workspace:
 
 # Captured calls of the 8-bit integer and grouped products do not use the stream's workspace: graphs
 # are often captured on one stream and replayed on several at a time, and would share it.  Each
-# capture gets a workspace of its own, allocated while capturing and therefore in the graph's
-# memory pool, whose counters a node of the graph zeroes at the start of every replay.  It is held
-# until another capture begins or a call is made outside one; from then on it belongs to the graph
-# like any tensor that its capture made and let go.  (Errors that a replayed kernel reports stay in
-# it: check_status() sees those of eager calls.)
-_capture_ws: dict[int, tuple[int, torch.Tensor]] = {}     # device -> capture id, workspace
+# capture gets workspaces of its own, one for each stream that it records (its branches may run at
+# the same time), allocated while capturing and therefore in the graph's memory pool, whose
+# counters a node of the graph zeroes at the start of every replay.  They are held until another
+# capture begins or a call is made outside one; from then on they belong to the graph like any
+# tensor that its capture made and let go.  (Errors that a replayed kernel reports stay in
+# them: check_status() sees those of eager calls.)
+_capture_ws: dict[int, tuple[int, dict[int, torch.Tensor]]] = {}     # device -> capture id, stream -> workspace
 
 
 def _call_workspace(device: torch.device) -> tuple[int, int]:
@@ -127,11 +128,14 @@ def _call_workspace(device: torch.device) -> tuple[int, int]:
         return ws.ptr, ws.nbytes
     held = _capture_ws.get(device.index)
     if held is None or held[0] != cid.value:
+        held = _capture_ws[device.index] = (cid.value, {})
+    buf = held[1].get(stream)
+    if buf is None:
         sms = torch.cuda.get_device_properties(device).multi_processor_count
         buf = torch.empty(int(lib.sk_workspace_bytes(sms)), dtype=torch.uint8, device=device)
         L.check(lib.sk_workspace_init(buf.data_ptr(), int(lib.sk_workspace_header_bytes(sms)), stream), "sk_workspace_init")
-        held = _capture_ws[device.index] = (cid.value, buf)
-    return held[1].data_ptr(), held[1].numel()
+        held[1][stream] = buf
+    return buf.data_ptr(), buf.numel()
 
 
 def reset_workspace(device=None) -> None:
@@ -146,6 +150,7 @@ def reset_workspace(device=None) -> None:
 def cached_memory_bytes() -> int:
     """Device bytes held by the cached workspaces and host-pipeline staging buffers."""
     n = sum(ws.nbytes for ws in _workspaces.values())
+    n += sum(buf.numel() for _, held in _capture_ws.values() for buf in held.values())
     for pipe in _host_pipes.values():
         n += pipe.nbytes
     return n
@@ -159,6 +164,7 @@ def release_cached_memory() -> None:
     if _fast is not None:
         _fast.clear_workspaces()
     _workspaces.clear()
+    _capture_ws.clear()
     _host_pipes.clear()
 
 

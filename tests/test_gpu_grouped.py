@@ -316,6 +316,34 @@ def test_two_captured_graphs_replayed_at_once():
                 assert torch.equal(r, x)
 
 
+def test_branches_of_one_captured_graph():
+    """Two streams recorded into one graph: their split sums run at the same time in every replay."""
+    sizes, N, K = [5, 40], 300, 6400
+    off = _offsets(sizes)
+    pairs = [_operands(sum(sizes), len(sizes), N, K, torch.bfloat16, i, "nt") for i in range(2)]
+    want = [sk.streamk_grouped_nt(A, B, off).clone() for A, B in pairs]
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        got = [[], []]
+        for _ in range(4):
+            got[0].append(sk.streamk_grouped_nt(*pairs[0], off))
+            with torch.cuda.stream(side):
+                got[1].append(sk.streamk_grouped_nt(*pairs[1], off))
+        main.wait_stream(side)
+    for _ in range(10):
+        for r in got[0] + got[1]:
+            r.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        for branch, x in zip(got, want):
+            for r in branch:
+                assert torch.equal(r, x)
+    sk.check_status()
+
+
 def test_few_sms():
     sizes = [100, 0, 260, 40]
     for kind in ("nt", "nn", "tn"):
