@@ -255,9 +255,10 @@ int sk_gemm_f16(const sk_problem* p, const void* A, const void* B, void* C,
  * bits; C = ((float)sum * scale_a[m]) * scale_b[n], rounded once more to 16 bits.  Same
  * schedules, tiles and workspace as sk_gemm_f16.  layout NT; fixup SK_FIXUP_BLOCK_REDUCE (there
  * is no fp32 partial to add atomically: SK_ERR_ARG); lda, ldb multiples of 16, A and B 16-byte
- * aligned; K at most SK_I8_MAX_K (the largest whose sum cannot leave 32 bits; SK_ERR_LIMIT);
+ * aligned; K at most SK_I8_MAX_K (the largest whose sum cannot leave 32 bits; SK_ERR_LIMIT), M
+ * and N at most SK_I8_MAX_ROWS;
  * CTA pairs (tile_m = 256): tile_n a multiple of 32.  No counterpart in the reference.       */
-enum { SK_I8_MAX_K = 131071 };
+enum { SK_I8_MAX_K = 131071, SK_I8_MAX_ROWS = 0x7fff0000 };
 int sk_gemm_i8(const sk_problem* p, const void* A, const void* B, const float* scale_a, const float* scale_b,
                void* C, void* ws, size_t ws_bytes, void* stream);
 /* Rows of fp16 (bf16 with SK_FLAG_BF16 in flags) to 8-bit integers, one scale per row: with
@@ -283,8 +284,8 @@ int sk_quantize_i8(const void* X, int M, int K, int ldx, int flags, void* Q, int
  * is one sum in a fixed order: bitwise reproducible.  What other rows hold (infinities, NaN) does
  * not reach a group's results.  Offsets that descend or leave [0, T] are clamped on the device,
  * nothing is read or written out of range, and the status word reports SK_ERR_ARG (detail0: the
- * first index found).  E at most SK_GROUPED_MAX_GROUPS, T at most SK_GROUPED_MAX_ROWS; the
- * workspace is that of the other products.  No counterpart in the reference.               */
+ * first index found).  E at most SK_GROUPED_MAX_GROUPS; T, N and K at most SK_GROUPED_MAX_ROWS;
+ * num_sms at least 2 (CTA pairs); the workspace is that of the other products.  No counterpart in the reference.               */
 enum { SK_GROUPED_NT = 0, SK_GROUPED_NN = 1, SK_GROUPED_TN = 2 };
 enum { SK_GROUPED_MAX_GROUPS = 1024, SK_GROUPED_MAX_ROWS = 0x7fff0000 };
 typedef struct sk_grouped_problem {

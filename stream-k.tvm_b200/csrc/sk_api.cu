@@ -521,7 +521,7 @@ static int schedule_for(const sk_problem* p, int kernel_kind, int num_sms, int n
   sk_problem q = *p, half;
   const bool i8 = kernel_kind == 4;
   if (i8) {
-    if (p->K > SK_I8_MAX_K) return SK_ERR_LIMIT;
+    if (p->K > SK_I8_MAX_K || p->M > SK_I8_MAX_ROWS || p->N > SK_I8_MAX_ROWS) return SK_ERR_LIMIT;
     half = sk_i8_problem(p);
     p = &half;
     kernel_kind = 1;

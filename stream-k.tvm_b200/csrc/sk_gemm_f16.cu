@@ -682,7 +682,7 @@ extern "C" int sk_gemm_i8(const sk_problem* prob, const void* A, const void* B, 
   if (!prob || !scale_a || !scale_b) return SK_ERR_ARG;
   if (prob->layout != SK_LAYOUT_NT || prob->fixup != SK_FIXUP_BLOCK_REDUCE) return SK_ERR_ARG;
   if (prob->M <= 0 || prob->N <= 0 || prob->K <= 0 || prob->lda < prob->K || prob->ldb < prob->K) return SK_ERR_SHAPE;
-  if (prob->K > SK_I8_MAX_K) return SK_ERR_LIMIT;
+  if (prob->K > SK_I8_MAX_K || prob->M > SK_I8_MAX_ROWS || prob->N > SK_I8_MAX_ROWS) return SK_ERR_LIMIT;
   if ((prob->lda & 15) != 0 || (prob->ldb & 15) != 0) return SK_ERR_ALIGN;
   if (((reinterpret_cast<uintptr_t>(scale_a) | reinterpret_cast<uintptr_t>(scale_b)) & 3u) != 0) return SK_ERR_ALIGN;
   const sk_problem half = sk_i8_problem(prob);

@@ -1037,6 +1037,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
   if (g->kind < SK_GROUPED_NT || g->kind > SK_GROUPED_TN) return SK_ERR_ARG;
   if (g->T <= 0 || g->E <= 0 || g->N <= 0 || g->K <= 0) return SK_ERR_SHAPE;
   if (g->E > SK_GROUPED_MAX_GROUPS || g->T > SK_GROUPED_MAX_ROWS) return SK_ERR_LIMIT;
+  if (g->N > SK_GROUPED_MAX_ROWS || g->K > SK_GROUPED_MAX_ROWS) return SK_ERR_LIMIT;   // (room to round up to a tile)
   const bool tn = g->kind == SK_GROUPED_TN, nn = g->kind == SK_GROUPED_NN;
   const bool f32 = (g->flags & SK_FLAG_OUT_F32) != 0;
   if (f32 && !tn) return SK_ERR_ARG;

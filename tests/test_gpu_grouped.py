@@ -344,6 +344,43 @@ def test_branches_of_one_captured_graph():
     sk.check_status()
 
 
+def _random(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(sum(shape)))
+
+
+@pytest.mark.parametrize("kind", ["nt", "nn"])
+def test_addresses_beyond_32_bits(kind):
+    """More than 2^31 elements in the rows, in the weights and in the result: what lies behind them
+    is right."""
+    for T, E, N, K in ((600_000, 3, 136, 4096), (70_000, 2, 33_000, 72), (40, 70, 8192, 4096)):
+        A = _random(T, K)
+        B = _random(E, N, K) if kind == "nt" else _random(E, K, N)
+        last = 37 if T > 100 else 3
+        sizes = [0] * E
+        sizes[0], sizes[-1] = T - last, last
+        got = RUN[kind](A, B, _offsets(sizes))
+        _verify(kind, A[-last:], B[-1:], [last], 0, got[-last:])
+        a = A[:5].clone()
+        _verify(kind, a, B, [5] + [0] * (E - 1), 0, got[:5])
+        sk.check_status()
+
+
+def test_weight_gradient_beyond_32_bits():
+    A, B = _random(600_000, 4096), _random(600_000, 72)         # rows of a group behind 2^31 elements
+    got = sk.streamk_grouped_tn(A, B, _offsets([599_900, 0, 100]))
+    _verify("tn", A[-100:], B[-100:], [100], 0, got[2:])
+    assert not bool(got[1].any())
+    A, B = _random(300, 8192), _random(300, 4096)               # a result of 2^31 elements and more
+    sizes = [0] * 66
+    sizes[0], sizes[-2] = 100, 200
+    for N in (4096, 4095):
+        got = sk.streamk_grouped_tn(A, B[:, :N], _offsets(sizes), out_dtype=torch.float32)
+        _verify("tn", A[100:], B[100:, :N], [200], 0, got[-2:-1])
+        assert not bool(got[-1].any()) and not bool(got[1:-2].any())
+        del got
+    sk.check_status()
+
+
 def test_few_sms():
     sizes = [100, 0, 260, 40]
     for kind in ("nt", "nn", "tn"):

@@ -292,3 +292,28 @@ def test_quantised_layer_is_near_the_unquantised_one():
     bound = X.double().abs().sum(1)[:, None] * sw / 2 + W.double().abs().sum(1)[None, :] * sx / 2 + 1024 * sx * sw / 4
     assert bool(((C - ref).abs() <= bound * (1 + 1e-6) + C.abs() * (2.0 ** -11 + 2.0 ** -21) + 2.0 ** -24).all())
     assert oracle.rel_err(C, ref) <= 2e-2
+
+
+def test_addresses_beyond_32_bits():
+    """More than 2^31 elements in the result, in the weights and in the quantised rows; what lies behind
+    them is compared with small calls on copies."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+
+    def ints(*shape):
+        return torch.randint(-128, 128, shape, generator=g, device=DEV, dtype=torch.int8)
+
+    for M, N, K in ((70_000, 33_000, 80), (20, 33_000, 70_000), (3, 33_000, 70_000), (33_000, 20, 70_000)):
+        A, B = ints(M, K), ints(N, K)
+        sa, sb = torch.rand(M, generator=g, device=DEV), torch.rand(N, generator=g, device=DEV)
+        got = sk.streamk_int8_nt(A, B, sa, sb, out_dtype=torch.bfloat16)
+        sk.check_status()
+        for rows in (slice(0, 3), slice(M - 3, M)):
+            for cols in (slice(0, 20), slice(N - 20, N)):
+                ref = _ref(*(t.cpu() for t in (A[rows], B[cols], sa[rows], sb[cols])), torch.bfloat16)
+                assert torch.equal(_bits(got[rows, cols].contiguous()), _bits(ref)), (M, N, K, rows, cols)
+        del A, B, got
+    X = torch.empty(530_000, 4104, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    q, s = sk.int8_quantize(X)
+    for rows in (slice(0, 5), slice(523_270, 523_275), slice(529_995, 530_000)):
+        q1, s1 = sk.int8_quantize(X[rows].clone())
+        assert torch.equal(q[rows], q1) and torch.equal(s[rows], s1)

@@ -26,7 +26,8 @@ def test_int8_refusals(lib):
         assert _i8(lib, **kw) == L.SK_ERR_SHAPE, kw
     for kw in (dict(lda=72), dict(ldb=65), dict(sa=FAKE + 2), dict(sb=FAKE + 1)):
         assert _i8(lib, **kw) == L.SK_ERR_ALIGN, kw
-    assert _i8(lib, K=131072, lda=131072, ldb=131072) == L.SK_ERR_LIMIT
+    for kw in (dict(K=131072, lda=131072, ldb=131072), dict(M=0x7fff0001), dict(N=0x7fffffff, ldc=0x7fffffff)):
+        assert _i8(lib, **kw) == L.SK_ERR_LIMIT, kw
 
 
 def _quant(lib, X=FAKE, M=2, K=8, ldx=8, Q=FAKE, ldq=16, s=FAKE):
@@ -57,7 +58,10 @@ def test_grouped_refusals(lib):
                dict(ldb=33),   # (16 rows of 33 do not fit the 512 between two groups)
                dict(kind=1, ldb=8), dict(kind=2, ldb=8), dict(kind=2, stride_c=511)):
         assert _grouped(lib, **kw) == L.SK_ERR_SHAPE, kw
-    for kw in (dict(E=1025), dict(T=0x7fff0001)):
+    wide = dict(ldb=0x7ffffff8, ldc=0x7fffffff, stride_b=1 << 40, stride_c=1 << 40)
+    for kw in (dict(E=1025), dict(T=0x7fff0001), dict(N=0x7fff0001, stride_b=1 << 40, ldc=0x7fffffff),
+               dict(kind=1, N=0x7fffffff, **wide), dict(kind=2, N=0x7fffffff, **wide),
+               dict(kind=2, K=0x7fff0001, lda=1 << 31, stride_c=1 << 40)):
         assert _grouped(lib, **kw) == L.SK_ERR_LIMIT, kw
     for kw in (dict(A=FAKE + 8), dict(B=FAKE + 2), dict(lda=36), dict(ldb=33, stride_b=528), dict(stride_b=516), dict(out=FAKE + 1),
                dict(off=FAKE + 2), dict(off=FAKE + 4, flags=L.SK_FLAG_OFFSETS_64),
