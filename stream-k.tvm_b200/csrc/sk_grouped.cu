@@ -29,9 +29,11 @@
 // TN: the sum runs over a group's rows, so both operands are MN-major (TMA boxes of 64 columns x
 // 64 rows) and a group's last step holds rows of the next group.  Those must not count, whatever
 // they hold: UMMAs past the group's end are not issued (16 rows each), and the rows of the last
-// one that lie past it are zeroed in shared memory, in both operands (0 x NaN is NaN).  Long sums are
+// one that lie past it are zeroed in shared memory, in both operands (0 x NaN is NaN).  A last step
+// of up to 16 or 32 rows loads only as many (60 groups of 5 rows, 1408 x 2048: 80 us with 64 loaded
+// and zeroed piece by piece, 64 now).  Long sums are
 // bound like the other two (16384 rows, 8 x 11008 x 4096: 0.98 ms), short ones by the writing of C
-// (32 groups of 128 rows, 4096 x 2048 in fp32: 208 us, 5.4 TB/s).
+// (32 groups of 128 rows, 4096 x 2048 in fp32: 202 us, 5.3 TB/s; zeros alone 5.9).
 #include "sk_common.cuh"
 #include "sk_epilogue.cuh"
 
@@ -623,12 +625,17 @@ __device__ __forceinline__ bool step_needs_zeros(int k, int rows) {
   return (k + 1) * BK > rows && (rows & 15) != 0;
 }
 
+// Tensor maps of A and B with boxes of 16, 32 and 64 rows.
+struct alignas(64) SumMaps {
+  CUtensorMap a[3], b[3];
+};
+
 constexpr int OUT_F16 = 0, OUT_BF16 = 1, OUT_F32 = 2;   // type of C
 
 template <int OUT, bool SPLIT>
 __global__ void __launch_bounds__(TN_THREADS, 1)
-sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                      const __grid_constant__ CUtensorMap tmC, void* __restrict__ Cv, const GroupedParams p) {
+sk_grouped_sum_kernel(const __grid_constant__ SumMaps maps, const __grid_constant__ CUtensorMap tmC,
+                      void* __restrict__ Cv, const GroupedParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -658,8 +665,10 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     ctrl->abort = 0u;
     fence_mbar_init();
     fence_proxy_async_smem();
-    prefetch_tensormap(&tmA);
-    prefetch_tensormap(&tmB);
+    for (int i = 0; i < 3; ++i) {
+      prefetch_tensormap(&maps.a[i]);
+      prefetch_tensormap(&maps.b[i]);
+    }
     if (p.c_tma) prefetch_tensormap(&tmC);
   }
   if (warp == 1) {
@@ -699,7 +708,10 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           // same, so that the parities of the ring stay in step.)
           const bool tail = step_needs_zeros(k, tile.rows);
           const int b_chunks = p.bn_max / 128;            // of 64 columns
-          const uint32_t bytes = A_STEP_BYTES + b_chunks * 8192u;
+          // (a short step loads 16 or 32 rows: what lies past them no UMMA reads)
+          const int left = tile.rows - k * BK, size = left <= 16 ? 0 : left <= 32 ? 1 : 2;
+          const CUtensorMap *tmA = &maps.a[size], *tmB = &maps.b[size];
+          const uint32_t bytes = (2 + b_chunks) * (2048u << size);
           uint32_t bar = full0_leader + 8u * stage;
           if (tail) bar = tail0 + 8u * stage;
           if (leader) {
@@ -714,11 +726,11 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           const int row = tile.r0 + k * BK;
           for (int h = 0; leader && h < 2; ++h) {
             if (tail) {
-              tma_load_2d(dA + h * 8192, &tmA, bar, a_col + h * 64, row);
-              if (h < b_chunks) tma_load_2d(dB + h * 8192, &tmB, bar, b_col + h * 64, row);
+              tma_load_2d(dA + h * 8192, tmA, bar, a_col + h * 64, row);
+              if (h < b_chunks) tma_load_2d(dB + h * 8192, tmB, bar, b_col + h * 64, row);
             } else {
-              tma_load_2d_pair(dA + h * 8192, &tmA, bar, a_col + h * 64, row);
-              if (h < b_chunks) tma_load_2d_pair(dB + h * 8192, &tmB, bar, b_col + h * 64, row);
+              tma_load_2d_pair(dA + h * 8192, tmA, bar, a_col + h * 64, row);
+              if (h < b_chunks) tma_load_2d_pair(dB + h * 8192, tmB, bar, b_col + h * 64, row);
             }
           }
           if (++stage == STAGES) { stage = 0; ph ^= 1u; }
@@ -792,11 +804,12 @@ sk_grouped_sum_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           // rows lo .. hi of the step's 64, 128 bytes in each of the four chunks (swizzling moves
           // 16-byte pieces inside a row, so a whole row is a whole row)
           const int lo = tile.rows - k * BK, hi = (lo + 15) & ~15;
-          const int pieces = (hi - lo) * 8;
-          for (int i = lane; i < 4 * pieces; i += 32) {
-            const int chunk = i / pieces, piece = i - chunk * pieces;
-            const uint32_t b = (chunk < 2 ? sA + stage * A_STEP_BYTES : sB + stage * TN_B_STEP) + (chunk & 1) * 8192;
-            st_shared_v4(b + lo * 128 + piece * 16, 0.f, 0.f, 0.f, 0.f);
+          const uint32_t a = sA + stage * A_STEP_BYTES, b = sB + stage * TN_B_STEP;
+          for (int i = lo * 128 + lane * 16; i < hi * 128; i += 512) {
+            st_shared_v4(a + i, 0.f, 0.f, 0.f, 0.f);
+            st_shared_v4(a + 8192 + i, 0.f, 0.f, 0.f, 0.f);
+            st_shared_v4(b + i, 0.f, 0.f, 0.f, 0.f);
+            st_shared_v4(b + 8192 + i, 0.f, 0.f, 0.f, 0.f);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -1119,23 +1132,29 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
     p.c_tma = aligned(C, 16) && (p.ldc * esz) % 16 == 0 && (p.stride_c * esz) % 16 == 0;
     p.c_flat = p.c_tma && p.ldc == g->N;
     p.idesc = umma_idesc_f16(2 * HALF_M, 0, 1, bf16) | (1u << 15);   // both operands MN-major
-    CUtensorMap tmA, tmB, tmC;
+    SumMaps maps;
+    CUtensorMap tmC;
     memset(&tmC, 0, sizeof(tmC));
-    st = make_map(&tmA, A, false, 0, g->T, g->K, g->lda, 0, 64, 64);
-    if (st == SK_OK) st = make_map(&tmB, B, false, 0, g->T, g->N, ldb, 0, 64, 64);
+    for (int i = 0; i < 3 && st == SK_OK; ++i) {
+      st = make_map(&maps.a[i], A, false, 0, g->T, g->K, g->lda, 0, 64, 16u << i);
+      if (st == SK_OK) st = make_map(&maps.b[i], B, false, 0, g->T, g->N, ldb, 0, 64, 16u << i);
+    }
     if (st == SK_OK && p.c_tma) st = make_map(&tmC, C, f32, g->E, g->K, g->N, p.ldc, p.stride_c, f32 ? 32 : 64, 32);
     if (st != SK_OK) return st;
     // Stages: as many as fit, six for up to 383 groups, five above.
     const int fixed = 1024 + EPI_WARPS * 4096 + CTRL_BYTES + table_bytes(g->E, false);
     p.stages = (SMEM_LIMIT - fixed) / TN_STEP;
-    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+    // fp32 results of short sums are bound by their stores, which do better with less read ahead of
+    // them: four, up to 2.5 steps per group (32 groups of 128 rows, 4096 x 2048: 213 -> 202 us; with
+    // 190 rows 211 -> 220)
+    if (f32 && 2LL * g->T <= 5LL * BK * g->E && p.stages > 4) p.stages = 4;
     const int smem = fixed + p.stages * TN_STEP;
     const int grid = 2 * static_cast<int>(total * p.parts < units ? total * p.parts : units);
     const bool split = p.parts > 1;
     auto kernel = f32 ? (split ? sk_grouped_sum_kernel<OUT_F32, true> : sk_grouped_sum_kernel<OUT_F32, false>)
                   : bf16 ? (split ? sk_grouped_sum_kernel<OUT_BF16, true> : sk_grouped_sum_kernel<OUT_BF16, false>)
                          : (split ? sk_grouped_sum_kernel<OUT_F16, true> : sk_grouped_sum_kernel<OUT_F16, false>);
-    e = sk_launch(kernel, grid, TN_THREADS, smem, cs, 2, pdl, tmA, tmB, tmC, C, p);
+    e = sk_launch(kernel, grid, TN_THREADS, smem, cs, 2, pdl, maps, tmC, C, p);
     return e == cudaSuccess ? SK_OK : sk_set_cuda_error(e);
   }
 
