@@ -77,7 +77,8 @@ struct SkParams {
   int bm;                  // rows of the UMMA M side a tile covers (tile pitch): 128, or fewer when the
                            //    weight tile is fitted to the SM count (rows beyond it hold stale data)
   int prefetch_steps;      // K steps whose boxes the producers ask L2 for before the pipeline is up
-  int c_tma;               // 1: whole tiles leave through shared memory and TMA stores (tensor map of C given)
+  int c_tma;               // 1: whole tiles leave through shared memory and TMA stores (tensor map of C given);
+                           // 2: likewise, and C is larger than L2, which evicts it first (sk_c_streams)
   int wide_units;          // CTA-pair kernel: 256 x 512 units walked whole after the schedule's tiles
   int wide_lag;            //    K steps the second half of a unit stays behind the first
   int kpair;               // 1: a stage is the K steps of one scale group (W4A16): two, or one at an odd
@@ -331,6 +332,11 @@ inline sk_problem sk_i8_problem(const sk_problem* p) {
   q.flags |= SK_FLAG_INTERNAL_I8 | SK_FLAG_NO_TABLE;
   return q;
 }
+// A result that L2 (126 MB) cannot keep for its reader is written so that it is evicted first: the
+// write-backs then come in the order of the stores, and what is read more than once stays.  For short
+// sums, up to 16 steps, which the stores bound (int8 8192 x 28672 x 256: 137 -> 104 us, 9472 x 8192 x
+// 512: 43.2 -> 42.6; gradients in sk_grouped.cu); long ones lose 1 % by it (fp16 8192 x 28672 x 8192).
+inline bool sk_c_streams(double bytes, long long steps) { return bytes > 126e6 && steps <= 16; }
 void sk_resolve_auto(sk_problem* q, int kernel_kind, int num_sms);
 // What the fp16 entry point runs for a problem: SK_SCHED_AUTO resolved, the fused gather's
 // link-bound rule applied (n_peers > 0), and the kernel chosen: *kernel_kind = 1 (single-CTA

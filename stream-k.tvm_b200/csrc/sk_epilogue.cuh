@@ -533,7 +533,8 @@ __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtens
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      tma_store_2d(tmC, buf, gcol0 + g * 64, grow0);
+      if (I8 && p.c_tma == 2) tma_store_2d_evict_first(tmC, buf, gcol0 + g * 64, grow0);
+      else tma_store_2d(tmC, buf, gcol0 + g * 64, grow0);
       if (peers != nullptr)   // the same box into every peer's matrix, in the same bulk group
         for (int i = 0; i < peers->n; ++i) tma_store_2d(&peers->tm[i], buf, gcol0 + g * 64, grow0);
       tma_store_commit();

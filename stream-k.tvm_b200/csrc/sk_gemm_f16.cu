@@ -555,7 +555,7 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
   const int split = p.sched.split;   // SK_SCHED_CLUSTER: CTAs per tile
   // Whole tiles of a row-major C leave through shared memory and TMA stores (not the
   // transposed store of the swapped order, not the cluster schedule's reduction).
-  p.c_tma = (!plan.swap && !split && p.c_vec_ok) ? 1 : 0;
+  p.c_tma = !plan.swap && !split && p.c_vec_ok ? (i8 && sk_c_streams(2.0 * M * N, K / 64) ? 2 : 1) : 0;
   // (8-bit integers: whole tiles are staged for rows that TMA cannot address, too)
   const bool stage_c = p.c_tma || (i8 && !plan.swap && !split);
   const int recv_bytes = split ? sk_cluster_recv_bytes(plan.bn, split) : stage_c ? 512 + SK_CSTAGE_BYTES + (i8 ? 512 : 0) : 0;   // (i8: 128 bytes per epilogue warp, SkScales)

@@ -501,7 +501,8 @@ int sk_launch_f16_2cta(const sk_problem* prob, const void* A, const void* B, voi
             : sk_make_tmap_f16(&tmB, B, prob->N, prob->K, prob->ldb, BK, bn / 2);
   CUtensorMap tmC;
   memset(&tmC, 0, sizeof(tmC));
-  p->c_tma = p->c_vec_ok;   // whole tiles leave through shared memory and TMA stores
+  // whole tiles leave through shared memory and TMA stores
+  p->c_tma = p->c_vec_ok ? (k_i8 > 0 && sk_c_streams(2.0 * prob->M * prob->N, prob->K / 64) ? 2 : 1) : 0;
   if (n_blocks) p->c_tma = 0;
   if (st == SK_OK && p->c_tma) st = sk_make_tmap_f16(&tmC, C, prob->M, prob->N, prob->ldc, 64, 32);
   if (st != SK_OK) return st;

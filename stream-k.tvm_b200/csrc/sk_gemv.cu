@@ -11,7 +11,7 @@
 // its kernels are tiled for the tensor cores at every M (streamk_fp16.py:143-371,
 // streamk_fp16_ladder_block_reduce_q4.py:143-522).
 //
-// Three kernels:
+// Four kernels:
 //   fp16 / bf16 weights [N, K] row-major, M <= 4 (CUDA cores).  CTA (g, s) walks K range s of
 //     the 128 rows of group g; a warp takes 16 rows, eight at a time; its 32 lanes read 512
 //     contiguous bytes of one row per instruction (8 K values each), the activations of the
@@ -26,6 +26,8 @@
 //     per scale group.
 //   W4A16 with scale groups of 128 and more, M <= 16 (register-level tensor-core instructions
 //     on nibbles read as fp16 subnormals; described at the kernel).
+//   8-bit integers [N, K] row-major with a scale per row, M <= 16 (the same instructions on
+//     integers, exact sums; described at the kernel).
 #include "sk_common.cuh"
 
 namespace {
@@ -643,6 +645,10 @@ sk_gemv_q4_mma_kernel(const uint16_t* __restrict__ A, int lda, int M, const uint
 // activations' pieces (row g8 of A) straight from global memory through L1, where every CTA of
 // the SM finds the same few KB.  Piece c of row r sits at c ^ 4 (r & 1), so that the eight lanes of
 // a quarter-warp, two rows of four pieces, read different banks.
+//
+// Bound: the stream of the weights, behind two to three microseconds of launch and first loads
+// (1 x 28672 x 8192: 42.7 us, 5.5 TB/s; 1 x 11008 x 4096: 10.1 us, of which the stream takes 6.9).  The
+// tensor-memory kernels take 14.4 us for the latter.
 __device__ __forceinline__ void mma_16832_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                              uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "

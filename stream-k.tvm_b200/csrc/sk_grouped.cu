@@ -33,7 +33,7 @@
 // of up to 16 or 32 rows loads only as many (60 groups of 5 rows, 1408 x 2048: 80 us with 64 loaded
 // and zeroed piece by piece, 64 now).  Long sums are
 // bound like the other two (16384 rows, 8 x 11008 x 4096: 0.98 ms), short ones by the writing of C
-// (32 groups of 128 rows, 4096 x 2048 in fp32: 202 us, 5.3 TB/s; zeros alone 5.9).
+// (32 groups of 128 rows, 4096 x 2048 in fp32: 199 us, 5.4 TB/s; zeros alone 6.0).
 #include "sk_common.cuh"
 #include "sk_epilogue.cuh"
 
@@ -70,6 +70,7 @@ struct GroupedParams {
   int c_vec_ok, c_words;     // rows of C can take 16-byte stores; 4-byte stores
   int c_tma;                 // TN: C leaves through TMA stores
   int c_flat;                // TN: and every C[e] is one piece of memory
+  int c_stream;              // TN: C is larger than L2, and leaves it first
   uint32_t idesc;            // with N = 0
   unsigned long long timeout_ns;
   SkWorkspace ws;
@@ -851,7 +852,9 @@ sk_grouped_sum_kernel(const __grid_constant__ SumMaps maps, const __grid_constan
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          tma_store_3d(&tmC, buf_smem, tile.c0 + c, r0, tile.e);   // clipped at the edges of C[e]
+          // (clipped at the edges of C[e])
+          if (p.c_stream) tma_store_3d_evict_first(&tmC, buf_smem, tile.c0 + c, r0, tile.e);
+          else tma_store_3d(&tmC, buf_smem, tile.c0 + c, r0, tile.e);
           tma_store_commit();
         }
         return;
@@ -1131,6 +1134,9 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
     const int esz = f32 ? 4 : 2;
     p.c_tma = aligned(C, 16) && (p.ldc * esz) % 16 == 0 && (p.stride_c * esz) % 16 == 0;
     p.c_flat = p.c_tma && p.ldc == g->N;
+    // (24 groups of 42 rows, 4096 x 2048, bf16: 81 -> 70 us; 60 of 5, 1408 x 2048: 64 -> 58; over eight
+    // results in turn)
+    p.c_stream = sk_c_streams(static_cast<double>(g->E) * g->K * g->N * esz, g->T / BK / g->E);
     p.idesc = umma_idesc_f16(2 * HALF_M, 0, 1, bf16) | (1u << 15);   // both operands MN-major
     SumMaps maps;
     CUtensorMap tmC;
@@ -1145,7 +1151,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
     const int fixed = 1024 + EPI_WARPS * 4096 + CTRL_BYTES + table_bytes(g->E, false);
     p.stages = (SMEM_LIMIT - fixed) / TN_STEP;
     // fp32 results of short sums are bound by their stores, which do better with less read ahead of
-    // them: four, up to 2.5 steps per group (32 groups of 128 rows, 4096 x 2048: 213 -> 202 us; with
+    // them: four, up to 2.5 steps per group (32 groups of 128 rows, 4096 x 2048: 207 -> 199 us; with
     // 190 rows 211 -> 220)
     if (f32 && 2LL * g->T <= 5LL * BK * g->E && p.stages > 4) p.stages = 4;
     const int smem = fixed + p.stages * TN_STEP;
