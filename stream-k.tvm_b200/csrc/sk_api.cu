@@ -193,7 +193,8 @@ static long long sk_i8_cluster_cap(int size, int num_sms) {
 //   256, or 256 x 192 where the waves then take a tenth less (200 x 11008 x 2048: 12.9 us against
 //   13.7; 400 x 12288 x 4096: 26.4 against 28.7).
 // Few tiles and a deep K: 128 x 64 tiles split over clusters (100 x 512 x 8192: 7.4 us against 10.9;
-// 32 tiles, K = 8192: 9.9 against 12.5; with clusters of two, or fewer steps, no gain).
+// 32 tiles, K = 8192: 9.9 against 12.5; with clusters of two, or fewer steps, no gain), or 128 x 128
+// tiles where K is deeper still (80 x 4096 x 11008: 15.4 us against 17.6; 128 rows: 16.5 and 17.7).
 // M <= 64 keeps the rules below (weights on the UMMA M side, split over clusters), but for short K
 // (48 x 512 x 512: 5.5 us against 11.5) and for more than a wave of tiles (48 x 28672 x 1024: 13.2
 // against 16.9).  False: not decided here.
@@ -211,6 +212,11 @@ static bool resolve_auto_i8(sk_problem* q, int num_sms) {
   if ((steps >= 32 && tiles(128, 64) <= sk_i8_cluster_cap(8, num_sms)) ||
       (steps >= 48 && tiles(128, 64) <= sk_i8_cluster_cap(4, num_sms))) {
     plan(128, 64);
+    q->schedule = SK_SCHED_CLUSTER;
+    return true;
+  }
+  if (steps >= 80 && tiles(128, 128) <= sk_i8_cluster_cap(4, num_sms)) {
+    plan(128, 128);
     q->schedule = SK_SCHED_CLUSTER;
     return true;
   }
