@@ -56,6 +56,7 @@ struct GroupedParams {
   long long ldc, stride_c;   // elements
   const void* offsets;
   int off64;
+  SkDiv d_rows[4];           // NT / NN: / tile_rows(bn_max, j)
   int bn_max;                // UMMA N of a tile: NT / NN: at most (rows of a group), a multiple of 32; TN: columns of N
   int tiles_f;               // tiles along the UMMA M side (NT / NN: of N; TN: of K)
   int steps;                 // NT / NN: K steps of a tile
@@ -102,97 +103,117 @@ static_assert(sizeof(Ctrl) <= CTRL_BYTES, "Ctrl must fit its reserved space");
 constexpr int SK_MAX_PARTS = 4;   // most pairs that share a tile's sum
 
 __host__ __device__ constexpr int align_up(int v, int a) { return (v + a - 1) / a * a; }
-// Group table in shared memory: start[E + 1], then (NT / NN) first[E + 1], the first row tile.
-__host__ __device__ constexpr int table_bytes(int E, bool tiles) { return align_up((tiles ? 2 : 1) * (E + 1) * 4, 16); }
+// Group table in shared memory: start[E + 1], then (NT / NN) first[E + 1], the first row tile, then
+// what make_table passes between its warps, five numbers for every 32 of the E + 1.
+__host__ __device__ constexpr int table_chunks(int E) { return (E + 32) / 32; }
+__host__ __device__ constexpr int table_bytes(int E, bool tiles) {
+  return align_up(((tiles ? 2 : 1) * (E + 1) + 5 * table_chunks(E)) * 4, 16);
+}
 
 // Rows per tile, choice j: bn_max, a half, a quarter, an eighth of it (multiples of 16, at least 32).
-__device__ __forceinline__ int tile_rows(const GroupedParams& p, int j) {
-  const int v = align_up(p.bn_max >> j, 16);
+__host__ __device__ __forceinline__ int tile_rows(int bn_max, int j) {
+  const int v = align_up(bn_max >> j, 16);
   return v < 32 ? 32 : v;
 }
 
-// Fills the table.  Called by every thread; ends with the table visible to all.
+// Fills the table.  Called by every thread; ends with the table visible to all.  A warp takes 32
+// of the E + 1 offsets at a time, and what passes from one 32 to the next (the running maximum of the
+// starts, the numbers of tiles) goes through `scratch`: with hundreds of groups and a few rows the
+// table is most of the launch (512 groups of 328 x 472, 10 rows: 31.2 us with one warp making it and
+// every role looking for its tiles group by group, 8.3 now).
 template <bool ROWS, bool SPLIT>
-__device__ __forceinline__ void make_table(const GroupedParams& p, int* start, int* first, RowPlan* plan, int units) {
-  for (int i = threadIdx.x; i <= p.E; i += blockDim.x) {
-    long long o = p.off64 ? __ldg(static_cast<const long long*>(p.offsets) + i)
-                          : static_cast<long long>(__ldg(static_cast<const int*>(p.offsets) + i));
-    bool bad = o < 0 || o > p.T;
-    o = o < 0 ? 0 : o > p.T ? p.T : o;
-    if (i > 0) {
-      const long long before = p.off64 ? __ldg(static_cast<const long long*>(p.offsets) + i - 1)
-                                       : static_cast<long long>(__ldg(static_cast<const int*>(p.offsets) + i - 1));
-      bad = bad || before > o;
+__device__ __forceinline__ void make_table(const GroupedParams& p, int* start, int* first, int* scratch, RowPlan* plan,
+                                           int units) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int chunks = table_chunks(p.E);
+  for (int c = warp; c < chunks; c += warps) {
+    const int i = c * 32 + lane;
+    int s = 0;
+    if (i <= p.E) {
+      long long o = p.off64 ? __ldg(static_cast<const long long*>(p.offsets) + i)
+                            : static_cast<long long>(__ldg(static_cast<const int*>(p.offsets) + i));
+      bool bad = o < 0 || o > p.T;
+      o = o < 0 ? 0 : o > p.T ? p.T : o;
+      if (i > 0) {
+        const long long before = p.off64 ? __ldg(static_cast<const long long*>(p.offsets) + i - 1)
+                                         : static_cast<long long>(__ldg(static_cast<const int*>(p.offsets) + i - 1));
+        bad = bad || before > o;
+      }
+      s = static_cast<int>(o);
+      if (bad && blockIdx.x == 0) sk_report(p.ws.status, SK_ERR_ARG, static_cast<uint32_t>(i), 0u);
     }
-    start[i] = static_cast<int>(o);
-    if (bad && blockIdx.x == 0) sk_report(p.ws.status, SK_ERR_ARG, static_cast<uint32_t>(i), 0u);
+    __syncwarp();
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d && o > s) s = o;
+    }
+    if (i <= p.E) start[i] = s;
+    if (lane == 31) scratch[c] = s;
   }
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    // running maximum of the starts; tiles if a tile takes bn_max, bn_max / 2, / 4, / 8 rows
-    int top = 0, count[4] = {0, 0, 0, 0};
-    for (int base = 0; base <= p.E; base += 32) {
-      const int i = base + lane;
-      int s = i <= p.E ? start[i] : 0;
+  for (int c = warp; c < chunks; c += warps) {
+    const int i = c * 32 + lane;
+    const int top = __reduce_max_sync(0xffffffffu, lane < c ? scratch[lane] : 0);   // (at most 33 chunks)
+    int s = i <= p.E ? start[i] : 0;
+    if (s < top) s = top;
+    int before = __shfl_up_sync(0xffffffffu, s, 1);
+    if (lane == 0) before = top;
+    if (i <= p.E) start[i] = s;
+#pragma unroll
+    for (int j = 0; ROWS && j < 4; ++j) {   // tiles if a tile takes bn_max, bn_max / 2, / 4, / 8 rows
+      const int n = i > 0 && i <= p.E ? sk_div(s - before + tile_rows(p.bn_max, j) - 1, p.d_rows[j]) : 0;
+      const int all = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0) scratch[(1 + j) * chunks + c] = all;
+    }
+  }
+  __syncthreads();
+  if constexpr (ROWS) {
+    // Too few tiles for the pairs: fewer rows per tile, as long as every tile gets a pair of its
+    // own (a step of 64 rows takes little more than half the time of one of 256).
+    int bn = 0, total = 0;
+    SkDiv d_bn = p.d_rows[0];
+    const int* counts = scratch;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int* mine = scratch + (1 + j) * chunks;
+      const int count = __reduce_add_sync(0xffffffffu, (lane < chunks ? mine[lane] : 0) + (lane == 0 && chunks > 32 ? mine[32] : 0));
+      if (j == 0 || static_cast<long long>(count) * p.tiles_f <= units) {
+        bn = tile_rows(p.bn_max, j);
+        total = count * p.tiles_f;
+        d_bn = p.d_rows[j];
+        counts = mine;
+      }
+    }
+    for (int c = warp; c < chunks; c += warps) {
+      const int i = c * 32 + lane;
+      const int earlier = __reduce_add_sync(0xffffffffu, lane < c ? counts[lane] : 0);
+      // tiles of group i - 1; first[i] = tiles of groups 0 .. i - 1
+      int t = i > 0 && i <= p.E ? sk_div(start[i] - start[i - 1] + bn - 1, d_bn) : 0;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, s, d);
-        if (lane >= d && o > s) s = o;
+        const int o = __shfl_up_sync(0xffffffffu, t, d);
+        if (lane >= d) t += o;
       }
-      if (s < top) s = top;
-      int before = __shfl_up_sync(0xffffffffu, s, 1);
-      if (lane == 0) before = top;
-      if (i <= p.E) start[i] = s;
-      top = __shfl_sync(0xffffffffu, s, 31);
-#pragma unroll
-      for (int j = 0; ROWS && j < 4; ++j) count[j] += i > 0 && i <= p.E ? (s - before + tile_rows(p, j) - 1) / tile_rows(p, j) : 0;
+      if (i <= p.E) first[i] = earlier + t;
     }
-    if constexpr (ROWS) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) count[j] = __reduce_add_sync(0xffffffffu, count[j]);
-      // Too few tiles for the pairs: fewer rows per tile, as long as every tile gets a pair of its
-      // own (a step of 64 rows takes little more than half the time of one of 256).
-      int bn = tile_rows(p, 0), total = count[0] * p.tiles_f;
-#pragma unroll
-      for (int j = 1; j < 4; ++j)
-        if (static_cast<long long>(count[j]) * p.tiles_f <= units) {
-          bn = tile_rows(p, j);
-          total = count[j] * p.tiles_f;
-        }
-      __syncwarp();
-      int sum = 0;
-      for (int base = 0; base <= p.E; base += 32) {
-        const int i = base + lane;
-        // tiles of group i - 1; first[i] = tiles of groups 0 .. i - 1
-        int t = i > 0 && i <= p.E ? (start[i] - start[i - 1] + bn - 1) / bn : 0;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int o = __shfl_up_sync(0xffffffffu, t, d);
-          if (lane >= d) t += o;
-        }
-        t += sum;
-        if (i <= p.E) first[i] = t;
-        sum = __shfl_sync(0xffffffffu, t, 31);
+    if (threadIdx.x == 0) {
+      // Still no more tiles than half of the pairs, and long sums: split each over up to four
+      // pairs, whose parts the last of them to finish adds (a part read back costs about 0.5 us
+      // for 64 rows, so more pairs per tile would gain nothing).
+      RowPlan q;
+      q.total = total; q.sk = 0; q.runs = 1; q.f = 0; q.r = 0;
+      if (SPLIT && total > 0 && 2 * total <= units) {
+        q.sk = total;
+        q.runs = units / total < SK_MAX_PARTS ? units / total * total : SK_MAX_PARTS * total;
+        const int S = q.sk * p.steps;
+        q.f = S / q.runs;
+        q.r = S - q.f * q.runs;
       }
-      if (lane == 0) {
-        // Still no more tiles than half of the pairs, and long sums: split each over up to four
-        // pairs, whose parts the last of them to finish adds (a part read back costs about 0.5 us
-        // for 64 rows, so more pairs per tile would gain nothing).
-        RowPlan q;
-        q.total = total; q.sk = 0; q.runs = 1; q.f = 0; q.r = 0;
-        if (SPLIT && total > 0 && 2 * total <= units) {
-          q.sk = total;
-          q.runs = units / total < SK_MAX_PARTS ? units / total * total : SK_MAX_PARTS * total;
-          const int S = q.sk * p.steps;
-          q.f = S / q.runs;
-          q.r = S - q.f * q.runs;
-        }
-        *plan = q;
-      }
+      *plan = q;
     }
+    __syncthreads();
   }
-  __syncthreads();
 }
 
 // ------------------------------------------------------------------------------- NT and NN
@@ -239,7 +260,17 @@ struct RowWalk {
       o.k1 = p.steps;
       t += units;
     }
-    while (first[e + 1] * p.tiles_f <= o.tile) ++e;
+    if (first[e + 1] * p.tiles_f <= o.tile) {   // (whole warps walk: 32 groups at a look)
+      for (const int lane = threadIdx.x & 31;; e += 32) {
+        if (e >= p.E) return false;               // (not reached: o.tile < first[E] * tiles_f)
+        const int i = e + 1 + lane < p.E ? e + 1 + lane : p.E;
+        const unsigned past = __ballot_sync(0xffffffffu, first[i] * p.tiles_f > o.tile);
+        if (past != 0u) {
+          e += __ffs(past) - 1;
+          break;
+        }
+      }
+    }
     const int mt = first[e + 1] - first[e];
     int local = o.tile - first[e] * p.tiles_f;
     const int band = local / (8 * p.tiles_f);
@@ -315,7 +346,7 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
     tmem_relinquish_pair();
   }
   griddep_wait();
-  make_table<true, SPLIT>(p, start, first, &ctrl->plan, units);
+  make_table<true, SPLIT>(p, start, first, first + p.E + 1, &ctrl->plan, units);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -677,7 +708,7 @@ sk_grouped_sum_kernel(const __grid_constant__ SumMaps maps, const __grid_constan
     tmem_relinquish_pair();
   }
   griddep_wait();
-  make_table<false, false>(p, start, nullptr, nullptr, units);
+  make_table<false, false>(p, start, nullptr, start + p.E + 1, nullptr, units);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -1147,7 +1178,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
     }
     if (st == SK_OK && p.c_tma) st = make_map(&tmC, C, f32, g->E, g->K, g->N, p.ldc, p.stride_c, f32 ? 32 : 64, 32);
     if (st != SK_OK) return st;
-    // Stages: as many as fit, six for up to 383 groups, five above.
+    // Stages: as many as fit, six for up to 328 groups, five above.
     const int fixed = 1024 + EPI_WARPS * 4096 + CTRL_BYTES + table_bytes(g->E, false);
     p.stages = (SMEM_LIMIT - fixed) / TN_STEP;
     // fp32 results of short sums are bound by their stores, which do better with less read ahead of
@@ -1166,6 +1197,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
 
   const int t32 = g->T < MAX_BN ? (g->T + 31) & ~31 : MAX_BN;
   p.bn_max = t32;
+  for (int j = 0; j < 4; ++j) p.d_rows[j] = sk_div_make(tile_rows(p.bn_max, j));
   p.tiles_f = (g->N + 255) / 256;
   // (row tiles: at most one ragged one per group besides the full ones)
   if ((static_cast<long long>(g->T) / p.bn_max + g->E + 1) * p.tiles_f > (1LL << 30)) return SK_ERR_LIMIT;
