@@ -101,9 +101,9 @@ struct SkScales {
 };
 __device__ __forceinline__ SkScales sk_fetch_scales(const SkParams& p, int grow, int gcol) {
   SkScales s;
-  s.row = grow < p.rows ? __ldg(p.row_scale + grow) : 0.f;
-  s.c0 = gcol < p.cols ? __ldg(p.col_scale + gcol) : 0.f;
-  s.c1 = gcol + 32 < p.cols ? __ldg(p.col_scale + gcol + 32) : 0.f;
+  s.row = grow < p.rows ? p.row_scale[grow] : 0.f;
+  s.c0 = gcol < p.cols ? p.col_scale[gcol] : 0.f;
+  s.c1 = gcol + 32 < p.cols ? p.col_scale[gcol + 32] : 0.f;
   return s;
 }
 
@@ -113,9 +113,9 @@ __device__ __forceinline__ void sk_store_cols(__half* __restrict__ C, const SkPa
                                               int gcol0, int nv, const float (&in)[NC]) {
   float v[NC];
   if constexpr (I8) {
-    const float rs = __ldg(p.row_scale + grow);
+    const float rs = p.row_scale[grow];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) v[j] = j < nv ? sk_scaled(p, in[j], rs, __ldg(p.col_scale + gcol0 + j)) : 0.f;
+    for (int j = 0; j < NC; ++j) v[j] = j < nv ? sk_scaled(p, in[j], rs, p.col_scale[gcol0 + j]) : 0.f;
   } else {
 #pragma unroll
     for (int j = 0; j < NC; ++j) v[j] = in[j];
@@ -156,10 +156,10 @@ __device__ __forceinline__ void sk_store4(__half* __restrict__ C, const SkParams
                                           const float4& x) {
   float v[4] = {x.x, x.y, x.z, x.w};
   if constexpr (I8) {
-    const float rs = __ldg(p.row_scale + grow);
+    const float rs = p.row_scale[grow];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      v[e] = gcol + e < p.cols ? sk_scaled(p, v[e], rs, __ldg(p.col_scale + gcol + e)) : 0.f;
+      v[e] = gcol + e < p.cols ? sk_scaled(p, v[e], rs, p.col_scale[gcol + e]) : 0.f;
   }
   if (p.transposed) {
 #pragma unroll

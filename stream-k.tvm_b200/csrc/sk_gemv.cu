@@ -35,9 +35,11 @@ namespace {
 constexpr int GEMV_THREADS_F16 = 256;
 constexpr int GEMV_THREADS_Q4 = 32 * SK_GEMV_Q4_WARPS;   // at most
 
+// (Ordinary loads here and below, and no `const __restrict__` on what they read, which would let the
+// compiler take the read-only path: see skptx::griddep_wait.)
 __device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
@@ -96,7 +98,7 @@ __device__ __forceinline__ void finish_group(const float* sums /* shared: [M][ro
                                              int S, int bf16, int tid, int nthreads, uint32_t* s_last,
                                              const float* scale_a = nullptr, const float* scale_b = nullptr) {
   auto result = [&](float sum, int m, int n) {
-    if constexpr (I8) sum = (__int2float_rn(__float_as_int(sum)) * __ldg(scale_a + m)) * __ldg(scale_b + n);
+    if constexpr (I8) sum = (__int2float_rn(__float_as_int(sum)) * scale_a[m]) * scale_b[n];
     return static_cast<uint16_t>(pack_out(sum, bf16));
   };
   const int row0 = g * rows, items = M * rows;
@@ -142,9 +144,8 @@ __device__ __forceinline__ void finish_group(const float* sums /* shared: [M][ro
 // ------------------------------------------------------------------------------------- fp16
 template <int M, bool BF16>
 __global__ void __launch_bounds__(GEMV_THREADS_F16, M == 1 ? 4 : 1)
-sk_gemv_f16_kernel(const uint16_t* __restrict__ A, int lda, const uint16_t* __restrict__ B, int ldb,
-                   uint16_t* __restrict__ C, int ldc, int N, int K, int k_per_split, int S, float* parts,
-                   uint32_t* counters) {
+sk_gemv_f16_kernel(const uint16_t* A, int lda, const uint16_t* B, int ldb, uint16_t* __restrict__ C, int ldc, int N,
+                   int K, int k_per_split, int S, float* parts, uint32_t* counters) {
   extern __shared__ __align__(16) float sA[];   // [M][k_per_split]
   __shared__ float sums[M * SK_GEMV_ROWS];
   __shared__ uint32_t s_last;
@@ -355,8 +356,8 @@ __device__ __forceinline__ void q4_step(Q4Sum<M>& t, const uint4 (&w)[Q4_UNR][2]
 // slices' sums meet in shared memory and are added in slice order.
 template <int M>
 __global__ void __launch_bounds__(GEMV_THREADS_Q4)
-sk_gemv_q4_kernel(const uint16_t* __restrict__ A, int lda, const uint8_t* __restrict__ qblocks,
-                  const uint8_t* __restrict__ szblocks, uint16_t* __restrict__ C, int ldc, int N, int K,
+sk_gemv_q4_kernel(const uint16_t* A, int lda, const uint8_t* qblocks, const uint8_t* szblocks,
+                  uint16_t* __restrict__ C, int ldc, int N, int K,
                   int kblocks, int kb_per_split, int kb_per_slice, int S, int gshift, int q_groups,
                   float* parts, uint32_t* counters) {
   extern __shared__ __align__(16) uint16_t sAh[];   // [warp][M][kb_per_slice * 64]
@@ -447,7 +448,7 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
 
 __device__ __forceinline__ uint4 ld_cached_v4(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 
@@ -482,8 +483,8 @@ __device__ __forceinline__ uint4 lds_v4(uint32_t addr) {
 // the activations.  ring_s: the warp's ring (shared-memory address); on return it is free again.
 // NT: column tiles of the instruction (8 rows of activations each): M <= 8 NT.
 template <int NT>
-__device__ __forceinline__ void q4m_segment(float (&acc)[NT][4][2], const uint16_t* __restrict__ A, int lda, int M,
-                                            const uint8_t* __restrict__ qblocks, const uint8_t* __restrict__ szblocks,
+__device__ __forceinline__ void q4m_segment(float (&acc)[NT][4][2], const uint16_t* A, int lda, int M,
+                                            const uint8_t* qblocks, const uint8_t* szblocks,
                                             int kblocks, int gshift, int q_groups, int row0, int kb_lo, int nsteps,
                                             uint32_t ring_s, int lane) {
   const int g8 = lane >> 2, t = lane & 3;
@@ -584,8 +585,8 @@ __device__ __forceinline__ void q4m_segment(float (&acc)[NT][4][2], const uint16
 // CTA (g, s): 32 weight rows, one K slice per warp (the split of the CUDA-core W4A16 kernel).
 template <int NT>
 __global__ void __launch_bounds__(GEMV_THREADS_Q4)
-sk_gemv_q4_mma_kernel(const uint16_t* __restrict__ A, int lda, int M, const uint8_t* __restrict__ qblocks,
-                      const uint8_t* __restrict__ szblocks, uint16_t* __restrict__ C, int ldc, int N, int K,
+sk_gemv_q4_mma_kernel(const uint16_t* A, int lda, int M, const uint8_t* qblocks, const uint8_t* szblocks,
+                      uint16_t* __restrict__ C, int ldc, int N, int K,
                       int kblocks, int kb_per_split, int kb_per_slice, int S, int gshift, int q_groups,
                       float* parts, uint32_t* counters) {
   extern __shared__ __align__(16) uint8_t ring[];    // [warp][Q4M_DEPTH][Q4M_SLOT], then red and sums
@@ -663,9 +664,8 @@ __device__ __forceinline__ void cp_async_16z(uint32_t dst, const void* src, int 
 
 template <int NT>   // column tiles (eight rows of A each)
 __global__ void __launch_bounds__(GEMV_THREADS_Q4)
-sk_gemv_i8_kernel(const int8_t* __restrict__ A, int lda, int M, const int8_t* __restrict__ B, int ldb,
-                  const float* __restrict__ scale_a, const float* __restrict__ scale_b, uint16_t* __restrict__ C, int ldc,
-                  int N, int K, int steps, int per_split, int S, int bf16, float* parts, uint32_t* counters) {
+sk_gemv_i8_kernel(const int8_t* A, int lda, int M, const int8_t* B, int ldb, const float* scale_a, const float* scale_b,
+                  uint16_t* __restrict__ C, int ldc, int N, int K, int steps, int per_split, int S, int bf16, float* parts, uint32_t* counters) {
   constexpr int DEPTH = SK_GEMV_I8_DEPTH, STEP = SK_GEMV_I8_STEP_BYTES;
   extern __shared__ __align__(128) uint8_t ring[];   // [warp][DEPTH][32 rows][128]; then red and sums
   __shared__ uint32_t s_last;

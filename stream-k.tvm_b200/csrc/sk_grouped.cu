@@ -130,13 +130,13 @@ __device__ __forceinline__ void make_table(const GroupedParams& p, int* start, i
     const int i = c * 32 + lane;
     int s = 0;
     if (i <= p.E) {
-      long long o = p.off64 ? __ldg(static_cast<const long long*>(p.offsets) + i)
-                            : static_cast<long long>(__ldg(static_cast<const int*>(p.offsets) + i));
+      long long o = p.off64 ? static_cast<const long long*>(p.offsets)[i]
+                            : static_cast<long long>(static_cast<const int*>(p.offsets)[i]);
       bool bad = o < 0 || o > p.T;
       o = o < 0 ? 0 : o > p.T ? p.T : o;
       if (i > 0) {
-        const long long before = p.off64 ? __ldg(static_cast<const long long*>(p.offsets) + i - 1)
-                                         : static_cast<long long>(__ldg(static_cast<const int*>(p.offsets) + i - 1));
+        const long long before = p.off64 ? static_cast<const long long*>(p.offsets)[i - 1]
+                                         : static_cast<long long>(static_cast<const int*>(p.offsets)[i - 1]);
         bad = bad || before > o;
       }
       s = static_cast<int>(o);

@@ -463,6 +463,9 @@ __device__ __forceinline__ uint32_t atom_add_acqrel_u32(uint32_t* p, uint32_t v)
 // Programmatic dependent launch (no-ops unless the kernel was launched with the attribute):
 // let the next kernel of the stream begin its start-up / wait until the previous kernel of
 // the stream has completed and its memory is visible.
+// What that kernel may have written is read by ordinary loads: it was still being written while this
+// kernel was resident, and ld.global.nc (__ldg, and what the compiler makes of loads through `const
+// __restrict__` parameters) is for memory that nobody writes as long as the kernel lives.
 __device__ __forceinline__ void griddep_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

@@ -30,12 +30,13 @@
 
 namespace {
 
-// 8 consecutive elements of a row, as packed pairs.  VEC: the rows allow 16-byte loads.
+// 8 consecutive elements of a row, as packed pairs.  VEC: the rows allow 16-byte loads.  (Ordinary loads,
+// and X is not `const __restrict__`: see skptx::griddep_wait.)
 template <bool VEC>
 __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int K) {
   if (VEC && k + 8 <= K) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "l"(row + k));
     return v;
@@ -43,7 +44,7 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int K) {
   uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    if (k + j < K) w[j >> 1] |= static_cast<uint32_t>(__ldg(row + k + j)) << (16 * (j & 1));
+    if (k + j < K) w[j >> 1] |= static_cast<uint32_t>(row[k + j]) << (16 * (j & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -129,8 +130,7 @@ __device__ __forceinline__ uint2 quantize8(const uint4& v, const RowScale& s) {
 // from L2).
 template <bool BF16, bool VEC, int G, int NV>
 __global__ void __launch_bounds__(G < 128 ? 128 : G, G == 256 ? 5 : 1)
-sk_quantize_i8_kernel(const uint16_t* __restrict__ X, int M, int K, int ldx, int8_t* __restrict__ Q, int ldq,
-                      float* __restrict__ scale) {
+sk_quantize_i8_kernel(const uint16_t* X, int M, int K, int ldx, int8_t* __restrict__ Q, int ldq, float* __restrict__ scale) {
   constexpr int THREADS = G < 128 ? 128 : G;
   constexpr int WARPS = THREADS / 32;
   __shared__ uint32_t part[WARPS];

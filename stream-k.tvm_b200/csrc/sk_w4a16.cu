@@ -107,8 +107,8 @@ constexpr int SK_MODE_CLUSTER = 3;
 
 template <int MODE>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-sk_gemm_w4a16_kernel(const __grid_constant__ CUtensorMap tmA, const uint8_t* __restrict__ qblocks,
-                     const uint8_t* __restrict__ szblocks, __half* __restrict__ C, const SkParams p) {
+sk_gemm_w4a16_kernel(const __grid_constant__ CUtensorMap tmA, const uint8_t* qblocks, const uint8_t* szblocks,
+                     __half* __restrict__ C, const SkParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
