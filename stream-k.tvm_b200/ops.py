@@ -222,6 +222,8 @@ def _problem(M, N, K, lda, ldb, ldc, layout, schedule, fixup, o: dict) -> L.SkPr
         raise ValueError(f"schedule must be one of {sorted(L.SCHEDULES)}, got {schedule!r}")
     if fixup not in L.FIXUPS:
         raise ValueError(f"fixup must be one of {sorted(L.FIXUPS)}, got {fixup!r}")
+    if max(M, N, K, lda, ldb, ldc) > 0x7fffffff:   # (ctypes would take them modulo 2^32)
+        _check_int32(M=M, N=N, K=K, pitch_a=lda, pitch_b=ldb, pitch_out=ldc)
     # (positional: the fields of sk_problem in order; half the time of keywords)
     return L.SkProblem(M, N, K, lda, ldb, ldc, L.LAYOUTS[layout], L.SCHEDULES[schedule], L.FIXUPS[fixup],
                        int(o["tile_m"] or 0), int(o["tile_n"] or 0), int(o["num_sms"] or 0), int(o["group_m"] or 0),
@@ -542,6 +544,7 @@ def ladder_prepack(B: torch.Tensor) -> LadderWeight:
     _check_matrix("B", B, HALF_TYPES)
     B = _rowmajor(B)
     N, K = B.shape
+    _check_int32(N=N, K=K, pitch=B.stride(0))
     lib = L.load()
     nbytes = int(lib.sk_ladder_bytes(N, K))
     out = torch.empty(nbytes, dtype=torch.uint8, device=B.device)
