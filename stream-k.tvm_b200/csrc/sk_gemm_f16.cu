@@ -108,10 +108,7 @@ sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_const
   const int lane = threadIdx.x & 31;
   const int pid = blockIdx.x;
   const SkSched& s = p.sched;
-  if (threadIdx.x == 0) {
-    sk_trace(p, 0);
-    griddep_launch_dependents();   // the next kernel of the stream may begin its own start-up
-  }
+  if (threadIdx.x == 0) sk_trace(p, 0);
   // Split-K inside a cluster: the partial tiles meet in a receive buffer behind the control block.
   const uint32_t recv_base = smem_u32(ctrl) + CTRL_BYTES;
 
@@ -180,6 +177,7 @@ sk_gemm_f16_kernel(const __grid_constant__ CUtensorMap tmRow, const __grid_const
     if (warp == 1) {
       tmem_alloc(smem_u32(&ctrl->tmem_base), p.tmem_cols);
       tmem_relinquish();
+      if (lane == 0) griddep_launch_dependents();   // the next kernel of the stream may begin its own start-up
     }
     tc_fence_before();
     named_bar_sync(BAR_CONSUMERS, NUM_THREADS - 64);   // warps 1..5 and 7

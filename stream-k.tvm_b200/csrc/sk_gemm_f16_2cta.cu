@@ -105,10 +105,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   const int rank = static_cast<int>(cluster_ctarank());   // 0 = leader of the pair
   const int unit = blockIdx.x >> 1;                        // the pair's index in the schedule
   const SkSched& s = p.sched;
-  if (threadIdx.x == 0) {
-    sk_trace(p, 0);
-    griddep_launch_dependents();   // the next kernel of the stream may begin its own start-up
-  }
+  if (threadIdx.x == 0) sk_trace(p, 0);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
@@ -137,6 +134,7 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(&ctrl->tmem_base), TMEM_COLS);
     tmem_relinquish_pair();
+    if (lane == 0) griddep_launch_dependents();   // the next kernel of the stream may begin its own start-up
   }
   tc_fence_before();
   __syncthreads();

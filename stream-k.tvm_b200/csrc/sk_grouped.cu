@@ -324,7 +324,6 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
   const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    griddep_launch_dependents();
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(smem_u32(&ctrl->full[i]), 1);
       mbar_init(smem_u32(&ctrl->empty[i]), 1);
@@ -344,6 +343,7 @@ sk_grouped_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(&ctrl->tmem_base), TMEM_COLS);
     tmem_relinquish_pair();
+    if (lane == 0) griddep_launch_dependents();   // the next kernel of the stream may begin its own start-up
   }
   griddep_wait();
   make_table<true, SPLIT>(p, start, first, first + p.E + 1, &ctrl->plan, units);
@@ -683,7 +683,6 @@ sk_grouped_sum_kernel(const __grid_constant__ SumMaps maps, const __grid_constan
   const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    griddep_launch_dependents();
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(smem_u32(&ctrl->full[i]), 1);
       mbar_init(smem_u32(&ctrl->empty[i]), 1);
@@ -706,6 +705,7 @@ sk_grouped_sum_kernel(const __grid_constant__ SumMaps maps, const __grid_constan
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(&ctrl->tmem_base), TMEM_COLS);
     tmem_relinquish_pair();
+    if (lane == 0) griddep_launch_dependents();   // the next kernel of the stream may begin its own start-up
   }
   griddep_wait();
   make_table<false, false>(p, start, nullptr, start + p.E + 1, nullptr, units);

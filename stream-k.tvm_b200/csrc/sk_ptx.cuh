@@ -463,6 +463,10 @@ __device__ __forceinline__ uint32_t atom_add_acqrel_u32(uint32_t* p, uint32_t v)
 // Programmatic dependent launch (no-ops unless the kernel was launched with the attribute):
 // let the next kernel of the stream begin its start-up / wait until the previous kernel of
 // the stream has completed and its memory is visible.
+// A kernel with tensor memory lets the next one in only when its own CTAs have theirs: the next one's
+// CTAs would otherwise take the columns, hold them while they wait for this kernel to complete, and
+// tcgen05.alloc here would wait for them without end, wherever both fit on an SM.  (As it is, no two fit
+// by their shared memory, 119 KB and more each of an SM's 228; nothing else keeps them apart.)
 // What that kernel may have written is read by ordinary loads: it was still being written while this
 // kernel was resident, and ld.global.nc (__ldg, and what the compiler makes of loads through `const
 // __restrict__` parameters) is for memory that nobody writes as long as the kernel lives.

@@ -140,10 +140,7 @@ sk_gemm_w4a16_kernel(const __grid_constant__ CUtensorMap tmA, const uint8_t* qbl
   const SkSched& s = p.sched;
   const int kblocks = s.iters_per_tile;  // K / 64
   const int groups = p.q_groups;         // group blocks per 128-row block: K / group size, or 1
-  if (threadIdx.x == 0) {
-    sk_trace(p, 0);
-    griddep_launch_dependents();   // the next kernel of the stream may begin its own start-up
-  }
+  if (threadIdx.x == 0) sk_trace(p, 0);
   // Split-K inside a cluster (sk_epilogue.cuh): receive buffer behind the control block,
   // staging area in the load ring, which is idle by then.
   const uint32_t recv_base = smem_u32(ctrl) + CTRL_BYTES;
@@ -212,6 +209,7 @@ sk_gemm_w4a16_kernel(const __grid_constant__ CUtensorMap tmA, const uint8_t* qbl
     if (warp == 1) {
       tmem_alloc(smem_u32(&ctrl->tmem_base), TMEM_COLS);
       tmem_relinquish();
+      if (lane == 0) griddep_launch_dependents();   // the next kernel of the stream may begin its own start-up
     }
     tc_fence_before();
     named_bar_sync(BAR_CONSUMERS, NUM_THREADS - 32);

@@ -42,3 +42,20 @@ def test_no_read_only_loads_of_what_a_predecessor_writes(name):
     for signature, body in _kernels(text):
         if "griddep_wait()" in body:
             assert not re.search(r"const\s+[\w:]+\s*\*\s*__restrict__", signature), signature.strip()[:80]
+
+
+@pytest.mark.parametrize("name", [f for f in WAITING if "tmem_alloc" in _source(f)])
+def test_the_next_kernel_is_let_in_after_the_tensor_memory_is_allocated(name):
+    """Let in before, the next kernel's CTAs could take the columns and wait for this kernel, whose
+    allocation would wait for them."""
+    found = 0
+    for _, body in _kernels(_source(name)):
+        alloc = [m.end() for m in re.finditer(r"\btmem_alloc(_pair)?\(", body)]
+        let_in = [m.start() for m in re.finditer(r"griddep_launch_dependents\(", body)]
+        if not alloc:
+            continue
+        found += 1
+        assert len(alloc) == 1 and len(let_in) == 1 and let_in[0] > alloc[0]
+        # in the allocating warp's own block, behind the instruction, so in its program order
+        assert "}" not in body[alloc[0]:let_in[0]]
+    assert found > 0
