@@ -120,6 +120,9 @@ enum { SK_FLAG_PDL = 1, /* fp16 / W4A16 entry points: launch with programmatic s
        /* sk_gemm_grouped: offsets are int64 (int32 without); TN: C is fp32; NT / NN: rows of C that
           belong to no group are set to zero (left as they are without).                         */
        SK_FLAG_OFFSETS_64 = 0x1000, SK_FLAG_OUT_F32 = 0x2000, SK_FLAG_ZERO_REST = 0x4000,
+       /* sk_gemm_i8, sk_gemm_grouped: errors go to the device's own status word (sk_device_status)
+          instead of the workspace's: for calls that are recorded into a graph.                  */
+       SK_FLAG_DEVICE_STATUS = 0x8000,
        SK_FLAG_NO_TABLE = 2 /* SK_SCHED_AUTO: resolve by the built-in rules only, without
                           consulting the table of tuned shapes (what the offline tuner itself
                           uses to time the rules' choice).                                 */ };
@@ -213,6 +216,14 @@ int sk_stream_capture_id(void* stream, unsigned long long* id);
 /* Asynchronously copies the 16-byte status word into host_out (pinned memory
  * recommended); valid after the stream is synchronised.                      */
 int sk_poll_status(const void* ws, sk_status* host_out, void* stream);
+/* A status word of the current device that belongs to no workspace, in device memory that lives as
+ * long as the library: where calls with SK_FLAG_DEVICE_STATUS report.  A recorded call's workspace is
+ * often the graph's, zeroed at the start of every replay and reused for something else by the
+ * graph's memory pool; an error of a replay that was reported there would be lost.  One word for all
+ * of them: the first error stays until it is cleared.  sk_poll_status reads it and sk_workspace_init
+ * over SK_DEVICE_STATUS_BYTES clears it like a workspace's.                                       */
+enum { SK_DEVICE_STATUS_BYTES = 256 };
+int sk_device_status(void** status);
 
 /* ---- GEMM entry points --------------------------------------------------- */
 /* C[M,N] = A[M,K] . B, fp32 in / fp32 accumulate / fp32 out, CUDA-core FFMA

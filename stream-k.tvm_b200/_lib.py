@@ -21,7 +21,8 @@ FIXUPS = {"atomic": 0, "block_reduce": 1}
 SK_FLAG_PDL = 1
 SK_FLAG_NO_TABLE = 2
 SK_FLAG_BF16 = 4
-SK_FLAG_OFFSETS_64, SK_FLAG_OUT_F32, SK_FLAG_ZERO_REST = 0x1000, 0x2000, 0x4000
+SK_FLAG_OFFSETS_64, SK_FLAG_OUT_F32, SK_FLAG_ZERO_REST, SK_FLAG_DEVICE_STATUS = 0x1000, 0x2000, 0x4000, 0x8000
+SK_DEVICE_STATUS_BYTES = 256
 GROUPED_KINDS = {"nt": 0, "nn": 1, "tn": 2}
 SK_FLAG_Q4_GROUP = {128: 0, 32: 0x100, 64: 0x200, 0: 0x300}   # group size -> sk_problem.flags bits (0 = per-channel)
 
@@ -77,6 +78,7 @@ SIGNATURES = {
     "sk_workspace_init": (C.c_int, [_P, C.c_size_t, _P]),
     "sk_workspace_header_bytes": (C.c_size_t, [C.c_int]),
     "sk_stream_capture_id": (C.c_int, [_P, C.POINTER(C.c_ulonglong)]),
+    "sk_device_status": (C.c_int, [C.POINTER(_P)]),
     "sk_poll_status": (C.c_int, [_P, C.POINTER(SkStatus), _P]),
     "sk_gemm_f32": (C.c_int, [C.POINTER(SkProblem), _P, _P, _P, _P, C.c_size_t, _P]),
     "sk_gemm_f32_noalloc": (C.c_int, [C.POINTER(SkProblem), _P, _P, _P, C.POINTER(SkStatus), _P]),

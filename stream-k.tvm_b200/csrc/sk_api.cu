@@ -618,6 +618,41 @@ extern "C" int sk_stream_capture_id(void* stream, unsigned long long* id) {
   return SK_OK;
 }
 
+// (aligned and sized like the header of a workspace, whose place it takes in the calls that read and clear it)
+__device__ __align__(256) uint32_t g_device_status[SK_DEVICE_STATUS_BYTES / 4];
+
+extern "C" int sk_device_status(void** status) {
+  static std::atomic<void*> cached[64];   // per device; racing first calls store the same value
+  if (!status) return SK_ERR_ARG;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return sk_set_cuda_error(e);
+  if (dev < 0 || dev >= 64) return SK_ERR_ARG;
+  void* p = cached[dev].load(std::memory_order_relaxed);
+  if (p == nullptr) {
+    // (asked for while a graph is being captured, perhaps, and the address may load the module)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return sk_set_cuda_error(e);
+    e = cudaGetSymbolAddress(&p, g_device_status);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) e = back;
+    if (e != cudaSuccess) return sk_set_cuda_error(e);
+    cached[dev].store(p, std::memory_order_relaxed);
+  }
+  *status = p;
+  return SK_OK;
+}
+
+// Where a call reports: the workspace's status word, or with SK_FLAG_DEVICE_STATUS the device's.
+int sk_choose_status(int flags, SkWorkspace* ws) {
+  if ((flags & SK_FLAG_DEVICE_STATUS) == 0) return SK_OK;
+  void* p = nullptr;
+  const int st = sk_device_status(&p);
+  if (st == SK_OK) ws->status = static_cast<uint32_t*>(p);
+  return st;
+}
+
 extern "C" int sk_poll_status(const void* ws, sk_status* host_out, void* stream) {
   if (!ws || !host_out) return SK_ERR_ARG;
   cudaError_t e = cudaMemcpyAsync(host_out, ws, sizeof(sk_status), cudaMemcpyDeviceToHost,

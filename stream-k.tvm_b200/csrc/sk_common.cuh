@@ -316,6 +316,7 @@ struct SkPlan {
 int sk_set_cuda_error(cudaError_t e);
 int sk_set_driver_error(int cu_result);   // a CUresult of the driver API; reported negated
 int sk_resolve_grid(const sk_problem* p, int* num_sms_out, int* device_sms_out);
+int sk_choose_status(int flags, SkWorkspace* ws);   // SK_FLAG_DEVICE_STATUS
 // kernel_kind 0: fp32 SIMT (64x64x16 tiles); 1: fp16 UMMA; 2: W4A16 UMMA.
 int sk_make_sched(const sk_problem* p, int kernel_kind, int num_sms, sk_schedule_info* info,
                   SkSched* s, SkPlan* plan);

@@ -540,6 +540,8 @@ static int gemm_f16(const sk_problem* prob, const void* A, const void* B, void* 
   p.ws = sk_ws_carve(ws, dev_sms);  // layout fixed per device, whatever the grid
   p.trace = sk_trace_buffer();
   if (i8) {
+    const int chosen = sk_choose_status(prob->flags, &p.ws);
+    if (chosen != SK_OK) return chosen;
     p.row_scale = plan.swap ? scale_b : scale_a;
     p.col_scale = plan.swap ? scale_a : scale_b;
   }

@@ -1116,6 +1116,8 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
   p.zero_rest = (g->flags & SK_FLAG_ZERO_REST) ? 1 : 0;
   p.timeout_ns = (g->timeout_us > 0 ? static_cast<unsigned long long>(g->timeout_us) : 2000000ULL) * 1000ULL;
   p.ws = sk_ws_carve(ws, dev_sms);
+  st = sk_choose_status(g->flags, &p.ws);
+  if (st != SK_OK) return st;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const bool pdl = (g->flags & SK_FLAG_PDL) != 0;
   const uint64_t ldb = static_cast<uint64_t>(g->ldb), stride_b = g->E > 1 ? static_cast<uint64_t>(g->stride_b) : ldb * b_rows;

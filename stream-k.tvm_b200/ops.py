@@ -45,7 +45,7 @@ class _Workspace:
         self.nbytes = int(lib.sk_workspace_bytes(sms))
         self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
         self.ptr = self.buf.data_ptr()
-        self.status_host = torch.zeros(4, dtype=torch.int32).pin_memory()
+        self.status_host = torch.zeros(8, dtype=torch.int32).pin_memory()   # this workspace's, the device's
         L.check(lib.sk_workspace_init(self.buf.data_ptr(), self.nbytes, stream_ptr),
                 "sk_workspace_init")
 
@@ -111,13 +111,13 @@ def _workspace(device: torch.device) -> _Workspace:
 # the same time), allocated while capturing and therefore in the graph's memory pool, whose
 # counters a node of the graph zeroes at the start of every replay.  They are held until another
 # capture begins or a call is made outside one; from then on they belong to the graph like any
-# tensor that its capture made and let go.  (Errors that a replayed kernel reports stay in
-# them: check_status() sees those of eager calls.)
+# tensor that its capture made and let go.  Errors of a replay are therefore not reported in them
+# but in the device's own status word (SK_FLAG_DEVICE_STATUS), which check_status() reads too.
 _capture_ws: dict[int, tuple[int, dict[int, torch.Tensor]]] = {}     # device -> capture id, stream -> workspace
 
 
-def _call_workspace(device: torch.device) -> tuple[int, int]:
-    """Address and size of the workspace of a call that may be captured."""
+def _call_workspace(device: torch.device) -> tuple[int, int, int]:
+    """Workspace of a call that may be captured: its address, its size, the flags that go with it."""
     stream = _stream_ptr(device)
     lib = L.load()
     cid = C.c_ulonglong(0)
@@ -125,7 +125,7 @@ def _call_workspace(device: torch.device) -> tuple[int, int]:
     if cid.value == 0:
         _capture_ws.pop(device.index, None)
         ws = _workspace(device)
-        return ws.ptr, ws.nbytes
+        return ws.ptr, ws.nbytes, 0
     held = _capture_ws.get(device.index)
     if held is None or held[0] != cid.value:
         held = _capture_ws[device.index] = (cid.value, {})
@@ -135,7 +135,7 @@ def _call_workspace(device: torch.device) -> tuple[int, int]:
         buf = torch.empty(int(lib.sk_workspace_bytes(sms)), dtype=torch.uint8, device=device)
         L.check(lib.sk_workspace_init(buf.data_ptr(), int(lib.sk_workspace_header_bytes(sms)), stream), "sk_workspace_init")
         held[1][stream] = buf
-    return buf.data_ptr(), buf.numel()
+    return buf.data_ptr(), buf.numel(), L.SK_FLAG_DEVICE_STATUS
 
 
 def reset_workspace(device=None) -> None:
@@ -169,18 +169,29 @@ def release_cached_memory() -> None:
 
 
 def check_status(device=None) -> None:
-    """Synchronise the current stream and raise if a kernel reported a timeout."""
+    """Synchronise the current stream and raise if a kernel reported an error: one of this stream's,
+    or one of a call of the 8-bit integer or grouped products that was captured into a graph (whatever
+    stream replayed it; the replays of other streams may not have finished)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     ws = _workspace(device)
     lib = L.load()
     with torch.cuda.device(device):
-        st = C.cast(ws.status_host.data_ptr(), C.POINTER(L.SkStatus))
-        L.check(lib.sk_poll_status(ws.buf.data_ptr(), st, _stream_ptr(device)), "sk_poll_status")
+        captured = C.c_void_p()
+        L.check(lib.sk_device_status(C.byref(captured)), "sk_device_status")
+        for i, status in enumerate((ws.ptr, captured)):
+            st = C.cast(ws.status_host.data_ptr() + 16 * i, C.POINTER(L.SkStatus))
+            L.check(lib.sk_poll_status(status, st, _stream_ptr(device)), "sk_poll_status")
         torch.cuda.current_stream(device).synchronize()
-    code, cta, d0, d1 = (int(x) & 0xFFFFFFFF for x in ws.status_host.tolist())
+    words = [int(x) & 0xFFFFFFFF for x in ws.status_host.tolist()]
+    where, (code, cta, d0, d1) = "device status", words[:4]
     if code != L.SK_OK:
         reset_workspace(device)
-        raise StreamKError(code, "device status", f"[cta {cta}, detail {d0}, {d1}]")
+    elif words[4] != L.SK_OK:     # (with both, this one is left for the next check)
+        where, (code, cta, d0, d1) = "device status of a captured call", words[4:]
+        with torch.cuda.device(device):
+            L.check(lib.sk_workspace_init(captured, L.SK_DEVICE_STATUS_BYTES, _stream_ptr(device)), "sk_workspace_init")
+    if code != L.SK_OK:
+        raise StreamKError(code, where, f"[cta {cta}, detail {d0}, {d1}]")
 
 
 def device_info(device: int = 0) -> dict:
@@ -760,7 +771,8 @@ def streamk_int8_nt(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, sca
         B, ldb = _rows16(B)
         Cout = _out(o["out"], M, N, out_dtype, device)
         prob = _problem(M, N, K, lda, ldb, Cout.stride(0), "nt", schedule, "block_reduce", o)
-        ws, ws_bytes = _call_workspace(device)
+        ws, ws_bytes, ws_flags = _call_workspace(device)
+        prob.flags |= ws_flags
         L.check(L.load().sk_gemm_i8(C.byref(prob), A.data_ptr(), B.data_ptr(), scale_a.data_ptr(), scale_b.data_ptr(),
                                     Cout.data_ptr(), ws, ws_bytes, _stream_ptr(device)), "sk_gemm_i8")
     return Cout
@@ -839,7 +851,8 @@ def _grouped(kind, A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl):
         bs, cs = B.stride(), Cout.stride()
         prob = L.SkGroupedProblem(L.GROUPED_KINDS[kind], T, E, N, K, num_sms or 0, timeout_us or 0, flags,
                                   A.stride(0), bs[-2], cs[-2], 0 if kind == "tn" else bs[0], cs[0] if kind == "tn" else 0)
-        ws, ws_bytes = _call_workspace(device)
+        ws, ws_bytes, ws_flags = _call_workspace(device)
+        prob.flags |= ws_flags
         L.check(L.load().sk_gemm_grouped(C.byref(prob), A.data_ptr(), B.data_ptr(), offsets.data_ptr(), Cout.data_ptr(),
                                          ws, ws_bytes, _stream_ptr(device)), "sk_gemm_grouped")
     return Cout
