@@ -7,7 +7,7 @@
 // options -- in about a third of the time, and return None for anything else: the caller then
 // takes the Python path, which knows how to help or what to raise.  They hold no state but the
 // addresses of the C functions and of the workspaces that the Python layer registers (one per
-// device and stream, as there).
+// device and stream, as there), and on which devices that layer holds workspaces of a capture.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <map>
+#include <set>
 #include <utility>
 
 #include "../../../include/streamk_b200.h"
@@ -34,6 +35,7 @@ GemmI8Fn g_gemm_i8 = nullptr;
 GroupedFn g_grouped = nullptr;
 struct Workspace { void* ptr; size_t bytes; };
 std::map<std::pair<int, void*>, Workspace> g_workspaces;   // (device, stream); under the GIL
+std::set<int> g_captured;   // devices with workspaces of a capture to be let go; under the GIL
 
 // A plain CUDA tensor (torch.Tensor or Parameter), or null.
 const at::Tensor* cuda_tensor(PyObject* o) {
@@ -59,9 +61,10 @@ at::Tensor empty(at::IntArrayRef sizes, at::IntArrayRef strides, at::ScalarType 
 bool half_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 
 // The workspace of an eager call; null while the stream captures (a graph has one of its own, which
-// the Python path makes).
+// the Python path makes) and for the first call behind a capture (the Python path lets go of that).
 const Workspace* workspace(int device, void* stream) {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return nullptr;
+  if (g_captured.count(device) != 0) return nullptr;
   const auto it = g_workspaces.find({device, stream});
   return it == g_workspaces.end() ? nullptr : &it->second;
 }
@@ -221,8 +224,19 @@ PyObject* set_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// set_captured(device, held)
+PyObject* set_captured(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2) { PyErr_SetString(PyExc_TypeError, "set_captured takes a device and a truth value"); return nullptr; }
+  const long device = PyLong_AsLong(args[0]);
+  if (PyErr_Occurred()) return nullptr;
+  if (args[1] == Py_True) g_captured.insert(static_cast<int>(device));
+  else g_captured.erase(static_cast<int>(device));
+  Py_RETURN_NONE;
+}
+
 PyObject* clear_workspaces(PyObject*, PyObject* const*, Py_ssize_t) {
   g_workspaces.clear();
+  g_captured.clear();
   Py_RETURN_NONE;
 }
 
@@ -232,6 +246,7 @@ PyMethodDef kMethods[] = {
     {"grouped", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&guarded<grouped>)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&bind)), METH_FASTCALL, nullptr},
     {"set_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&set_workspace)), METH_FASTCALL, nullptr},
+    {"set_captured", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&set_captured)), METH_FASTCALL, nullptr},
     {"clear_workspaces", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&clear_workspaces)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -88,6 +88,8 @@ def _load_fast():
     _fast = L.load_host()
     for (device, stream), ws in _workspaces.items():
         _fast.set_workspace(device, stream, ws.ptr, ws.nbytes)
+    for device in _capture_ws:
+        _fast.set_captured(device, True)
     return _fast
 
 
@@ -110,7 +112,7 @@ def _workspace(device: torch.device) -> _Workspace:
 # capture gets workspaces of its own, one for each stream that it records (its branches may run at
 # the same time), allocated while capturing and therefore in the graph's memory pool, whose
 # counters a node of the graph zeroes at the start of every replay.  They are held until another
-# capture begins or a call is made outside one; from then on they belong to the graph like any
+# capture begins or one of these products is called outside one; from then on they belong to the graph like any
 # tensor that its capture made and let go.  Errors of a replay are therefore not reported in them
 # but in the device's own status word (SK_FLAG_DEVICE_STATUS), which check_status() reads too.
 _capture_ws: dict[int, tuple[int, dict[int, torch.Tensor]]] = {}     # device -> capture id, stream -> workspace
@@ -123,12 +125,15 @@ def _call_workspace(device: torch.device) -> tuple[int, int, int]:
     cid = C.c_ulonglong(0)
     L.check(lib.sk_stream_capture_id(stream, C.byref(cid)), "sk_stream_capture_id")
     if cid.value == 0:
-        _capture_ws.pop(device.index, None)
+        if _capture_ws.pop(device.index, None) is not None and _fast is not None:
+            _fast.set_captured(device.index, False)
         ws = _workspace(device)
         return ws.ptr, ws.nbytes, 0
     held = _capture_ws.get(device.index)
     if held is None or held[0] != cid.value:
         held = _capture_ws[device.index] = (cid.value, {})
+        if _fast is not None:   # (the next eager call on this device comes here, too)
+            _fast.set_captured(device.index, True)
     buf = held[1].get(stream)
     if buf is None:
         sms = torch.cuda.get_device_properties(device).multi_processor_count

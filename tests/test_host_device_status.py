@@ -13,3 +13,14 @@ def test_the_flag_is_its_own():
               *L.SK_FLAG_Q4_GROUP.values(), 1 << 30)
     assert all(L.SK_FLAG_DEVICE_STATUS & f == 0 for f in others)
     assert L.SK_DEVICE_STATUS_BYTES >= C.sizeof(L.SkStatus)
+
+
+def test_the_shortcut_is_told_of_captures():
+    m = L.load_host()
+    assert m.set_captured(63, True) is None and m.set_captured(63, False) is None and m.set_captured(63, False) is None
+    for bad in ((), (0,), ("0", True), (0, True, 1)):
+        try:
+            m.set_captured(*bad)
+        except TypeError:
+            continue
+        raise AssertionError(bad)
