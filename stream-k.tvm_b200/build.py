@@ -1,9 +1,10 @@
 """Build recipe: compiles csrc/*.cu for sm_100a into lib/libstreamk_b200.so.
 
-The library is a plain C-ABI shared object (no torch, no pybind): nvcc only.
-Objects are rebuilt when a source or header is newer than the object.  Beside it the host
-compiler makes lib/sk_torch_host.so from csrc/host/sk_torch_host.cpp, a small CPython module
-over torch's headers: the shortcut from tensors to the C ABI that ops.py takes in plain cases.
+The library is a plain C-ABI shared object (no torch, no pybind): nvcc only, and build() needs
+nothing else.  Objects are rebuilt when a source or header is newer than the object.  Beside it,
+where torch is installed, the host compiler makes lib/sk_torch_host.so from
+csrc/host/sk_torch_host.cpp (build_host()), a small CPython module over torch's headers: the
+shortcut from tensors to the C ABI that ops.py takes in plain cases.
 
 STREAMK_B200_TRACE=1 builds a second library, lib/libstreamk_b200_trace.so, compiled with
 -DSK_TRACE: its kernels record per-CTA timestamps while sk_debug_set_trace() names a buffer.
@@ -11,6 +12,7 @@ The ordinary library carries no tracing code.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -89,8 +91,19 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile (if needed) and return the path of the shared library, and where torch is installed the
+    host module as well; without torch, or if the module does not compile, the library is all."""
+    out = build_library(force, verbose)
+    if importlib.util.find_spec("torch") is not None:
+        try:
+            build_host(force, verbose)
+        except (ImportError, OSError, RuntimeError) as e:
+            sys.stderr.write(f"{os.path.basename(HOST_SRC)} was not built: {e}\n")
+    return out
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
     """Compile (if needed) and return the path of the shared library."""
-    build_host(force, verbose)
     objdir = OBJDIR + ("_trace" if trace_build() else "")
     os.makedirs(LIBDIR, exist_ok=True)
     os.makedirs(objdir, exist_ok=True)
