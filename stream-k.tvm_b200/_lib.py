@@ -147,7 +147,8 @@ _host = None
 
 def load_host():
     """The CPython module of the host fast path (csrc/host/sk_torch_host.cpp), bound to the loaded
-    library; built if missing, like the library, and an error if it cannot be loaded."""
+    library; built if missing, like the library, and an error if it cannot be loaded (which ops.py
+    turns into a warning: it can do without)."""
     global _host
     if _host is None:
         import importlib.machinery

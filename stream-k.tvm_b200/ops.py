@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import warnings
 from dataclasses import dataclass
 
 import torch
@@ -79,13 +80,29 @@ def _on(device: torch.device):
 
 # The fast path from tensors to the C ABI (csrc/host/sk_torch_host.cpp): int8_quantize,
 # streamk_int8_nt and the grouped products offer it their arguments first; it returns None where
-# there is anything to check, copy or refuse, and the code below takes over.
+# there is anything to check, copy or refuse, and the code below takes over.  Where it cannot be
+# built or loaded the code below does it all, at 11-14 us of host time a call instead of 4-5.
 _fast = None
+
+
+class _NoShortcut:
+    """Stands in for the module: takes nothing."""
+    @staticmethod
+    def _none(*args):
+        return None
+    quantize = gemm_i8 = grouped = set_workspace = clear_workspaces = set_captured = _none
 
 
 def _load_fast():
     global _fast
-    _fast = L.load_host()
+    L.load()                 # (the kernels themselves: an error if they are missing)
+    try:
+        _fast = L.load_host()
+    except (ImportError, OSError, RuntimeError) as e:
+        warnings.warn(f"calls take the longer host path: the host module could not be loaded ({e})", RuntimeWarning,
+                      stacklevel=3)
+        _fast = _NoShortcut()
+    _fast.clear_workspaces()
     for (device, stream), ws in _workspaces.items():
         _fast.set_workspace(device, stream, ws.ptr, ws.nbytes)
     for device in _capture_ws:
