@@ -155,7 +155,7 @@ def load_host():
         import importlib.util
         import torch  # noqa: F401  (its libraries have to be loaded first)
         lib = load()
-        path = _build.HOST_LIB if os.path.exists(_build.HOST_LIB) else _build.build_host()
+        path = _build.host_lib() if os.path.exists(_build.host_lib()) else _build.build_host()
         loader = importlib.machinery.ExtensionFileLoader("sk_torch_host", path)
         mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("sk_torch_host", loader))
         loader.exec_module(mod)

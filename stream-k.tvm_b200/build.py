@@ -2,7 +2,7 @@
 
 The library is a plain C-ABI shared object (no torch, no pybind): nvcc only, and build() needs
 nothing else.  Objects are rebuilt when a source or header is newer than the object.  Beside it,
-where torch is installed, the host compiler makes lib/sk_torch_host.so from
+where torch is installed, the host compiler makes lib/sk_torch_host.<torch>-<python>.so from
 csrc/host/sk_torch_host.cpp (build_host()), a small CPython module over torch's headers: the
 shortcut from tensors to the C ABI that ops.py takes in plain cases.
 
@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -27,7 +28,7 @@ OBJDIR = os.path.join(HERE, "build")
 LIBNAME = "libstreamk_b200.so"
 TRACE_LIBNAME = "libstreamk_b200_trace.so"
 HOST_SRC = os.path.join(CSRC, "host", "sk_torch_host.cpp")
-HOST_LIB = os.path.join(LIBDIR, "sk_torch_host.so")
+HOST_LIB = os.path.join(LIBDIR, "sk_torch_host.so")   # (see host_lib())
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -63,12 +64,21 @@ def _stale(target: str, deps: list[str]) -> bool:
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def host_lib() -> str:
+    """Path of the host module.  It is compiled against the insides of one torch and one Python, so its
+    name tells which: another version of either has a file of its own instead of loading this one."""
+    import torch
+    tag = re.sub(r"[^\w.+-]", "_", f"torch{torch.__version__}-{sys.implementation.cache_tag}")
+    return f"{HOST_LIB[:-len('.so')]}.{tag}.so"
+
+
 def build_host(force: bool = False, verbose: bool = False) -> str:
     """Compile (if needed) the CPython module of the host fast path and return its path."""
-    header = os.path.join(HERE, "..", "include", "streamk_b200.h")
-    if not force and not _stale(HOST_LIB, [HOST_SRC, header]):
-        return HOST_LIB
     import torch
+    header = os.path.join(HERE, "..", "include", "streamk_b200.h")
+    out = host_lib()
+    if not force and not _stale(out, [HOST_SRC, header]):
+        return out
     os.makedirs(LIBDIR, exist_ok=True)
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
@@ -80,14 +90,14 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
            *(f"-I{d}" for d in (os.path.join(root, "include"),
                                 os.path.join(root, "include", "torch", "csrc", "api", "include"),
                                 sysconfig.get_paths()["include"], os.path.join(cuda, "include"))),
-           HOST_SRC, "-o", HOST_LIB, f"-L{os.path.join(root, 'lib')}",
+           HOST_SRC, "-o", out, f"-L{os.path.join(root, 'lib')}",
            "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or r.returncode != 0:
         sys.stderr.write(f"--- {os.path.basename(HOST_SRC)}\n{r.stdout}{r.stderr}\n")
     if r.returncode != 0:
         raise RuntimeError(f"compiling {HOST_SRC} failed")
-    return HOST_LIB
+    return out
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
