@@ -64,6 +64,20 @@ def _stale(target: str, deps: list[str]) -> bool:
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def _make(cmd: list[str], out: str) -> subprocess.CompletedProcess:
+    """Runs a compiler or linker that writes `out`, under another name until it is whole: processes
+    that find it missing at the same time, or load it meanwhile, never meet half a file."""
+    part = f"{out}.{os.getpid()}.tmp"
+    try:
+        r = subprocess.run([*cmd, "-o", part], capture_output=True, text=True)
+        if r.returncode == 0:
+            os.replace(part, out)
+    finally:
+        if os.path.exists(part):
+            os.remove(part)
+    return r
+
+
 def host_lib() -> str:
     """Path of the host module.  It is compiled against the insides of one torch and one Python, so its
     name tells which: another version of either has a file of its own instead of loading this one."""
@@ -90,9 +104,9 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
            *(f"-I{d}" for d in (os.path.join(root, "include"),
                                 os.path.join(root, "include", "torch", "csrc", "api", "include"),
                                 sysconfig.get_paths()["include"], os.path.join(cuda, "include"))),
-           HOST_SRC, "-o", out, f"-L{os.path.join(root, 'lib')}",
+           HOST_SRC, f"-L{os.path.join(root, 'lib')}",
            "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    r = _make(cmd, out)
     if verbose or r.returncode != 0:
         sys.stderr.write(f"--- {os.path.basename(HOST_SRC)}\n{r.stdout}{r.stderr}\n")
     if r.returncode != 0:
@@ -133,8 +147,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
 
     def compile_one(job):
         src, obj = job
-        r = subprocess.run([*common, "-c", src, "-o", obj], capture_output=True, text=True)
-        return src, r
+        return src, _make([*common, "-c", src], obj)
 
     with ThreadPoolExecutor(max_workers=max(1, min(8, len(jobs) or 1))) as ex:
         for src, r in ex.map(compile_one, jobs):
@@ -144,8 +157,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
                 raise RuntimeError(f"nvcc failed on {src}")
     out = lib_path()
     if force or jobs or _stale(out, objs):
-        r = subprocess.run([nvcc, "-shared", *ARCH_FLAGS, "-o", out, *objs],
-                           capture_output=True, text=True)
+        r = _make([nvcc, "-shared", *ARCH_FLAGS, *objs], out)
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
