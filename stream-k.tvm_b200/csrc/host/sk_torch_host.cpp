@@ -60,14 +60,29 @@ at::Tensor empty(at::IntArrayRef sizes, at::IntArrayRef strides, at::ScalarType 
 
 bool half_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 
-// The workspace of an eager call; null while the stream captures (a graph has one of its own, which
+// The workspace of an eager call; none (a null address) while the stream captures (a graph has one of its own, which
 // the Python path makes) and for the first call behind a capture (the Python path lets go of that).
-const Workspace* workspace(int device, void* stream) {
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return nullptr;
-  if (g_captured.count(device) != 0) return nullptr;
+Workspace workspace(int device, void* stream) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return {nullptr, 0};
+  if (g_captured.count(device) != 0) return {nullptr, 0};
   const auto it = g_workspaces.find({device, stream});
-  return it == g_workspaces.end() ? nullptr : &it->second;
+  return it == g_workspaces.end() ? Workspace{nullptr, 0} : it->second;
 }
+
+// Lets other threads have the interpreter for as long as it lives: an allocation may wait for the
+// device and a launch for room in its queue, and what they wait for may need another thread of this
+// process (a callback on the host, the launch of a kernel that the queued ones wait for).  Whatever
+// belongs to Python or to the maps above is read before.
+class Unlocked {
+ public:
+  Unlocked() : state_(PyEval_SaveThread()) {}
+  ~Unlocked() { PyEval_RestoreThread(state_); }
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+
+ private:
+  PyThreadState* state_;
+};
 
 #define SK_MISS Py_RETURN_NONE
 
@@ -84,12 +99,18 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Device device = x->device();
   const c10::cuda::CUDAGuard guard(device);
   void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-  at::Tensor Q = empty({M, K}, {pitch, 1}, at::kChar, device);
-  at::Tensor scale = empty({M}, {1}, at::kFloat, device);
   const int flags = SK_FLAG_PDL | (x->scalar_type() == at::kBFloat16 ? SK_FLAG_BF16 : 0);
-  if (g_quantize(x->const_data_ptr(), static_cast<int>(M), static_cast<int>(K), static_cast<int>(ld), flags,
-                 Q.mutable_data_ptr(), static_cast<int>(pitch), static_cast<float*>(scale.mutable_data_ptr()), stream) != SK_OK)
-    SK_MISS;
+  const void* X = x->const_data_ptr();
+  at::Tensor Q, scale;
+  int status;
+  {
+    const Unlocked unlocked;
+    Q = empty({M, K}, {pitch, 1}, at::kChar, device);
+    scale = empty({M}, {1}, at::kFloat, device);
+    status = g_quantize(X, static_cast<int>(M), static_cast<int>(K), static_cast<int>(ld), flags, Q.mutable_data_ptr(),
+                        static_cast<int>(pitch), static_cast<float*>(scale.mutable_data_ptr()), stream);
+  }
+  if (status != SK_OK) SK_MISS;
   PyObject* q = THPVariable_Wrap(std::move(Q));
   PyObject* s = THPVariable_Wrap(std::move(scale));
   if (q == nullptr || s == nullptr) { Py_XDECREF(q); Py_XDECREF(s); return nullptr; }
@@ -126,16 +147,22 @@ PyObject* gemm_i8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const bool bf16 = args[4] == Py_True;
   const c10::cuda::CUDAGuard guard(device);
   void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-  const Workspace* ws = workspace(device.index(), stream);
-  if (ws == nullptr) SK_MISS;
-  at::Tensor C = empty({M, N}, {N, 1}, bf16 ? at::kBFloat16 : at::kHalf, device);
+  const Workspace ws = workspace(device.index(), stream);
+  if (ws.ptr == nullptr) SK_MISS;
   sk_problem p = {};
   p.M = static_cast<int32_t>(M); p.N = static_cast<int32_t>(N); p.K = static_cast<int32_t>(K);
   p.lda = static_cast<int32_t>(lda); p.ldb = static_cast<int32_t>(ldb); p.ldc = static_cast<int32_t>(N);
   p.layout = SK_LAYOUT_NT; p.schedule = SK_SCHED_AUTO; p.fixup = SK_FIXUP_BLOCK_REDUCE;
   p.flags = SK_FLAG_PDL | (bf16 ? SK_FLAG_BF16 : 0);
-  if (g_gemm_i8(&p, a->const_data_ptr(), b->const_data_ptr(), sa, sb, C.mutable_data_ptr(), ws->ptr, ws->bytes, stream) != SK_OK)
-    SK_MISS;
+  const void *A = a->const_data_ptr(), *B = b->const_data_ptr();
+  at::Tensor C;
+  int status;
+  {
+    const Unlocked unlocked;
+    C = empty({M, N}, {N, 1}, bf16 ? at::kBFloat16 : at::kHalf, device);
+    status = g_gemm_i8(&p, A, B, sa, sb, C.mutable_data_ptr(), ws.ptr, ws.bytes, stream);
+  }
+  if (status != SK_OK) SK_MISS;
   return THPVariable_Wrap(std::move(C));
 }
 
@@ -170,10 +197,9 @@ PyObject* grouped(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Device device = a->device();
   const c10::cuda::CUDAGuard guard(device);
   void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-  const Workspace* ws = workspace(device.index(), stream);
-  if (ws == nullptr) SK_MISS;
+  const Workspace ws = workspace(device.index(), stream);
+  if (ws.ptr == nullptr) SK_MISS;
   const at::ScalarType type = fp32 ? at::kFloat : a->scalar_type();
-  at::Tensor C = tn ? empty({E, K, N}, {K * N, N, 1}, type, device) : empty({T, N}, {N, 1}, type, device);
   sk_grouped_problem g = {};
   g.kind = static_cast<int32_t>(kind);
   g.T = static_cast<int32_t>(T); g.E = static_cast<int32_t>(E);
@@ -181,9 +207,15 @@ PyObject* grouped(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g.flags = SK_FLAG_PDL | (a->scalar_type() == at::kBFloat16 ? SK_FLAG_BF16 : 0) | (off64 ? SK_FLAG_OFFSETS_64 : 0) |
             (fp32 ? SK_FLAG_OUT_F32 : 0) | (tn ? 0 : SK_FLAG_ZERO_REST);
   g.lda = lda; g.ldb = ldb; g.ldc = N; g.stride_b = stride_b; g.stride_c = tn ? K * N : 0;
-  if (g_grouped(&g, a->const_data_ptr(), b->const_data_ptr(), off->const_data_ptr(), C.mutable_data_ptr(), ws->ptr, ws->bytes,
-                stream) != SK_OK)
-    SK_MISS;
+  const void *A = a->const_data_ptr(), *B = b->const_data_ptr(), *offsets = off->const_data_ptr();
+  at::Tensor C;
+  int status;
+  {
+    const Unlocked unlocked;
+    C = tn ? empty({E, K, N}, {K * N, N, 1}, type, device) : empty({T, N}, {N, 1}, type, device);
+    status = g_grouped(&g, A, B, offsets, C.mutable_data_ptr(), ws.ptr, ws.bytes, stream);
+  }
+  if (status != SK_OK) SK_MISS;
   return THPVariable_Wrap(std::move(C));
 }
 
