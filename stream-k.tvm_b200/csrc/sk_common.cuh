@@ -156,9 +156,10 @@ struct SkGemvPlan {
 };
 //   8-bit integers: a CTA takes 32 weight rows over all of K, its warps take steps of 128 bytes in
 //     turn, each with a ring of SK_GEMV_I8_DEPTH steps (4 KB each) in flight.  As many warps per
-//     CTA as let every CTA be resident at once, up to 16: all of the weights are then being
-//     asked for from the start, and an SM with one CTA more than another simply draws more of
-//     the bandwidth.  Few rows: K split across CTAs, at least eight steps each.
+//     CTA as let every CTA be resident at once (one of 16, two of 8 or four of 4 to an SM; with more
+//     than four, 4 as well): all of the weights are then being asked for from the start, and an SM
+//     with one CTA more than another simply draws more of the bandwidth.  Few rows: K split across
+//     CTAs, at least eight steps each.
 constexpr int SK_GEMV_I8_MAX_M = 16;
 constexpr int SK_GEMV_I8_DEPTH = 3;
 constexpr int SK_GEMV_I8_STEP_BYTES = 32 * 128;

@@ -665,9 +665,10 @@ __device__ __forceinline__ void cp_async_16z(uint32_t dst, const void* src, int 
 template <int NT>   // column tiles (eight rows of A each)
 __global__ void __launch_bounds__(GEMV_THREADS_Q4)
 sk_gemv_i8_kernel(const int8_t* A, int lda, int M, const int8_t* B, int ldb, const float* scale_a, const float* scale_b,
-                  uint16_t* __restrict__ C, int ldc, int N, int K, int steps, int per_split, int S, int bf16, float* parts, uint32_t* counters) {
+                  uint16_t* __restrict__ C, int ldc, int N, int K, int steps, int per_split, int S, int bf16, int sums_at,
+                  float* parts, uint32_t* counters) {
   constexpr int DEPTH = SK_GEMV_I8_DEPTH, STEP = SK_GEMV_I8_STEP_BYTES;
-  extern __shared__ __align__(128) uint8_t ring[];   // [warp][DEPTH][32 rows][128]; then red and sums
+  extern __shared__ __align__(128) uint8_t ring[];   // [warp][DEPTH][32 rows][128]; red and sums behind it or, at the end, in its place (sums_at)
   __shared__ uint32_t s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g8 = lane >> 2, t = lane & 3;
@@ -747,7 +748,8 @@ sk_gemv_i8_kernel(const int8_t* A, int lda, int M, const int8_t* B, int ldb, con
   }
   cp_async_wait<0>();
   skptx::griddep_launch_dependents();
-  int* red = reinterpret_cast<int*>(ring + warps * (DEPTH * STEP));    // [warp][m][row of the CTA]
+  if (sums_at == 0) __syncthreads();                                   // every warp's ring has been filled and read
+  int* red = reinterpret_cast<int*>(ring + sums_at);                   // [warp][m][row of the CTA]
   float* sums = reinterpret_cast<float*>(red + warps * M * 32);        // [m][row]
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -780,11 +782,24 @@ int sk_launch_gemv_i8(const sk_problem* prob, const void* A, const void* B, cons
     return SK_ERR_LIMIT;
   const bool pdl = (prob->flags & SK_FLAG_PDL) != 0;
   const int warps = pl.slices;
-  const size_t smem = static_cast<size_t>(warps) * SK_GEMV_I8_DEPTH * SK_GEMV_I8_STEP_BYTES +
-                      static_cast<size_t>(warps + 1) * prob->M * 32 * sizeof(int);
-  constexpr size_t smem_max = static_cast<size_t>(16) * SK_GEMV_I8_DEPTH * SK_GEMV_I8_STEP_BYTES +
-                              static_cast<size_t>(17) * SK_GEMV_I8_MAX_M * 32 * sizeof(int);
-  static_assert(smem_max + 64 <= 232448, "shared memory of the largest CTA");
+  // The warps' rings and their sums.  The plan counts on two CTAs of 8 warps to an SM, or four of 4
+  // (sk_gemv_plan_i8); an SM has 228 KB, of which a CTA takes its own, 128 bytes of static variables
+  // and 1 KB for the system.  Where the sums behind the rings would keep a CTA of the launch off
+  // its SM, they take the rings' place once those are done (16 x 8192 x 4096, two CTAs of 8 warps:
+  // 12.7 us behind, in two waves, 10.2 in place); elsewhere the barrier that this needs costs more
+  // than it gives (16 x 14208 x 4096, three of 4: 14.0 us behind, 14.8 in place).
+  constexpr auto ring_bytes = [](int n) { return static_cast<size_t>(n) * SK_GEMV_I8_DEPTH * SK_GEMV_I8_STEP_BYTES; };
+  constexpr auto sums_bytes = [](int n, int m) { return static_cast<size_t>(n + 1) * m * 32 * sizeof(int); };
+  constexpr auto per_sm = [](size_t bytes) { return static_cast<int>(233472 / (bytes + 128 + 1024)); };
+  static_assert(sums_bytes(1, SK_GEMV_I8_MAX_M) <= ring_bytes(1) && sums_bytes(16, SK_GEMV_I8_MAX_M) <= ring_bytes(16), "the sums fit the rings");
+  static_assert(per_sm(ring_bytes(16)) >= 1 && per_sm(ring_bytes(8)) >= 2 && per_sm(ring_bytes(4)) >= 4, "CTAs that an SM holds at once");
+  constexpr size_t smem_max = ring_bytes(16) + sums_bytes(16, SK_GEMV_I8_MAX_M);
+  static_assert(smem_max + 128 <= 232448, "shared memory of the largest CTA");
+  const size_t behind = ring_bytes(warps) + sums_bytes(warps, prob->M);
+  const int wanted = (pl.grid - 1) / dev_sms + 1, most = per_sm(ring_bytes(warps));
+  const bool in_place = per_sm(behind) < (wanted < most ? wanted : most);
+  const size_t smem = in_place ? ring_bytes(warps) : behind;
+  const int sums_at = in_place ? 0 : static_cast<int>(ring_bytes(warps));
   static SkPerDeviceOnce attrs;
   cudaError_t e = attrs.run([]() {
     cudaError_t r = cudaFuncSetAttribute(sk_gemv_i8_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_max);
@@ -799,7 +814,7 @@ int sk_launch_gemv_i8(const sk_problem* prob, const void* A, const void* B, cons
   auto kernel = prob->M <= 8 ? sk_gemv_i8_kernel<1> : sk_gemv_i8_kernel<2>;
   e = sk_launch(kernel, pl.grid, pl.threads, smem, cs, 1, pdl, static_cast<const int8_t*>(A), 2 * prob->lda, prob->M,
                 static_cast<const int8_t*>(B), 2 * prob->ldb, scale_a, scale_b, static_cast<uint16_t*>(C), prob->ldc,
-                prob->N, k_elems, steps, per_split, pl.splits, bf16, ws.part_slots, ws.counters);
+                prob->N, k_elems, steps, per_split, pl.splits, bf16, sums_at, ws.part_slots, ws.counters);
   return e == cudaSuccess ? SK_OK : sk_set_cuda_error(e);
 }
 
