@@ -255,7 +255,7 @@ def _problem(M, N, K, lda, ldb, ldc, layout, schedule, fixup, o: dict) -> L.SkPr
         raise ValueError(f"schedule must be one of {sorted(L.SCHEDULES)}, got {schedule!r}")
     if fixup not in L.FIXUPS:
         raise ValueError(f"fixup must be one of {sorted(L.FIXUPS)}, got {fixup!r}")
-    if max(M, N, K, lda, ldb, ldc) > 0x7fffffff:   # (ctypes would take them modulo 2^32)
+    if (M | N | K | lda | ldb | ldc) > 0x7fffffff:   # (ctypes would take them modulo 2^32)
         _check_int32(M=M, N=N, K=K, pitch_a=lda, pitch_b=ldb, pitch_out=ldc)
     # (positional: the fields of sk_problem in order; half the time of keywords)
     return L.SkProblem(M, N, K, lda, ldb, ldc, L.LAYOUTS[layout], L.SCHEDULES[schedule], L.FIXUPS[fixup],
