@@ -422,25 +422,27 @@ constexpr int SK_CSTAGE_BYTES = 4 * 2 * 4096;
 // groups g_first, g_first + g_step, ... (the warps that share a TMEM lane quadrant split the
 // columns).  NBUF: staging buffers per warp.  Returns the number of columns the warps handle
 // together (a multiple of 64; the rest of the tile goes through sk_store_chunk).
-// ROWS: C's rows are not what TMA can address (a pitch or a base off the 16-byte grid): the warp
-// stores the staged box itself, a row at a time and consecutive lanes to consecutive columns
-// (4-byte words where the rows allow them), instead of every lane walking a row of its own.
-template <int NBUF = 2, bool I8 = false, bool ROWS = false>
+// I8: where C's rows are not what TMA can address (p.c_tma is 0: a pitch or a base off the 16-byte
+// grid), the warp stores the staged box itself, a row at a time and consecutive lanes to consecutive
+// columns (4-byte words where the rows allow them), instead of every lane walking a row of its own.
+template <int NBUF = 2, bool I8 = false>
 __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtensorMap* tmC, uint32_t cstage,
                                                  int warp_slot, int lane, uint32_t t_addr, uint32_t b_off,
                                                  int grow0, int gcol0, int valid_cols, uint32_t& groups,
                                                  const SkPeers* peers = nullptr, int g_first = 0,
                                                  int g_step = 1, __half* C = nullptr, SkScales scales = SkScales{}) {
   using namespace skptx;
-  // I8: a last group that the matrix ends in goes the same way (TMA clips it; the row stores mind the
-  // edge), if the tile's own columns are whole groups.  (Through registers it cost 4 us more:
-  // 531 x 696 x 2144 12.9 -> 8.2 us.)
+  // I8: a last group that the matrix ends in goes the same way, if the tile's own columns are whole
+  // groups.  (Through registers it cost 4 us more: 531 x 696 x 2144 12.9 -> 8.2 us.)  TMA clips it, but
+  // to whole 16 bytes: where the matrix ends between, the rest of them would be overwritten with zeros,
+  // and they may be somebody's (`out` as a part of a wider buffer), so that group is stored by rows.
   const int full = I8 && (p.bn & 63) == 0 ? (valid_cols + 63) >> 6 : valid_cols >> 6;
   const uint32_t share = cstage + static_cast<uint32_t>(SK_CSTAGE_BYTES) + static_cast<uint32_t>(warp_slot) * 128u;
   for (int g = g_first; g < full; g += g_step, ++groups) {
     const uint32_t buf = cstage + static_cast<uint32_t>(warp_slot * NBUF + (NBUF == 2 ? (groups & 1u) : 0u)) * 4096u;
+    const int left = valid_cols - g * 64;      // columns of this group inside the matrix
     // the store issued from this buffer NBUF groups ago must have read it
-    if (!ROWS && lane == 0) tma_store_wait_read<NBUF - 1>();
+    if ((!I8 || p.c_tma) && lane == 0) tma_store_wait_read<NBUF - 1>();
     __syncwarp();
     // both 32-column reads of the group in flight before the one wait
     uint32_t raw[2][32];
@@ -487,12 +489,11 @@ __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtens
                      : "memory");
       }
     }
-    if constexpr (ROWS) {
+    if (I8 && (!p.c_tma || ((left & 7) != 0 && left < 64))) {
       // (eight rows read, then stored: a store between two reads would make the reads wait in line)
       __syncwarp();
       int rows = p.rows - grow0;
       if (rows > 32) rows = 32;
-      const int left = valid_cols - g * 64;      // columns of this group inside the matrix
       uint16_t* const dst = reinterpret_cast<uint16_t*>(C) + static_cast<size_t>(grow0) * p.ldc + gcol0 + g * 64;
       if ((p.ldc & 1) == 0 && (reinterpret_cast<uintptr_t>(C) & 3u) == 0) {
         for (int r0 = 0; r0 < rows; r0 += 8) {
@@ -528,6 +529,7 @@ __device__ __forceinline__ int sk_store_tile_tma(const SkParams& p, const CUtens
               if (r0 + i < rows && h * 32 + lane < left) dst[static_cast<size_t>(r0 + i) * p.ldc + h * 32 + lane] = w[i][h];
         }
       }
+      if (p.c_tma && lane == 0) tma_store_commit();   // (a group of none: the wait above counts them)
       continue;
     }
     fence_proxy_async_smem();
@@ -650,13 +652,9 @@ __device__ __forceinline__ void sk_epilogue_loop(const SkParams& p, __half* __re
     // two MMA issuers: the second one's accumulator holds every other stage of the segment
     const bool two = sk_second_acc_used(p, seg.k0, seg.k1);
     int c_first = 0;   // first 32-column chunk that still has to go through the register path
-    if (whole && p.c_tma && cstage != 0 && warp_ok && !dead)
+    if (whole && (I8 || p.c_tma) && cstage != 0 && warp_ok && !dead)
       c_first = sk_store_tile_tma<NBUF, I8>(p, tmC, cstage, warp - 2, lane, t_addr, two ? p.acc_b_off : 0,
-                                        r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB, nullptr, scales) >> 5;
-    if constexpr (I8)
-      if (whole && !p.c_tma && cstage != 0 && warp_ok && !dead)
-        c_first = sk_store_tile_tma<NBUF, I8, true>(p, tmC, cstage, warp - 2, lane, t_addr, two ? p.acc_b_off : 0,
-                                                    r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB, C, scales) >> 5;
+                                        r0 + q * 32, c0, valid_cols, tma_groups, peers, sub, NSUB, C, scales) >> 5;
     if (warp_ok && !dead) {
       for (int c = c_first + sub; c < nchunks; c += NSUB) {
         float v[32];

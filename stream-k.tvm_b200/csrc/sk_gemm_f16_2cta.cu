@@ -410,12 +410,9 @@ sk_gemm_f16_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           const uint32_t t_addr = tmem_base + buf * BN + (static_cast<uint32_t>(q * 32) << 16);
           if (warp_ok && !dead && valid_cols > 0) {
             int c_first = 0;
-            if (I8 && !p.c_tma)
-              c_first = sk_store_tile_tma<1, I8, true>(p, &tmC, cstage, warp - 2, lane, t_addr, 0, r0 + q * 32, c0,
-                                                       valid_cols, groups, peers, sub, EPI_WARPS / 4, C, scales) >> 5;
-            else if (cstage != 0)
+            if (cstage != 0)
               c_first = sk_store_tile_tma<1, I8>(p, &tmC, cstage, warp - 2, lane, t_addr, 0, r0 + q * 32, c0,
-                                             valid_cols, groups, peers, sub, EPI_WARPS / 4, nullptr, scales) >> 5;
+                                             valid_cols, groups, peers, sub, EPI_WARPS / 4, C, scales) >> 5;
             for (int c = c_first + sub; c < ((valid_cols + 31) >> 5); c += EPI_WARPS / 4) {
               float v[32];
               sk_load_acc(t_addr + c * 32, 0, v);

@@ -879,11 +879,12 @@ sk_grouped_sum_kernel(const __grid_constant__ SumMaps maps, const __grid_constan
                        : "memory");
         }
       }
-      if (p.c_tma) {
+      // (TMA clips at the edges of C[e], but columns to whole 16 bytes: where N ends between, the rest of
+      // them would be overwritten, so that group is stored by rows)
+      if (p.c_tma && (valid - c >= gcols || ((valid - c) * (F32 ? 4 : 2) & 15) == 0)) {
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          // (clipped at the edges of C[e])
           if (p.c_stream) tma_store_3d_evict_first(&tmC, buf_smem, tile.c0 + c, r0, tile.e);
           else tma_store_3d(&tmC, buf_smem, tile.c0 + c, r0, tile.e);
           tma_store_commit();
