@@ -118,7 +118,7 @@ def _workspace(device: torch.device) -> _Workspace:
     if ws is None:
         with torch.cuda.device(device):
             ws = _Workspace(device, key[1])
-        _workspaces[key] = ws
+        ws = _workspaces.setdefault(key, ws)   # (another thread may have been first: one for both, and the shortcut's)
         if _fast is not None:
             _fast.set_workspace(key[0], key[1], ws.ptr, ws.nbytes)
     return ws
