@@ -2,6 +2,7 @@
 does: a launch that waits for room in the device's queue must not keep other Python threads from
 running, since what the queue waits for may need one of them."""
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -44,3 +45,39 @@ def test_an_allocation_that_fails_takes_it_back(module):
     assert ctypes.pythonapi.PyGILState_Check() == 1
     with pytest.raises(torch.OutOfMemoryError):          # ... which says why
         sk.streamk_grouped_tn(A, A, offsets)
+
+
+@pytest.mark.parametrize("own_stream", [True, False])
+def test_calls_from_several_threads(own_stream):
+    """Each thread with a stream of its own, or all on one."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    sizes, N, K = [5, 40, 0, 200], 300, 3336                # (short ones: shared sums in the workspace)
+    A = torch.randint(-2, 3, (sum(sizes), K), generator=g, device=DEV).half()
+    W = torch.randint(-2, 3, (len(sizes), N, K), generator=g, device=DEV).half()
+    q = torch.randint(-127, 128, (7, 8192), generator=g, device=DEV, dtype=torch.int8)
+    w = torch.randint(-127, 128, (512, 8192), generator=g, device=DEV, dtype=torch.int8)
+    sa, sb = torch.rand(7, generator=g, device=DEV), torch.rand(512, generator=g, device=DEV)
+    off = torch.tensor([0, 5, 45, 45, 245], device=DEV)
+
+    def run():
+        return [sk.streamk_grouped_nt(A, W, off), sk.streamk_int8_nt(q, w, sa, sb), *sk.int8_quantize(A),
+                sk.streamk_grouped_tn(A[:, :256], A[:, :128], off)]
+    want = [r.clone() for r in run()]
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(4)
+
+    def work(stream):
+        with torch.cuda.stream(stream):
+            start.wait()
+            for _ in range(50):
+                got = run()
+                stream.synchronize()
+                wrong.extend(i for i, (a, b) in enumerate(zip(got, want)) if not torch.equal(a, b))
+    one = torch.cuda.Stream()
+    threads = [threading.Thread(target=work, args=(torch.cuda.Stream() if own_stream else one,)) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    sk.check_status()
