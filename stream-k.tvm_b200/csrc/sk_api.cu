@@ -190,14 +190,14 @@ static long long sk_i8_cluster_cap(int size, int num_sms) {
 // plan tried on all but a few.  The tile:
 //   128 x 64 while those fit on the SMs at once (the latency of one tile is all there is), then
 //   128 x 128 likewise, 128 x 256 for a single row of tiles beyond that; otherwise CTA pairs, 256 x
-//   256, or 256 x 192 where the waves then take a tenth less (200 x 11008 x 2048: 12.9 us against
-//   13.7; 400 x 12288 x 4096: 26.4 against 28.7).
-// Few tiles and a deep K: 128 x 64 tiles split over clusters (100 x 512 x 8192: 7.4 us against 10.9;
-// 32 tiles, K = 8192: 9.9 against 12.5; with clusters of two, or fewer steps, no gain), or 128 x 128
-// tiles where K is deeper still (80 x 4096 x 11008: 15.4 us against 17.6; 128 rows: 16.5 and 17.7).
+//   256, or 256 x 192 where the waves then take a tenth less (200 x 11008 x 2048: 10.3 us against
+//   11.4; 400 x 12288 x 4096: 21.5 against 24.8).
+// Few tiles and a deep K: 128 x 64 tiles split over clusters (100 x 512 x 8192: 8.6 us against 13.9;
+// 32 tiles, K = 8192: 11.0 against 13.4; with clusters of two, or fewer steps, no gain), or 128 x 128
+// tiles where K is deeper still (80 x 4096 x 11008: 15.9 us against 18.0; 128 rows: 16.9 and 18.0).
 // M <= 64 keeps the rules below (weights on the UMMA M side, split over clusters), but for short K
-// (48 x 512 x 512: 5.5 us against 11.5) and for more than a wave of tiles (48 x 28672 x 1024: 13.2
-// against 16.9).  False: not decided here.
+// (48 x 512 x 512: 3.4 us against 5.4) and for more than a wave of tiles (48 x 28672 x 1024: 11.9
+// against 14.5).  False: not decided here.
 static bool resolve_auto_i8(sk_problem* q, int num_sms) {
   const int steps = (q->K - 1) / 64 + 1;          // (K in pairs of elements)
   auto tiles = [&](int m, int n) {
@@ -250,12 +250,21 @@ void sk_resolve_auto(sk_problem* q, int kernel_kind, int num_sms) {
   const int gemv_kind = sk_gemv_kind(kernel_kind, q->flags);
   // (W4A16: 9 to 16 rows cost the small-M kernel twice the instructions of 1 to 8: only where the
   // launch is short enough to be bound by latencies, at most one 32-row CTA per SM)
-  // (8-bit integers: 9 to 16 rows take a second column tile and a second set of activations; ahead of
-  // the tensor-memory kernels, 12.4 against 13.7 us at 16 x 11008 x 4096, until the weights are
-  // many waves of CTAs: 53.6 against 44.5 at 16 x 28672 x 8192.
-  // And every CTA reads all the activations, half as many bytes as its weights at N = 4096: with a
-  // deep K the cluster schedule is ahead, 11.4 against 12.2 us at 16 x 4096 x 11008.)
-  const int gemv_m = gemv_kind == 4 ? (q->N > 96LL * num_sms || (q->N <= 32LL * num_sms && q->K > 4096) ? 8 : SK_GEMV_I8_MAX_M) : gemv_kind != 2 ? SK_GEMV_AUTO_M : (q->N <= 32LL * num_sms ? SK_GEMV_Q4_MAX_M : 8);
+  // (8-bit integers, us on 148 SMs, small-M kernel / tensor-memory kernels at M = 16:
+  //     N         1024        4096        4736        8192        11008       14208       16384       20480
+  //   K = 1024   3.1 / 5.2   4.7 / 6.1   4.9 / 6.4   5.5 / 6.7   6.2 / 6.7   6.7 / 7.2   7.5 / 7.4  11.0 / 9.2
+  //   K = 2048   6.5 / 5.8   5.3 / 6.8   5.6 / 7.2   7.2 / 7.8   8.4 / 8.4   9.1 / 9.2  10.3 / 9.4  15.6 / 11.9
+  //   K = 4096   6.8 / 6.2   7.1 / 7.7   7.6 / 8.9  10.2 / 10.3 12.3 / 11.5 13.9 / 13.0 15.2 / 14.1 24.3 / 19.5
+  //   K = 8192   7.1 / 7.3  10.4 / 10.2 11.2 / 12.4 15.9 / 14.9 20.9 / 19.5 24.5 / 22.4 26.7 / 24.3 42.2 / 35.1
+  //   K = 11008  7.8 / 8.2  12.6 / 11.7 13.4 / 15.4 19.0 / 19.4 25.5 / 23.7 28.9 / 27.5 33.3 / 30.8 53.4 / 45.1
+  // 9 to 16 rows take a second column tile and a second set of activations, so that up to 96 weight rows
+  // to an SM the two are within an eighth of one another or the small-M kernel is ahead; beyond that,
+  // with many waves of CTAs, the others are.  Every CTA reads all the activations, half as many bytes as its
+  // weights at N = 4096: up to 32 weight rows to an SM a deep K goes to the cluster schedule.  8 rows
+  // and fewer: ahead up to 64 weight rows to an SM (8 x 8192 x 4096: 9.0 / 10.3; 1 x 11008 x 4096: 10.2 /
+  // 11.5), within 5 % up to 110, behind by up to a fifth with more (8 x 28672 x 4096: 24.7 / 22.1).)
+  const int i8_m = q->N > 96LL * num_sms || (q->N <= 32LL * num_sms && q->K > 4096) ? 8 : SK_GEMV_I8_MAX_M;
+  const int gemv_m = gemv_kind == 4 ? i8_m : gemv_kind != 2 ? SK_GEMV_AUTO_M : (q->N <= 32LL * num_sms ? SK_GEMV_Q4_MAX_M : 8);
   if (tiles_open && q->M <= gemv_m && (kernel_kind == 2 || q->layout == SK_LAYOUT_NT)) {
     // Few rows of activations: the weights stream once through a kernel without the tensor-core
     // kernels' fixed costs (tensor-memory allocation, mbarrier rings, a cluster exchange or a

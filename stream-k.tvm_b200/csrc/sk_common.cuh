@@ -336,7 +336,7 @@ inline sk_problem sk_i8_problem(const sk_problem* p) {
 }
 // A result that L2 (126 MB) cannot keep for its reader is written so that it is evicted first: the
 // write-backs then come in the order of the stores, and what is read more than once stays.  For short
-// sums, up to 16 steps, which the stores bound (int8 8192 x 28672 x 256: 137 -> 104 us, 9472 x 8192 x
+// sums, up to 16 steps, which the stores bound (int8 8192 x 28672 x 256: 137 -> 102 us, 9472 x 8192 x
 // 512: 43.2 -> 42.6; gradients in sk_grouped.cu); long ones lose 1 % by it (fp16 8192 x 28672 x 8192).
 inline bool sk_c_streams(double bytes, long long steps) { return bytes > 126e6 && steps <= 16; }
 void sk_resolve_auto(sk_problem* q, int kernel_kind, int num_sms);

@@ -648,8 +648,8 @@ sk_gemv_q4_mma_kernel(const uint16_t* A, int lda, int M, const uint8_t* qblocks,
 // a quarter-warp, two rows of four pieces, read different banks.
 //
 // Bound: the stream of the weights, behind two to three microseconds of launch and first loads
-// (1 x 28672 x 8192: 42.7 us, 5.5 TB/s; 1 x 11008 x 4096: 10.1 us, of which the stream takes 6.9).  The
-// tensor-memory kernels take 14.4 us for the latter.
+// (1 x 28672 x 8192: 40-42 us, 5.7 TB/s; 1 x 11008 x 4096: 10.3 us, of which the stream takes 6.9).  The
+// tensor-memory kernels take 11.6 us for the latter.
 __device__ __forceinline__ void mma_16832_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                              uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "

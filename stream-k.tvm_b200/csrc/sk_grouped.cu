@@ -21,7 +21,7 @@
 // for it: 9472 x 8192 x 512 89 us, turned 63.)
 //
 // What bounds them.  Few rows per group: the stream of the weights (16 rows over eight groups of
-// 11008 x 4096: 112 us, 98 % of the rate of a copy).  Many rows: the tensor cores, 87 % of their
+// 11008 x 4096: 112-115 us, 96-98 % of the rate of a copy).  Many rows: the tensor cores, 89 % of their
 // cycles at 4 x 8192 x 4096 with 1000 rows each, and under a long load the power limit (16384 rows,
 // 8 x 11008 x 4096: 0.97 ms, 1.52 PFLOP/s, alone; 1.13 ms among others like it).  In between: what an
 // SM can load, 32 KB per step and CTA.
@@ -33,7 +33,7 @@
 // of up to 16 or 32 rows loads only as many (60 groups of 5 rows, 1408 x 2048: 80 us with 64 loaded
 // and zeroed piece by piece, 64 now).  Long sums are
 // bound like the other two (16384 rows, 8 x 11008 x 4096: 0.98 ms), short ones by the writing of C
-// (32 groups of 128 rows, 4096 x 2048 in fp32: 199 us, 5.4 TB/s; zeros alone 6.0).
+// (32 groups of 128 rows, 4096 x 2048 in fp32: 223 us, 4.8 TB/s; of 100 rows 202 us, 5.3; zeros alone 6.0).
 #include "sk_common.cuh"
 #include "sk_epilogue.cuh"
 
@@ -1185,8 +1185,9 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
     const int fixed = 1024 + EPI_WARPS * 4096 + CTRL_BYTES + table_bytes(g->E, false);
     p.stages = (SMEM_LIMIT - fixed) / TN_STEP;
     // fp32 results of short sums are bound by their stores, which do better with less read ahead of
-    // them: four, up to 2.5 steps per group (32 groups of 128 rows, 4096 x 2048: 207 -> 199 us; with
-    // 190 rows 211 -> 220)
+    // them, or no worse: four, up to 2.5 steps per group (32 groups of 4096 x 2048: 100 rows 207 -> 202 us,
+    // 64 and 128 rows the same within 1 %; 190 rows 211 -> 220; 32 uneven groups of 4099 rows in all, 2048 x 4096,
+    // both gradients 340 -> 338)
     if (f32 && 2LL * g->T <= 5LL * BK * g->E && p.stages > 4) p.stages = 4;
     const int smem = fixed + p.stages * TN_STEP;
     const int grid = 2 * static_cast<int>(total * p.parts < units ? total * p.parts : units);

@@ -236,7 +236,7 @@ def _options(kw: dict) -> dict:
     """Common keyword arguments of every GEMM entry point:
     tile_m / tile_n  tile extents (None = choose; tile_m < 128 puts the weights on the UMMA
                      M dimension, the short-M form), num_sms (grid bound), group_m (tile
-                     rasterisation), out (result buffer), timeout_us (bound of every device
+                     rasterisation), out (result buffer, which shares no element with the operands), timeout_us (bound of every device
                      wait), pdl (True: programmatic dependent launch, the kernel's start-up may
                      overlap the tail of the previous kernel of the stream; fp16 / W4A16),
                      no_table (True: schedule "auto" by the built-in rules only, ignoring the table
@@ -703,8 +703,8 @@ def int8_quantize(X: torch.Tensor, *, pdl: bool = True) -> tuple[torch.Tensor, t
     [N,K].  A row of zeros has scale 0; a row that holds a NaN or an infinity has scale NaN and
     Q = 0, so that products with it are NaN.  Q's row pitch is K rounded up to 16 bytes (what
     streamk_int8_nt reads without a copy).  Rows of X may be strided.  pdl: programmatic
-    dependent launch (see _options(); here on unless switched off).  No counterpart in the
-    reference."""
+    dependent launch (see _options(); here on unless switched off).  No autograd graph is recorded.
+    No counterpart in the reference."""
     if pdl:
         r = (_fast or _load_fast()).quantize(X)
         if r is not None:
@@ -762,8 +762,8 @@ def streamk_int8_nt(A: torch.Tensor, B: torch.Tensor, scale_a: torch.Tensor, sca
     32-bit integer sums, exact whatever the schedule: every schedule returns the same bits.
     C = (float(sum) * scale_a) * scale_b, then one rounding to out_dtype.  K at most 131071.
     Operands whose rows are not 16-byte aligned are copied first.  Same schedules and keyword
-    options as streamk_fp16_nt (see _options(); pdl is on unless switched off).  No counterpart
-    in the reference."""
+    options as streamk_fp16_nt (see _options(); pdl is on unless switched off).  No autograd graph is
+    recorded.  No counterpart in the reference."""
     if not kw and schedule == "auto" and out_dtype in HALF_TYPES:
         r = (_fast or _load_fast()).gemm_i8(A, B, scale_a, scale_b, out_dtype == torch.bfloat16)
         if r is not None:
@@ -886,11 +886,12 @@ def streamk_grouped_nt(A, B, offsets, *, out=None, num_sms=None, timeout_us=None
 
     The rows of A are sorted by group: group e holds rows offsets[e] .. offsets[e+1]; offsets is
     an int32 or int64 CUDA tensor of E + 1 ascending numbers (nothing is read back by the host, so
-    the call can be captured and replayed with other sizes).  Groups may be empty.  Rows before
-    offsets[0] and from offsets[E] on belong to no group: zero in a fresh result, left as they
-    are in `out`.  Offsets out of order are clamped on the device and reported by check_status().
-    Its gradients: streamk_grouped_nn(dC, B, offsets) for A, streamk_grouped_tn(dC, A, offsets)
-    for B.  Operands whose rows are not 16-byte aligned are copied first.  num_sms, timeout_us, pdl:
+    the call can be captured and replayed with other sizes).  Groups may be empty; there are at most
+    1024.  Rows before offsets[0] and from offsets[E] on belong to no group: zero in a fresh result,
+    left as they are in `out`, which shares no element with the operands.  Offsets out of order are
+    clamped on the device and reported by check_status(), those of a replay as well.
+    No autograd graph is recorded, here and in the two gradients, which are calls of their own:
+    streamk_grouped_nn(dC, B, offsets) for A, streamk_grouped_tn(dC, A, offsets) for B.  Operands whose rows are not 16-byte aligned are copied first.  num_sms, timeout_us, pdl:
     see _options() (pdl is on unless switched off).  No counterpart in the reference."""
     return _grouped("nt", A, B, offsets, out, None, num_sms, timeout_us, pdl)
 
