@@ -292,7 +292,8 @@ int sk_quantize_i8(const void* X, int M, int K, int ldx, int flags, void* Q, int
  * With Y = NT(X, W): the gradient of X is NN(dY, W), that of W is TN(dY, X).  lda, ldb, stride_b
  * (between the groups' matrices) multiples of 8 elements, A and B 16-byte aligned; any C aligned
  * to its type, any ldc >= N and stride_c >= K ldc (16-byte rows are the fast ones).  Every value
- * is one sum in a fixed order: bitwise reproducible.  What other rows hold (infinities, NaN) does
+ * is one sum in a fixed order: bitwise reproducible.  (TN into fp32: 512 rows at a time by the tensor
+ * cores, whose adders truncate, and those sums rounded to nearest.)  What other rows hold (infinities, NaN) does
  * not reach a group's results.  Offsets that descend or leave [0, T] are clamped on the device,
  * nothing is read or written out of range, and the status word reports SK_ERR_ARG (detail0: the
  * first index found).  E at most SK_GROUPED_MAX_GROUPS; T, N and K at most SK_GROUPED_MAX_ROWS;

@@ -664,7 +664,16 @@ struct alignas(64) SumMaps {
 
 constexpr int OUT_F16 = 0, OUT_BF16 = 1, OUT_F32 = 2;   // type of C
 
-template <int OUT, bool SPLIT>
+// LONG: a group may have more than SUM_RUN steps, and C is fp32.  The tensor cores' adders truncate: a sum
+// that stays in tensor memory loses half a unit in the last place with every 16 rows, always towards
+// zero, and with it the last bits that fp32 is asked for (8192 rows of normal numbers: off by 9.1e-6 in
+// the norm).  So they add up SUM_RUN steps, 512 rows, at a time, and the epilogue adds those sums in
+// registers, rounding to nearest: off by 4.8e-7 whatever the length.  It costs long sums 1-4 % (8 groups
+// of 2048 rows, 11008 x 4096: 1205 -> 1245 us; of 500 rows, 4096 x 4096, one run: 153 and 155); runs of
+// four steps are off by 2.4e-7 and cost 6 %.  (16-bit results are rounded a hundred times as coarsely.)
+constexpr int SUM_RUN = 8;
+
+template <int OUT, bool SPLIT, bool LONG>
 __global__ void __launch_bounds__(TN_THREADS, 1)
 sk_grouped_sum_kernel(const __grid_constant__ SumMaps maps, const __grid_constant__ CUtensorMap tmC,
                       void* __restrict__ Cv, const GroupedParams p) {
@@ -783,38 +792,44 @@ sk_grouped_sum_kernel(const __grid_constant__ SumMaps maps, const __grid_constan
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(p.bn_max >> 3) << 17);
       while (ok && walk.next(p, start, units, tile)) {
         if (tile.rows == 0) continue;   // (the epilogue writes zeros)
-        const uint32_t buf = nseg & 1u;
-        if (!sk_wait_bar_warp(smem_u32(&ctrl->tmem_empty[buf]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf, 1)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + buf * MAX_BN;
-        uint32_t accumulate = 0u;
-        for (int k = tile.k0; k < tile.k1; ++k) {
-          if (!sk_wait_bar_warp(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
+        for (int k = tile.k0; ok && k < tile.k1;) {
+          const int run_end = LONG && tile.k1 - k > SUM_RUN ? k + SUM_RUN : tile.k1;
+          const uint32_t buf = nseg & 1u;
+          if (!sk_wait_bar_warp(smem_u32(&ctrl->tmem_empty[buf]), ((nseg >> 1) & 1u) ^ 1u, abort_flag, p, 16 + buf, 1)) {
             ok = false;
             break;
           }
-          if (step_needs_zeros(k, tile.rows)) {
-            if (!sk_wait_bar_warp<true>(ready0 + 8u * stage, (tail_ph >> stage) & 1u, abort_flag, p, 48 + stage, 1)) {
+          tc_fence_after();
+          const uint32_t d_tmem = tmem_base + buf * MAX_BN;
+          uint32_t accumulate = 0u;
+          for (; k < run_end; ++k) {
+            if (!sk_wait_bar_warp(full0 + 8u * stage, ph, abort_flag, p, 32 + stage, 1)) {
               ok = false;
               break;
             }
-            tail_ph ^= 1u << stage;
-          }
-          tc_fence_after();
-          const uint32_t a_lo = a_lo0 + stage * (A_STEP_BYTES >> 4), b_lo = b_lo0 + stage * (TN_B_STEP >> 4);
-          const int left = tile.rows - k * BK;              // rows of the group in this step
+            if (step_needs_zeros(k, tile.rows)) {
+              if (!sk_wait_bar_warp<true>(ready0 + 8u * stage, (tail_ph >> stage) & 1u, abort_flag, p, 48 + stage, 1)) {
+                ok = false;
+                break;
+              }
+              tail_ph ^= 1u << stage;
+            }
+            tc_fence_after();
+            const uint32_t a_lo = a_lo0 + stage * (A_STEP_BYTES >> 4), b_lo = b_lo0 + stage * (TN_B_STEP >> 4);
+            const int left = tile.rows - k * BK;              // rows of the group in this step
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) {
-            if (leader && kk * 16 < left)
-              umma_f16_ss_pair(d_tmem, hi | (a_lo + kk * 128), hi | (b_lo + kk * 128), idesc, accumulate);
-            accumulate = 1u;
+            for (int kk = 0; kk < BK / 16; ++kk) {
+              if (leader && kk * 16 < left)
+                umma_f16_ss_pair(d_tmem, hi | (a_lo + kk * 128), hi | (b_lo + kk * 128), idesc, accumulate);
+              accumulate = 1u;
+            }
+            if (leader) umma_commit_pair(empty0 + 8u * stage);
+            if (++stage == STAGES) { stage = 0; ph ^= 1u; }
           }
-          if (leader) umma_commit_pair(empty0 + 8u * stage);
-          if (++stage == STAGES) { stage = 0; ph ^= 1u; }
+          if (!ok) break;
+          if (leader) umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));
+          ++nseg;
         }
-        if (!ok) break;
-        if (leader) umma_commit_pair(smem_u32(&ctrl->tmem_full[buf]));
-        ++nseg;
       }
     }
   } else if (warp == 2 + EPI_WARPS) {
@@ -929,55 +944,107 @@ sk_grouped_sum_kernel(const __grid_constant__ SumMaps maps, const __grid_constan
           base[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         continue;
       }
-      const uint32_t buf = nseg & 1u;
-      if (some) {
+      uint32_t buf = 0u;
+      auto next_sum = [&]() {   // waits for the next accumulator
+        buf = nseg & 1u;
         if (!dead) {
           const bool got = sk_wait_bar(tmem_full0 + 8u * buf, (nseg >> 1) & 1u, abort_flag, p, 24 + buf, 2);
           if (!__all_sync(0xffffffffu, got)) dead = true;
         }
         ++nseg;
         tc_fence_after();
-      }
-      const uint32_t t_addr = tmem_base + buf * MAX_BN + (static_cast<uint32_t>(q * 32) << 16);
+        return tmem_base + buf * MAX_BN + (static_cast<uint32_t>(q * 32) << 16);
+      };
+      auto hand_back = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(tmem_empty0 + 8u * buf);
+      };
       const int r0 = tile.f0 + rank * HALF_M + q * 32;      // first of this warp's 32 rows of C[e]
       int valid = p.N - tile.c0;
       if (valid > p.bn_max) valid = p.bn_max;
       const bool whole = !SPLIT || tile.parts == 1;
-      if (!dead && r0 < p.K) {
-        for (int c = sub * gcols; c < valid; c += 2 * gcols) {
-          float v[gcols / 32][32];
-          if (some) {
-            uint32_t raw[gcols / 32][32];
+      float4* const mine = reinterpret_cast<float4*>(p.ws.part_slots + static_cast<size_t>(2 * (unit * 2 + rank)) * SK_SLOT_FLOATS);
+      bool one_run = true;
+      if constexpr (LONG) {
+        static_assert(F32, "16-bit results are rounded far above this");
+        one_run = tile.k1 - tile.k0 <= SUM_RUN;
+        if (!one_run) {
+          float sum[MAX_BN / 64][1][32];
 #pragma unroll
-            for (int h = 0; h < gcols / 32; ++h) tmem_ld_32x32(t_addr + c + h * 32, raw[h]);
-            tmem_ld_wait();
+          for (int g = 0; g < MAX_BN / 64; ++g)
 #pragma unroll
-            for (int h = 0; h < gcols / 32; ++h)
+            for (int j = 0; j < 32; ++j) sum[g][0][j] = 0.f;
+          for (int k = tile.k0; k < tile.k1; k += SUM_RUN) {
+            const uint32_t t_addr = next_sum();
+            if (!dead && r0 < p.K) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[h][j] = __uint_as_float(raw[h][j]);
-          } else {
+              for (int g = 0; g < MAX_BN / 64; ++g) {
+                const int c = (2 * g + sub) * 32;
+                if (c < valid) {
 #pragma unroll
-            for (int h = 0; h < gcols / 32; ++h)
+                  for (int h = 0; h < 32; h += 16) {           // (sixteen at a time: registers)
+                    uint32_t raw[16];
+                    tmem_ld_32x16(t_addr + c + h, raw);
+                    tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[h][j] = 0.f;
+                    for (int j = 0; j < 16; ++j) sum[g][0][h + j] += __uint_as_float(raw[j]);
+                  }
+                }
+              }
+            }
+            hand_back();
           }
-          if (whole) {
-            store_group(tile, r0, c, valid, v);
-          } else {
-            float4* mine = reinterpret_cast<float4*>(p.ws.part_slots + static_cast<size_t>(2 * (unit * 2 + rank)) * SK_SLOT_FLOATS);
+          if (!dead && r0 < p.K) {
 #pragma unroll
-            for (int h = 0; h < gcols / 32; ++h)
+            for (int g = 0; g < MAX_BN / 64; ++g) {
+              const int c = (2 * g + sub) * 32;
+              if (c >= valid) break;
+              if (whole) {
+                store_group(tile, r0, c, valid, sum[g]);
+              } else {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                __stcg(mine + ((c + h * 32) / 4 + j) * HALF_M + q * 32 + lane,
-                       make_float4(v[h][4 * j], v[h][4 * j + 1], v[h][4 * j + 2], v[h][4 * j + 3]));
+                for (int j = 0; j < 8; ++j)
+                  __stcg(mine + (c / 4 + j) * HALF_M + q * 32 + lane,
+                         make_float4(sum[g][0][4 * j], sum[g][0][4 * j + 1], sum[g][0][4 * j + 2], sum[g][0][4 * j + 3]));
+              }
+            }
           }
         }
       }
-      if (some) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(tmem_empty0 + 8u * buf);
+      if (one_run) {
+        const uint32_t t_addr = some ? next_sum() : 0u;
+        if (!dead && r0 < p.K) {
+          for (int c = sub * gcols; c < valid; c += 2 * gcols) {
+            float v[gcols / 32][32];
+            if (some) {
+              uint32_t raw[gcols / 32][32];
+#pragma unroll
+              for (int h = 0; h < gcols / 32; ++h) tmem_ld_32x32(t_addr + c + h * 32, raw[h]);
+              tmem_ld_wait();
+#pragma unroll
+              for (int h = 0; h < gcols / 32; ++h)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[h][j] = __uint_as_float(raw[h][j]);
+            } else {
+#pragma unroll
+              for (int h = 0; h < gcols / 32; ++h)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[h][j] = 0.f;
+            }
+            if (whole) {
+              store_group(tile, r0, c, valid, v);
+            } else {
+#pragma unroll
+              for (int h = 0; h < gcols / 32; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  __stcg(mine + ((c + h * 32) / 4 + j) * HALF_M + q * 32 + lane,
+                         make_float4(v[h][4 * j], v[h][4 * j + 1], v[h][4 * j + 2], v[h][4 * j + 3]));
+            }
+          }
+        }
+        if (some) hand_back();
       }
       if (whole) continue;
 
@@ -1124,7 +1191,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
   const uint64_t ldb = static_cast<uint64_t>(g->ldb), stride_b = g->E > 1 ? static_cast<uint64_t>(g->stride_b) : ldb * b_rows;
   static SkPerDeviceOnce attrs;
   cudaError_t e = attrs.run([]() {
-    const void* kernels[14] = {
+    const void* kernels[15] = {
         reinterpret_cast<const void*>(sk_grouped_rows_kernel<false, false, false>),
         reinterpret_cast<const void*>(sk_grouped_rows_kernel<false, false, true>),
         reinterpret_cast<const void*>(sk_grouped_rows_kernel<false, true, false>),
@@ -1133,14 +1200,15 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
         reinterpret_cast<const void*>(sk_grouped_rows_kernel<true, false, true>),
         reinterpret_cast<const void*>(sk_grouped_rows_kernel<true, true, false>),
         reinterpret_cast<const void*>(sk_grouped_rows_kernel<true, true, true>),
-        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F16, false>),
-        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F16, true>),
-        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_BF16, false>),
-        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_BF16, true>),
-        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F32, false>),
-        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F32, true>)};
+        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F16, false, false>),
+        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F16, true, false>),
+        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_BF16, false, false>),
+        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_BF16, true, false>),
+        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F32, false, false>),
+        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F32, false, true>),
+        reinterpret_cast<const void*>(sk_grouped_sum_kernel<OUT_F32, true, true>)};
     cudaError_t r = cudaSuccess;
-    for (int i = 0; i < 14 && r == cudaSuccess; ++i)
+    for (int i = 0; i < 15 && r == cudaSuccess; ++i)
       r = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
     return r;
   });
@@ -1191,10 +1259,12 @@ extern "C" int sk_gemm_grouped(const sk_grouped_problem* g, const void* A, const
     if (f32 && 2LL * g->T <= 5LL * BK * g->E && p.stages > 4) p.stages = 4;
     const int smem = fixed + p.stages * TN_STEP;
     const int grid = 2 * static_cast<int>(total * p.parts < units ? total * p.parts : units);
-    const bool split = p.parts > 1;
-    auto kernel = f32 ? (split ? sk_grouped_sum_kernel<OUT_F32, true> : sk_grouped_sum_kernel<OUT_F32, false>)
-                  : bf16 ? (split ? sk_grouped_sum_kernel<OUT_BF16, true> : sk_grouped_sum_kernel<OUT_BF16, false>)
-                         : (split ? sk_grouped_sum_kernel<OUT_F16, true> : sk_grouped_sum_kernel<OUT_F16, false>);
+    const bool split = p.parts > 1;   // (fp32: then also long)
+    const bool lengthy = g->T > SUM_RUN * BK;
+    auto kernel = f32 ? (split ? sk_grouped_sum_kernel<OUT_F32, true, true>
+                               : lengthy ? sk_grouped_sum_kernel<OUT_F32, false, true> : sk_grouped_sum_kernel<OUT_F32, false, false>)
+                  : bf16 ? (split ? sk_grouped_sum_kernel<OUT_BF16, true, false> : sk_grouped_sum_kernel<OUT_BF16, false, false>)
+                         : (split ? sk_grouped_sum_kernel<OUT_F16, true, false> : sk_grouped_sum_kernel<OUT_F16, false, false>);
     e = sk_launch(kernel, grid, TN_THREADS, smem, cs, 2, pdl, maps, tmC, C, p);
     return e == cudaSuccess ? SK_OK : sk_set_cuda_error(e);
   }

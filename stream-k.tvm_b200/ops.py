@@ -905,6 +905,6 @@ def streamk_grouped_nn(A, B, offsets, *, out=None, num_sms=None, timeout_us=None
 def streamk_grouped_tn(A, B, offsets, *, out=None, out_dtype=None, num_sms=None, timeout_us=None, pdl=True):
     """C[e] = sum over the rows t of group e of outer(A[t], B[t]): A [T,K], B [T,N], C [E,K,N], zero
     for an empty group.  The weight gradient of streamk_grouped_nt (dB = streamk_grouped_tn(dC, A,
-    offsets)).  out_dtype: the operands' type (default) or torch.float32 (unrounded sums).
-    Offsets as in streamk_grouped_nt; rows of no group, whatever they hold, do not count."""
+    offsets)).  out_dtype: the operands' type (default) or torch.float32 (off by a few 2^-23 of the
+    sums' norm, however many rows a group has).  Offsets as in streamk_grouped_nt; rows of no group, whatever they hold, do not count."""
     return _grouped("tn", A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl)
