@@ -129,8 +129,8 @@ def _workspace(device: torch.device) -> _Workspace:
 # capture gets workspaces of its own, one for each stream that it records (its branches may run at
 # the same time), allocated while capturing and therefore in the graph's memory pool, whose
 # counters a node of the graph zeroes at the start of every replay.  They are held until another
-# capture begins or one of these products is called outside one; from then on they belong to the graph like any
-# tensor that its capture made and let go.  Errors of a replay are therefore not reported in them
+# capture begins or one of these products is called outside one; from then on they belong to the
+# graph like any tensor that its capture made and let go.  Errors of a replay are therefore not reported in them
 # but in the device's own status word (SK_FLAG_DEVICE_STATUS), which check_status() reads too.
 _capture_ws: dict[int, tuple[int, dict[int, torch.Tensor]]] = {}     # device -> capture id, stream -> workspace
 
@@ -236,7 +236,8 @@ def _options(kw: dict) -> dict:
     """Common keyword arguments of every GEMM entry point:
     tile_m / tile_n  tile extents (None = choose; tile_m < 128 puts the weights on the UMMA
                      M dimension, the short-M form), num_sms (grid bound), group_m (tile
-                     rasterisation), out (result buffer, which shares no element with the operands), timeout_us (bound of every device
+                     rasterisation), out (result buffer, which shares no element with the operands),
+                     timeout_us (bound of every device
                      wait), pdl (True: programmatic dependent launch, the kernel's start-up may
                      overlap the tail of the previous kernel of the stream; fp16 / W4A16),
                      no_table (True: schedule "auto" by the built-in rules only, ignoring the table
@@ -891,8 +892,8 @@ def streamk_grouped_nt(A, B, offsets, *, out=None, num_sms=None, timeout_us=None
     left as they are in `out`, which shares no element with the operands.  Offsets out of order are
     clamped on the device and reported by check_status(), those of a replay as well.
     No autograd graph is recorded, here and in the two gradients, which are calls of their own:
-    streamk_grouped_nn(dC, B, offsets) for A, streamk_grouped_tn(dC, A, offsets) for B.  Operands whose rows are not 16-byte aligned are copied first.  num_sms, timeout_us, pdl:
-    see _options() (pdl is on unless switched off).  No counterpart in the reference."""
+    streamk_grouped_nn(dC, B, offsets) for A, streamk_grouped_tn(dC, A, offsets) for B.  Operands whose
+    rows are not 16-byte aligned are copied first.  num_sms, timeout_us, pdl: see _options() (pdl is on unless switched off).  No counterpart in the reference."""
     return _grouped("nt", A, B, offsets, out, None, num_sms, timeout_us, pdl)
 
 
@@ -906,5 +907,6 @@ def streamk_grouped_tn(A, B, offsets, *, out=None, out_dtype=None, num_sms=None,
     """C[e] = sum over the rows t of group e of outer(A[t], B[t]): A [T,K], B [T,N], C [E,K,N], zero
     for an empty group.  The weight gradient of streamk_grouped_nt (dB = streamk_grouped_tn(dC, A,
     offsets)).  out_dtype: the operands' type (default) or torch.float32 (off by a few 2^-23 of the
-    sums' norm, however many rows a group has).  Offsets as in streamk_grouped_nt; rows of no group, whatever they hold, do not count."""
+    sums' norm, however many rows a group has).  Offsets as in streamk_grouped_nt; rows of no group,
+    whatever they hold, do not count."""
     return _grouped("tn", A, B, offsets, out, out_dtype, num_sms, timeout_us, pdl)
